@@ -592,4 +592,210 @@ int mnemo_moe_decode_rmsnorm_noalloc(const float *router_w, const void *experts,
                                      norm_w, eps, hidden, eff, n_experts, k, out, topk_idx, topk_w, s);
 }
 
+// ------------------------------------------------------------------ paged cache
+static int check_pages(const char *what, const KvPagesArgs &a) {
+    if (!a.table || !a.lens || !a.refs) return set_error(kErrBadArg, "%s: NULL block table, lengths or references", what);
+    if (a.n_seqs <= 0 || a.n_seqs > kMaxSeqs || a.max_pages <= 0 || a.n_pages <= 0)
+        return set_error(kErrBadArg, "%s: need 1 <= n_seqs <= %d, max_pages > 0 and n_pages > 0", what, kMaxSeqs);
+    if (a.ps != 16 && a.ps != 32 && a.ps != 64 && a.ps != 128)
+        return set_error(kErrBadArg, "%s: page_size %d (16, 32, 64, 128)", what, a.ps);
+    if ((long long)a.max_pages * a.ps > INT_MAX || (long long)a.n_seqs * a.max_pages > INT_MAX)
+        return set_error(kErrBadArg, "%s: max_pages * page_size and n_seqs * max_pages must be below 2^31", what);
+    return 0;
+}
+
+static int check_cache(const char *what, const PagedCache &c) {
+    if (c.kv_type != kKvF16 && c.kv_type != kKvInt8) return set_error(kErrBadArg, "%s: kv_type %d", what, c.kv_type);
+    if (!c.k || !c.v || (c.kv_type == kKvInt8 && (!c.ksc || !c.vsc)))
+        return set_error(kErrBadArg, "%s: NULL cache or scales", what);
+    if (c.hd != 64 && c.hd != 128 && c.hd != 256)
+        return set_error(kErrBadArg, "%s: head_dim %d (64, 128, 256)", what, c.hd);
+    if (c.ps != 16 && c.ps != 32 && c.ps != 64 && c.ps != 128)
+        return set_error(kErrBadArg, "%s: page_size %d (16, 32, 64, 128)", what, c.ps);
+    if (c.nkv <= 0 || c.nkv > 4096 || c.n_pages <= 0)
+        return set_error(kErrBadArg, "%s: need 1 <= n_kv_heads <= 4096 and n_pages > 0", what);
+    if (((uintptr_t)c.k | (uintptr_t)c.v | (c.kv_type == kKvInt8 ? (uintptr_t)c.ksc | (uintptr_t)c.vsc : 0)) % 16)
+        return set_error(kErrBadArg, "%s: pages and scales must be 16-byte aligned", what);
+    return 0;
+}
+
+size_t mnemo_paged_cache_bytes(int n_pages, int page_size, int n_kv_heads, int head_dim, int kv_type) {
+    if (n_pages <= 0 || page_size <= 0 || n_kv_heads <= 0 || head_dim <= 0) return 0;
+    return (size_t)n_pages * page_size * n_kv_heads * head_dim * (kv_type == kKvInt8 ? 1 : 2);
+}
+
+int mnemo_paged_attn_prep(const float *q, const float *k, const float *v, const float *q_norm_w, const float *k_norm_w,
+                          float eps, float theta, int n_tokens, int n_heads, int head_dim, int n_kv_heads,
+                          const int *positions, const int *seq_ids, const int *block_table, const int *seq_lens,
+                          int n_seqs, int max_pages, void *k_pages, void *v_pages, float *k_scales, float *v_scales,
+                          int kv_type, int n_pages, int page_size, float *q_out, hipStream_t s) {
+    const char *what = "paged_attn_prep";
+    PagedPrepArgs a = {};
+    a.c = {k_pages, v_pages, k_scales, v_scales, kv_type, n_pages, page_size, n_kv_heads, head_dim};
+    if (int rc = check_cache(what, a.c)) return rc;
+    if ((q_norm_w == nullptr) != (k_norm_w == nullptr))
+        return set_error(kErrBadArg, "%s: give both QK-norm weights or neither", what);
+    if (n_seqs <= 0 || n_seqs > kMaxSeqs || max_pages <= 0 || (long long)max_pages * page_size > INT_MAX)
+        return set_error(kErrBadArg, "%s: need 1 <= n_seqs <= %d and 1 <= max_pages * page_size < 2^31", what, kMaxSeqs);
+    if (n_heads <= 0 || n_heads > 65536) return set_error(kErrBadArg, "%s: n_heads must be in 1..65536", what);
+    if (!(theta > 0.0f)) return set_error(kErrBadArg, "%s: theta must be positive", what);
+    if (n_tokens == 0) return kOk;
+    if (n_tokens < 0 || n_tokens > 1 << 22)
+        return set_error(kErrBadArg, "%s: n_tokens must be in 0..%d", what, 1 << 22);
+    if (!q || !k || !v || !q_out || !block_table) return set_error(kErrBadArg, "%s: NULL pointer", what);
+    if ((positions == nullptr) != (seq_ids == nullptr) || (!positions && (!seq_lens || n_tokens > n_seqs)))
+        return set_error(kErrBadArg, "%s: give positions and seq_ids, or neither, seq_lens and n_tokens <= n_seqs",
+                         what);
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.qw = q_norm_w;
+    a.kw = k_norm_w;
+    a.q_out = q_out;
+    a.table = block_table;
+    a.lens = seq_lens;
+    a.pos = positions;
+    a.seq = seq_ids;
+    a.n_tokens = n_tokens;
+    a.n_seqs = n_seqs;
+    a.max_pages = max_pages;
+    a.nh = n_heads;
+    a.eps = eps;
+    return launch_paged_prep(a, theta, s);
+}
+
+size_t mnemo_paged_attention_workspace_bytes(int n_heads, int n_kv_heads, int head_dim) {
+    return n_heads > 0 && n_kv_heads > 0 && head_dim > 0 ? paged_attn_workspace_bytes(n_kv_heads, head_dim) : 0;
+}
+
+int mnemo_paged_attention_decode(const float *q, const void *k_pages, const void *v_pages, const float *k_scales,
+                                 const float *v_scales, int kv_type, float *out, int n_seqs, int n_heads, int head_dim,
+                                 int n_kv_heads, int n_pages, int page_size, const int *block_table, int max_pages,
+                                 const int *seq_lens, float scale, void *workspace, size_t workspace_bytes,
+                                 hipStream_t s) {
+    const char *what = "paged_attention_decode";
+    PagedAttnArgs a = {};
+    a.c = {(void *)k_pages, (void *)v_pages, (float *)k_scales, (float *)v_scales, kv_type, n_pages, page_size,
+           n_kv_heads, head_dim};
+    if (int rc = check_cache(what, a.c)) return rc;
+    if (!q || !out || !block_table || !seq_lens || !workspace) return set_error(kErrBadArg, "%s: NULL pointer", what);
+    if (n_heads <= 0 || n_heads % n_kv_heads || n_heads / n_kv_heads > 16)
+        return set_error(kErrBadArg, "%s: n_heads must be 1 to 16 times n_kv_heads", what);
+    if (n_seqs <= 0 || n_seqs > kMaxSeqs || max_pages <= 0 || (long long)max_pages * page_size > INT_MAX)
+        return set_error(kErrBadArg, "%s: need 1 <= n_seqs <= %d and 1 <= max_pages * page_size < 2^31", what, kMaxSeqs);
+    if ((uintptr_t)workspace % 16 || workspace_bytes < paged_attn_workspace_bytes(n_kv_heads, head_dim))
+        return set_error(kErrBadArg, "%s: workspace not 16-byte aligned, or %zu < %zu bytes", what, workspace_bytes,
+                         paged_attn_workspace_bytes(n_kv_heads, head_dim));
+    a.q = q;
+    a.out = out;
+    a.table = block_table;
+    a.lens = seq_lens;
+    a.n_seqs = n_seqs;
+    a.max_pages = max_pages;
+    a.nh = n_heads;
+    a.gqa = n_heads / n_kv_heads;
+    a.scale = scale;
+    a.ws = (float *)workspace;
+    a.ws_bytes = workspace_bytes;
+    return launch_paged_attention(a, s);
+}
+
+size_t mnemo_kv_pages_workspace_bytes(int n_seqs, int n_pages) {
+    return n_seqs > 0 && n_pages > 0 ? kv_pages_workspace_bytes(n_seqs, n_pages) : 0;
+}
+
+int mnemo_kv_pages_extend(int *block_table, int *seq_lens, int *page_refs, const int *new_lens, int n_seqs,
+                          int max_pages, int n_pages, int page_size, int *status, hipStream_t s) {
+    const KvPagesArgs a = {block_table, seq_lens, page_refs, n_seqs, max_pages, n_pages, page_size};
+    if (int rc = check_pages("kv_pages_extend", a)) return rc;
+    if (!new_lens) return set_error(kErrBadArg, "kv_pages_extend: new_lens is NULL");
+    return launch_kv_extend(a, new_lens, status, s);
+}
+
+int mnemo_kv_pages_free(int *block_table, int *seq_lens, int *page_refs, const int *gone, int n_seqs, int max_pages,
+                        int n_pages, int page_size, hipStream_t s) {
+    const KvPagesArgs a = {block_table, seq_lens, page_refs, n_seqs, max_pages, n_pages, page_size};
+    if (int rc = check_pages("kv_pages_free", a)) return rc;
+    if (!gone) return set_error(kErrBadArg, "kv_pages_free: gone is NULL");
+    return launch_kv_free(a, gone, s);
+}
+
+static int check_moving(const char *what, const PagedCache &c, int n_layers, const void *ws, size_t ws_bytes,
+                        size_t need) {
+    if (int rc = check_cache(what, c)) return rc;
+    if (n_layers <= 0) return set_error(kErrBadArg, "%s: need n_layers > 0", what);
+    if (need && (!ws || (uintptr_t)ws % 16 || ws_bytes < need))
+        return set_error(kErrBadArg, "%s: workspace NULL, not 16-byte aligned, or %zu < %zu bytes", what, ws_bytes,
+                         need);
+    return 0;
+}
+
+int mnemo_kv_pages_fork(int *block_table, int *seq_lens, int *page_refs, const int *parents, int n_seqs, int max_pages,
+                        void *k_pages, void *v_pages, float *k_scales, float *v_scales, int kv_type, int n_layers,
+                        int n_pages, int page_size, int n_kv_heads, int head_dim, int *status, void *workspace,
+                        size_t workspace_bytes, hipStream_t s) {
+    const KvPagesArgs a = {block_table, seq_lens, page_refs, n_seqs, max_pages, n_pages, page_size};
+    const PagedCache c = {k_pages, v_pages, k_scales, v_scales, kv_type, n_pages, page_size, n_kv_heads, head_dim};
+    if (int rc = check_pages("kv_pages_fork", a)) return rc;
+    if (!parents) return set_error(kErrBadArg, "kv_pages_fork: parents is NULL");
+    if (int rc = check_moving("kv_pages_fork", c, n_layers, workspace, workspace_bytes,
+                              kv_pages_workspace_bytes(n_seqs, n_pages)))
+        return rc;
+    return launch_kv_fork(a, c, n_layers, parents, status, (int *)workspace, s);
+}
+
+int mnemo_kv_pages_compact(int *block_table, int *page_refs, int n_seqs, int max_pages, void *k_pages, void *v_pages,
+                           float *k_scales, float *v_scales, int kv_type, int n_layers, int n_pages, int page_size,
+                           int n_kv_heads, int head_dim, int *n_live, void *workspace, size_t workspace_bytes,
+                           hipStream_t s) {
+    // compaction needs no lengths: every table entry at n or above is renamed
+    const KvPagesArgs a = {block_table, block_table, page_refs, n_seqs, max_pages, n_pages, page_size};
+    const PagedCache c = {k_pages, v_pages, k_scales, v_scales, kv_type, n_pages, page_size, n_kv_heads, head_dim};
+    if (int rc = check_pages("kv_pages_compact", a)) return rc;
+    if (int rc = check_moving("kv_pages_compact", c, n_layers, workspace, workspace_bytes,
+                              kv_pages_workspace_bytes(n_seqs, n_pages)))
+        return rc;
+    return launch_kv_compact(a, c, n_layers, n_live, (int *)workspace, s);
+}
+
+int mnemo_kv_pages_copy(const int *src, const int *dst, int n, void *k_pages, void *v_pages, float *k_scales,
+                        float *v_scales, int kv_type, int n_layers, int n_pages, int page_size, int n_kv_heads,
+                        int head_dim, hipStream_t s) {
+    const PagedCache c = {k_pages, v_pages, k_scales, v_scales, kv_type, n_pages, page_size, n_kv_heads, head_dim};
+    if (int rc = check_moving("kv_pages_copy", c, n_layers, nullptr, 0, 0)) return rc;
+    if (n < 0 || (n > 0 && (!src || !dst))) return set_error(kErrBadArg, "kv_pages_copy: n < 0, or src or dst NULL");
+    return launch_kv_copy(c, n_layers, src, dst, n, s);
+}
+
+// ------------------------------------------------------------------ logits
+int mnemo_logits_process(const float *logits, float *out, int n_rows, int vocab, const int *history,
+                         const int *history_lens, const int *prompt_lens, int max_history, const float *repetition,
+                         const float *frequency, const float *presence, const int *bias_ids, const float *bias,
+                         int n_bias, const unsigned *allowed, hipStream_t s) {
+    if (n_rows < 0 || n_rows > 65535 || vocab <= 0)
+        return set_error(kErrBadArg, "logits_process: need 0 <= n_rows <= 65535 and vocab > 0");
+    if (history && (!history_lens || !prompt_lens || !repetition || !frequency || !presence || max_history < 0))
+        return set_error(kErrBadArg, "logits_process: a history needs its lengths and the three penalties");
+    if (bias_ids && (!bias || n_bias < 0)) return set_error(kErrBadArg, "logits_process: bias_ids needs bias");
+    if (n_rows == 0) return kOk;
+    if (!logits || !out) return set_error(kErrBadArg, "logits_process: logits or out is NULL");
+    LogitsArgs a = {};
+    a.z = logits;
+    a.out = out;
+    a.n_rows = n_rows;
+    a.vocab = vocab;
+    a.hist = history;
+    a.hist_len = history_lens;
+    a.prompt_len = prompt_lens;
+    a.max_hist = max_history;
+    a.rep = repetition;
+    a.freq = frequency;
+    a.pres = presence;
+    a.bias_ids = bias_ids;
+    a.bias = bias;
+    a.n_bias = n_bias;
+    a.allowed = allowed;
+    return launch_logits_process(a, s);
+}
+
 }  // extern "C"

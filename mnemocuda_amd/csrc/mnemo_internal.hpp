@@ -183,6 +183,69 @@ int launch_f32_to_f16_dual(const float *a, const float *b, void *oa, void *ob, i
 int launch_head_pass(HeadPassArgs a, hipStream_t s);
 int launch_attention(AttnArgs a, int kv_type, hipStream_t s);
 
+// ---- several sequences in one paged cache (paged_attn.hip, kv_pages.hip)
+// K pages [page][nkv][ps][hd], V pages [page][nkv][hd][ps], int8 scales [page][nkv][ps]; row s of
+// the block table names the pages of sequence s in order.
+constexpr int kMaxSeqs = 4096;  // rows of a block table
+
+struct PagedCache {
+    void *k, *v;
+    float *ksc, *vsc;
+    int kv_type, n_pages, ps, nkv, hd;
+};
+
+struct PagedAttnArgs {
+    const float *q;
+    float *out;
+    PagedCache c;
+    const int *table, *lens;
+    int n_seqs, max_pages, nh, gqa;
+    float scale;
+    float *ws;
+    size_t ws_bytes;
+};
+size_t paged_attn_workspace_bytes(int nkv, int hd);
+int launch_paged_attention(const PagedAttnArgs &a, hipStream_t s);
+
+struct PagedPrepArgs {
+    const float *q, *k, *v;  // [n_tokens][nh | nkv][hd]
+    const float *qw, *kw;    // QK-norm weights [hd], or both NULL
+    float *q_out;
+    PagedCache c;
+    const int *table, *lens;
+    const int *pos, *seq;  // of each token; both NULL: token t is position lens[t] - 1 of sequence t
+    int n_tokens, n_seqs, max_pages, nh;
+    float eps;
+    uint64_t turn[128];  // theta^(-2j/hd) / (2 pi) in units of 2^-64
+};
+int launch_paged_prep(PagedPrepArgs &a, double theta, hipStream_t s);
+
+struct KvPagesArgs {
+    int *table, *lens, *refs;
+    int n_seqs, max_pages, n_pages, ps;
+};
+int launch_kv_extend(const KvPagesArgs &a, const int *new_lens, int *status, hipStream_t s);
+int launch_kv_free(const KvPagesArgs &a, const int *gone, hipStream_t s);
+int launch_kv_fork(const KvPagesArgs &a, const PagedCache &c, int n_layers, const int *parents, int *status, int *ws,
+                   hipStream_t s);
+int launch_kv_compact(const KvPagesArgs &a, const PagedCache &c, int n_layers, int *n_live, int *ws, hipStream_t s);
+int launch_kv_copy(const PagedCache &c, int n_layers, const int *src, const int *dst, int n, hipStream_t s);
+size_t kv_pages_workspace_bytes(int n_seqs, int n_pages);
+
+struct LogitsArgs {
+    const float *z;
+    float *out;
+    int n_rows, vocab;
+    const int *hist, *hist_len, *prompt_len;  // [n_rows][max_hist], [n_rows], [n_rows]; hist NULL: no penalties
+    int max_hist;
+    const float *rep, *freq, *pres;  // [n_rows]
+    const int *bias_ids;             // [n_rows][n_bias], or NULL
+    const float *bias;
+    int n_bias;
+    const uint32_t *allowed;  // [n_rows][ceil(vocab / 32)], or NULL
+};
+int launch_logits_process(const LogitsArgs &a, hipStream_t s);
+
 // Records (and prints, as the reference's KERNEL_LAUNCH_CHECK does, kernels.cu:1062-1067)
 // the error of the last launch; returns a kErr code.
 int check_launch(const char *what);

@@ -77,6 +77,22 @@ SIGNATURES: dict[str, tuple] = {
                                           i32, ip, f32, vp, sz, stream_t]),
     "cuda_embedding_lookup_q4k": (None, [vp, fp, i32, i32, i32, stream_t]),
     "mnemo_embedding_lookup": (i32, [vp, i32, ip, i32, fp, i32, stream_t]),
+    # paged cache and logits of several sequences
+    "mnemo_paged_cache_bytes": (sz, [i32, i32, i32, i32, i32]),
+    "mnemo_paged_attn_prep": (i32, [fp, fp, fp, fp, fp, f32, f32, i32, i32, i32, i32, ip, ip, ip, ip, i32, i32, vp, vp,
+                                    fp, fp, i32, i32, i32, fp, stream_t]),
+    "mnemo_paged_attention_workspace_bytes": (sz, [i32, i32, i32]),
+    "mnemo_paged_attention_decode": (i32, [fp, vp, vp, fp, fp, i32, fp, i32, i32, i32, i32, i32, i32, ip, i32, ip, f32,
+                                           vp, sz, stream_t]),
+    "mnemo_kv_pages_extend": (i32, [ip, ip, ip, ip, i32, i32, i32, i32, ip, stream_t]),
+    "mnemo_kv_pages_free": (i32, [ip, ip, ip, ip, i32, i32, i32, i32, stream_t]),
+    "mnemo_kv_pages_workspace_bytes": (sz, [i32, i32]),
+    "mnemo_kv_pages_fork": (i32, [ip, ip, ip, ip, i32, i32, vp, vp, fp, fp, i32, i32, i32, i32, i32, i32, ip, vp, sz,
+                                  stream_t]),
+    "mnemo_kv_pages_compact": (i32, [ip, ip, i32, i32, vp, vp, fp, fp, i32, i32, i32, i32, i32, i32, ip, vp, sz,
+                                     stream_t]),
+    "mnemo_kv_pages_copy": (i32, [ip, ip, i32, vp, vp, fp, fp, i32, i32, i32, i32, i32, i32, stream_t]),
+    "mnemo_logits_process": (i32, [fp, fp, i32, i32, ip, ip, ip, i32, fp, fp, fp, ip, fp, i32, vp, stream_t]),
     # model directory (mnemo_model.h); structs travel as void*
     "mnemo_parse_config": (i32, [C.c_char_p, vp]),
     "mnemo_parse_resident_manifest": (i32, [C.c_char_p, vp, i32, vp]),

@@ -476,3 +476,185 @@ def embedding_lookup_q4k(table, out, token_id: int, hidden: int, row_bytes: int)
     tp = table if isinstance(table, int) else _dev(table, "table")
     lib.cuda_embedding_lookup_q4k(tp, _dev(out, "out", F32), int(token_id), int(hidden), int(row_bytes), _stream())
     check(lib, "cuda_embedding_lookup_q4k")
+
+
+# ---------------------------------------------------------------- several sequences in one paged cache
+I32 = torch.int32
+
+
+def paged_cache_bytes(n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, kv_type: int) -> int:
+    return int(load_library().mnemo_paged_cache_bytes(n_pages, page_size, n_kv_heads, head_dim, kv_type))
+
+
+def _need(t, n: int, name: str) -> None:
+    if t.numel() < n:
+        raise MnemoError(f"{name}: {t.numel()} elements < {n}")
+
+
+def _pages(k, v, ks, vs, layers: bool):
+    """The arguments (pointers, kv_type) and shape (n_layers, n_pages, n_kv_heads, page_size, head_dim) of cache
+    pages k [..., n_kv_heads, page_size, head_dim] and v [..., n_kv_heads, head_dim, page_size]."""
+    nd = 5 if layers else 4
+    if k.dtype not in (torch.float16, torch.int8) or v.dtype != k.dtype:
+        raise MnemoError(f"pages must be float16 or int8, got {k.dtype} and {v.dtype}")
+    if k.dim() != nd or tuple(v.shape) != (*k.shape[:-2], k.shape[-1], k.shape[-2]):
+        raise MnemoError(f"pages: k {tuple(k.shape)} and v {tuple(v.shape)} do not fit ({nd} dimensions, v transposed)")
+    kv_type = int(k.dtype == torch.int8)
+    if kv_type:
+        if ks is None or vs is None:
+            raise MnemoError("int8 pages need scales")
+        _need(ks, k.numel() // k.shape[-1], "k_scales")
+        _need(vs, k.numel() // k.shape[-1], "v_scales")
+    n_layers = k.shape[0] if layers else 1
+    ptrs = (_dev(k, "k_pages"), _dev(v, "v_pages"), _opt(ks if kv_type else None, "k_scales", F32),
+            _opt(vs if kv_type else None, "v_scales", F32), kv_type)
+    return ptrs, (n_layers, *k.shape[-4:])
+
+
+def _rows(table, *per_row):
+    """(n_seqs, max_pages) of a block table; per_row: (tensor, name) with one int32 per row."""
+    if table.dim() != 2:
+        raise MnemoError(f"block_table must have 2 dimensions, got {table.dim()}")
+    for t, name in per_row:
+        _dev(t, name, I32)
+        _need(t, table.shape[0], name)
+    return table.shape
+
+
+def paged_attn_prep(q, k, v, qw, kw, eps: float, theta: float, k_pages, v_pages, block_table, q_out, positions=None,
+                    seq_ids=None, ks=None, vs=None, seq_lens=None):
+    """QK norm (when qw/kw are given) + RoPE of the new tokens q [T, n_heads, head_dim] (into q_out, which may be q)
+    and k [T, n_kv_heads, head_dim], and the store of k and v into the pages.  Token t is position positions[t] of
+    row seq_ids[t] of the block table; without them it is the last position of row t (seq_lens[t] - 1)."""
+    lib = load_library()
+    ptrs, (_, n_pages, nkv, ps, hd) = _pages(k_pages, v_pages, ks, vs, False)
+    n_seqs, max_pages = _rows(block_table, *(((seq_lens, "seq_lens"),) if seq_lens is not None else ()))
+    T, nh = q.shape[0], q.shape[1]
+    if tuple(q.shape) != (T, nh, hd) or tuple(k.shape) != (T, nkv, hd) or v.shape != k.shape or q_out.shape != q.shape:
+        raise MnemoError("paged_attn_prep: q, k, v and q_out must be [T, heads, head_dim]")
+    for t, name in ((positions, "positions"), (seq_ids, "seq_ids")):
+        if t is not None:
+            _need(t, T, name)
+    for t, name in ((qw, "qw"), (kw, "kw")):
+        if t is not None:
+            _need(t, hd, name)
+    rc = lib.mnemo_paged_attn_prep(
+        _dev(q, "q", F32), _dev(k, "k", F32), _dev(v, "v", F32), _opt(qw, "qw", F32), _opt(kw, "kw", F32), float(eps),
+        float(theta), T, nh, hd, nkv, _opt(positions, "positions", I32), _opt(seq_ids, "seq_ids", I32),
+        _dev(block_table, "block_table", I32), _opt(seq_lens, "seq_lens", I32), n_seqs, max_pages, *ptrs, n_pages, ps,
+        _dev(q_out, "q_out", F32), _stream())
+    _check_rc(lib, rc, "mnemo_paged_attn_prep")
+
+
+def paged_attention_workspace_bytes(n_heads: int, n_kv_heads: int, head_dim: int) -> int:
+    return int(load_library().mnemo_paged_attention_workspace_bytes(n_heads, n_kv_heads, head_dim))
+
+
+def paged_attention_decode(q, k_pages, v_pages, block_table, seq_lens, out, scale: float, ws, ks=None, vs=None):
+    """out[s] = attention of q[s] [n_heads, head_dim] over the positions 0..seq_lens[s]-1 that row s of the block
+    table holds (zeros for an empty row)."""
+    lib = load_library()
+    ptrs, (_, n_pages, nkv, ps, hd) = _pages(k_pages, v_pages, ks, vs, False)
+    n_seqs, max_pages = _rows(block_table, (seq_lens, "seq_lens"))
+    if q.dim() != 3 or q.shape[0] != n_seqs or q.shape[2] != hd or out.shape != q.shape:
+        raise MnemoError("paged_attention_decode: q and out must be [n_seqs, n_heads, head_dim]")
+    rc = lib.mnemo_paged_attention_decode(
+        _dev(q, "q", F32), *ptrs, _dev(out, "out", F32), n_seqs, q.shape[1], hd, nkv, n_pages, ps,
+        _dev(block_table, "block_table", I32), max_pages, seq_lens.data_ptr(), float(scale), _dev(ws, "ws"),
+        ws.numel() * ws.element_size(), _stream())
+    _check_rc(lib, rc, "mnemo_paged_attention_decode")
+
+
+def kv_pages_extend(block_table, seq_lens, page_refs, new_lens, page_size: int, status=None):
+    """Gives pages to every row with new_lens > seq_lens; status[0] = rows that could not be served."""
+    lib = load_library()
+    n_seqs, max_pages = _rows(block_table, (seq_lens, "seq_lens"), (new_lens, "new_lens"))
+    rc = lib.mnemo_kv_pages_extend(_dev(block_table, "block_table", I32), seq_lens.data_ptr(),
+                                   _dev(page_refs, "page_refs", I32), new_lens.data_ptr(), n_seqs, max_pages,
+                                   page_refs.numel(), int(page_size), _opt(status, "status", I32), _stream())
+    _check_rc(lib, rc, "mnemo_kv_pages_extend")
+
+
+def kv_pages_free(block_table, seq_lens, page_refs, gone, page_size: int):
+    """Drops the pages of every row with gone != 0."""
+    lib = load_library()
+    n_seqs, max_pages = _rows(block_table, (seq_lens, "seq_lens"), (gone, "gone"))
+    rc = lib.mnemo_kv_pages_free(_dev(block_table, "block_table", I32), seq_lens.data_ptr(),
+                                 _dev(page_refs, "page_refs", I32), gone.data_ptr(), n_seqs, max_pages,
+                                 page_refs.numel(), int(page_size), _stream())
+    _check_rc(lib, rc, "mnemo_kv_pages_free")
+
+
+def kv_pages_workspace_bytes(n_seqs: int, n_pages: int) -> int:
+    return int(load_library().mnemo_kv_pages_workspace_bytes(n_seqs, n_pages))
+
+
+def kv_pages_fork(block_table, seq_lens, page_refs, parents, k_pages, v_pages, status, ws, ks=None, vs=None):
+    """Every empty row with parents >= 0 becomes a copy of that row: full pages shared, a partly filled last page
+    copied in all layers of k_pages / v_pages [n_layers, n_pages, ...]; status[0] = rows that could not be served."""
+    lib = load_library()
+    ptrs, (n_layers, n_pages, nkv, ps, hd) = _pages(k_pages, v_pages, ks, vs, True)
+    n_seqs, max_pages = _rows(block_table, (seq_lens, "seq_lens"), (parents, "parents"))
+    _need(page_refs, n_pages, "page_refs")
+    rc = lib.mnemo_kv_pages_fork(_dev(block_table, "block_table", I32), seq_lens.data_ptr(),
+                                 _dev(page_refs, "page_refs", I32), parents.data_ptr(), n_seqs, max_pages, *ptrs,
+                                 n_layers, n_pages, ps, nkv, hd, _opt(status, "status", I32), _dev(ws, "ws"),
+                                 ws.numel() * ws.element_size(), _stream())
+    _check_rc(lib, rc, "mnemo_kv_pages_fork")
+
+
+def kv_pages_compact(block_table, page_refs, k_pages, v_pages, n_live, ws, ks=None, vs=None):
+    """Moves the pages in use to the front of the pool, in all layers; n_live[0] = their number."""
+    lib = load_library()
+    ptrs, (n_layers, n_pages, nkv, ps, hd) = _pages(k_pages, v_pages, ks, vs, True)
+    n_seqs, max_pages = _rows(block_table)
+    _need(page_refs, n_pages, "page_refs")
+    rc = lib.mnemo_kv_pages_compact(_dev(block_table, "block_table", I32), _dev(page_refs, "page_refs", I32), n_seqs,
+                                    max_pages, *ptrs, n_layers, n_pages, ps, nkv, hd, _opt(n_live, "n_live", I32),
+                                    _dev(ws, "ws"), ws.numel() * ws.element_size(), _stream())
+    _check_rc(lib, rc, "mnemo_kv_pages_compact")
+
+
+def kv_pages_copy(src, dst, k_pages, v_pages, ks=None, vs=None):
+    """Copies page src[i] to page dst[i] in all layers (int32 device tensors; destinations distinct, no source)."""
+    lib = load_library()
+    ptrs, (n_layers, n_pages, nkv, ps, hd) = _pages(k_pages, v_pages, ks, vs, True)
+    if src.numel() != dst.numel():
+        raise MnemoError("kv_pages_copy: src and dst differ in length")
+    rc = lib.mnemo_kv_pages_copy(_dev(src, "src", I32), _dev(dst, "dst", I32), src.numel(), *ptrs, n_layers, n_pages,
+                                 ps, nkv, hd, _stream())
+    _check_rc(lib, rc, "mnemo_kv_pages_copy")
+
+
+# ---------------------------------------------------------------- logits before sampling
+def logits_process(logits, out, history=None, history_lens=None, prompt_lens=None, repetition=None, frequency=None,
+                   presence=None, bias_ids=None, bias=None, allowed=None):
+    """Repetition, frequency and presence penalties over each row's history [n, max_history], biases of single
+    tokens [n, n_bias] and a mask of allowed tokens (int32 bit words [n, ceil(vocab / 32)]) applied to
+    logits [n, vocab] into out (which may be logits)."""
+    lib = load_library()
+    if logits.dim() != 2 or out.shape != logits.shape:
+        raise MnemoError("logits_process: logits and out must be [n, vocab]")
+    n, vocab = logits.shape
+    max_history = n_bias = 0
+    if history is not None:
+        if history.dim() != 2 or history.shape[0] != n:
+            raise MnemoError("logits_process: history must be [n, max_history]")
+        max_history = history.shape[1]
+        for t, name in ((history_lens, "history_lens"), (prompt_lens, "prompt_lens"), (repetition, "repetition"),
+                        (frequency, "frequency"), (presence, "presence")):
+            if t is None:
+                raise MnemoError(f"logits_process: history needs {name}")
+            _need(t, n, name)
+    if bias_ids is not None:
+        if bias is None or bias_ids.dim() != 2 or bias_ids.shape[0] != n or bias.shape != bias_ids.shape:
+            raise MnemoError("logits_process: bias_ids and bias must be [n, n_bias]")
+        n_bias = bias_ids.shape[1]
+    if allowed is not None:
+        _need(allowed, n * ((vocab + 31) // 32), "allowed")
+    rc = lib.mnemo_logits_process(
+        _dev(logits, "logits", F32), _dev(out, "out", F32), n, vocab, _opt(history, "history", I32),
+        _opt(history_lens, "history_lens", I32), _opt(prompt_lens, "prompt_lens", I32), max_history,
+        _opt(repetition, "repetition", F32), _opt(frequency, "frequency", F32), _opt(presence, "presence", F32),
+        _opt(bias_ids, "bias_ids", I32), _opt(bias, "bias", F32), n_bias, _opt(allowed, "allowed", I32), _stream())
+    _check_rc(lib, rc, "mnemo_logits_process")
