@@ -357,7 +357,7 @@ int mnemo_attention_decode_prep(const float *q, const float *k, const float *v,
  * kv_type 0 f16, 1 int8; head_dim 64, 128 or 256; all four arrays 16-byte aligned.
  * block_table [n_seqs][max_pages]: row s lists the pages of sequence s in order, position p is
  * at entry p / page_size, row p % page_size.  seq_lens [n_seqs]: positions held; a row with
- * length 0 is empty.  n_seqs <= 4096, max_pages * page_size and n_seqs * max_pages < 2^31.
+ * length 0 is empty.  n_seqs <= 4096, max_pages * page_size and n_seqs * max_pages <= 2^30.
  * Table, lengths and ids live in device memory and are read by the kernels, so that captured
  * graphs serve every step.  A page id outside 0..n_pages-1 is never followed: attention takes
  * its positions as absent, stores and copies to it are dropped. */
@@ -382,7 +382,7 @@ int mnemo_paged_attn_prep(const float *q, const float *k, const float *v, const 
 /* Attention of one new token per sequence, n_heads = gqa * n_kv_heads with gqa <= 16:
  * out[s][h] = softmax_p(scale q[s][h] . k_p) v_p over the positions p < seq_lens[s] (at most
  * max_pages * page_size), q and out [n_seqs][n_heads][head_dim] fp32.  A sequence with no
- * positions gets zeros.  workspace: mnemo_paged_attention_workspace_bytes(...) bytes, 16-byte
+ * positions gets zeros.  n_seqs * n_kv_heads * max_pages * page_size < 2^38.  workspace: mnemo_paged_attention_workspace_bytes(...) bytes, 16-byte
  * aligned, no initialisation; calls sharing it must not overlap. */
 size_t mnemo_paged_attention_workspace_bytes(int n_heads, int n_kv_heads, int head_dim);
 int mnemo_paged_attention_decode(const float *q, const void *k_pages, const void *v_pages,

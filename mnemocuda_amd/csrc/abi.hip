@@ -599,8 +599,8 @@ static int check_pages(const char *what, const KvPagesArgs &a) {
         return set_error(kErrBadArg, "%s: need 1 <= n_seqs <= %d, max_pages > 0 and n_pages > 0", what, kMaxSeqs);
     if (a.ps != 16 && a.ps != 32 && a.ps != 64 && a.ps != 128)
         return set_error(kErrBadArg, "%s: page_size %d (16, 32, 64, 128)", what, a.ps);
-    if ((long long)a.max_pages * a.ps > INT_MAX || (long long)a.n_seqs * a.max_pages > INT_MAX)
-        return set_error(kErrBadArg, "%s: max_pages * page_size and n_seqs * max_pages must be below 2^31", what);
+    if ((long long)a.max_pages * a.ps > 1 << 30 || (long long)a.n_seqs * a.max_pages > 1 << 30)
+        return set_error(kErrBadArg, "%s: max_pages * page_size and n_seqs * max_pages must be at most 2^30", what);
     return 0;
 }
 
@@ -635,8 +635,8 @@ int mnemo_paged_attn_prep(const float *q, const float *k, const float *v, const 
     if (int rc = check_cache(what, a.c)) return rc;
     if ((q_norm_w == nullptr) != (k_norm_w == nullptr))
         return set_error(kErrBadArg, "%s: give both QK-norm weights or neither", what);
-    if (n_seqs <= 0 || n_seqs > kMaxSeqs || max_pages <= 0 || (long long)max_pages * page_size > INT_MAX)
-        return set_error(kErrBadArg, "%s: need 1 <= n_seqs <= %d and 1 <= max_pages * page_size < 2^31", what, kMaxSeqs);
+    if (n_seqs <= 0 || n_seqs > kMaxSeqs || max_pages <= 0 || (long long)max_pages * page_size > 1 << 30)
+        return set_error(kErrBadArg, "%s: need 1 <= n_seqs <= %d and 1 <= max_pages * page_size <= 2^30", what, kMaxSeqs);
     if (n_heads <= 0 || n_heads > 65536) return set_error(kErrBadArg, "%s: n_heads must be in 1..65536", what);
     if (!(theta > 0.0f)) return set_error(kErrBadArg, "%s: theta must be positive", what);
     if (n_tokens == 0) return kOk;
@@ -681,8 +681,10 @@ int mnemo_paged_attention_decode(const float *q, const void *k_pages, const void
     if (!q || !out || !block_table || !seq_lens || !workspace) return set_error(kErrBadArg, "%s: NULL pointer", what);
     if (n_heads <= 0 || n_heads % n_kv_heads || n_heads / n_kv_heads > 16)
         return set_error(kErrBadArg, "%s: n_heads must be 1 to 16 times n_kv_heads", what);
-    if (n_seqs <= 0 || n_seqs > kMaxSeqs || max_pages <= 0 || (long long)max_pages * page_size > INT_MAX)
-        return set_error(kErrBadArg, "%s: need 1 <= n_seqs <= %d and 1 <= max_pages * page_size < 2^31", what, kMaxSeqs);
+    if (n_seqs <= 0 || n_seqs > kMaxSeqs || max_pages <= 0 || (long long)max_pages * page_size > 1 << 30)
+        return set_error(kErrBadArg, "%s: need 1 <= n_seqs <= %d and 1 <= max_pages * page_size <= 2^30", what, kMaxSeqs);
+    if ((long long)n_seqs * n_kv_heads * max_pages * page_size >= 1LL << 38)
+        return set_error(kErrBadArg, "%s: n_seqs * n_kv_heads * max_pages * page_size must be below 2^38", what);
     if ((uintptr_t)workspace % 16 || workspace_bytes < paged_attn_workspace_bytes(n_kv_heads, head_dim))
         return set_error(kErrBadArg, "%s: workspace not 16-byte aligned, or %zu < %zu bytes", what, workspace_bytes,
                          paged_attn_workspace_bytes(n_kv_heads, head_dim));
