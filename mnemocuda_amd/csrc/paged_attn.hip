@@ -13,18 +13,18 @@ namespace mnemo {
 // ------------------------------------------------------------------ attention
 // out[s][h] = sum_p P_p v_p / sum_p P_p,  P_p = exp(scale q.k_p - m), over the positions of row s.
 //
-// The work is cut into units of kUnit positions of one (sequence, KV head), in that order, and the
-// workgroups take equal shares of the row of units, whatever the lengths are: every workgroup
+// The work is cut into steps of kStep positions of one (sequence, KV head), in that order, and the
+// waves of the launch take equal shares of the row of steps, whatever the lengths are: every wave
 // computes its share from the lengths itself.  A (sequence, KV head) that lies within one share
-// is finished there; one that several shares cut leaves a partial (max, sum, O) in each, which a
-// second launch merges.
+// is finished there; pieces of one that several shares cut meet in LDS where the shares belong to
+// one workgroup, and as partials (max, sum, O) in memory, which a second launch merges, where not.
 //
-// Within a share the four waves take STEP positions each in turn, with no exchange between them
-// until the end, and no LDS: S^T = K Q^T (positions x heads) comes out of the matrix instruction
-// with a lane holding four positions of one head, which is how O^T = V^T P^T (dims x heads) wants
-// P^T, when the K rows of a tile are picked so: lane row m of tile t is position
-// (STEP/4)(m/4) + 4t + m%4, so that a lane's rows over the tiles are STEP/4 consecutive positions.
-// K fragments are 16 bytes of a K row, V fragments 16 bytes of positions of one dim.
+// A wave streams its steps with no exchange with others and no LDS: S^T = K Q^T (positions x heads)
+// comes out of the matrix instruction with a lane holding four positions of one head, which is how
+// O^T = V^T P^T (dims x heads) wants P^T, when the K rows of a tile are picked so: lane row m of
+// tile t is position (kStep/4)(m/4) + 4t + m%4, so that a lane's rows over the tiles are kStep/4
+// consecutive positions.  K fragments are 16 bytes of a K row, V fragments 16 bytes of positions of
+// one dim.
 //
 // Precision: Q is scaled by a power of two into [1, 2) per head and split into two f16 parts, P
 // likewise split; K and V enter exactly (f16 or int8).  P is formed relative to a reference that
@@ -37,29 +37,33 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-constexpr int kPaThreads = 256, kPaWaves = 4, kPaRows = 16;
+constexpr int kPaRows = 16;
 constexpr float kSlack = 5.0f, kLift = 9.0f;  // powers of two: P <= 2^14, times a scale below 2
 
 template <int KV, int HD>
 struct PaShape {
     static constexpr int kStep = KV == kKvF16 ? 32 : 64;  // positions of a wave's step
-    static constexpr int kUnit = kPaWaves * kStep;
     static constexpr int kTiles = kStep / 16;
     static constexpr int kKs = HD / 32, kNd = HD / 16;  // dim steps of S, dim tiles of O
+    // one workgroup per CU; its pieces fill LDS (135 KB at head_dim 128)
+    static constexpr int kWaves = HD == 256 ? 4 : HD == 64 && KV == kKvF16 ? 16 : 8;
+    static constexpr int kThreads = 64 * kWaves;
 };
 
-constexpr int kPaMaxGroups = 768;
+constexpr int kPaGroups = 256;  // one per CU
 static int part_floats(int hd) { return kPaRows * (hd + 2); }
-size_t paged_attn_workspace_bytes(int, int hd) { return (size_t)2 * kPaMaxGroups * part_floats(hd) * sizeof(float); }
+size_t paged_attn_workspace_bytes(int, int hd) { return (size_t)2 * kPaGroups * part_floats(hd) * sizeof(float); }
 
 // Inclusive sum over the lower lanes.
 __device__ __forceinline__ int wave_scan(int v) {
-    const int lane = lane_id();
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(v, o);
-        if (lane >= o) v += y;
-    }
+#define MNEMO_SCAN(CTRL, ROWS) v += __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false)
+    MNEMO_SCAN(0x111, 0xF);  // row_shr 1, 2, 4, 8: lanes that would read past their row of 16 add 0
+    MNEMO_SCAN(0x112, 0xF);
+    MNEMO_SCAN(0x114, 0xF);
+    MNEMO_SCAN(0x118, 0xF);
+    MNEMO_SCAN(kDppRowBcast15, 0xA);
+    MNEMO_SCAN(kDppRowBcast31, 0xC);
+#undef MNEMO_SCAN
     return v;
 }
 
@@ -67,53 +71,77 @@ __device__ __forceinline__ int seq_len(const PagedAttnArgs &a, int s) {
     return min(max(a.lens[s], 0), a.max_pages * a.c.ps);
 }
 
-// Where the units begin: the row of units is [sequence][KV head][unit].
+// The row of steps, [sequence][KV head][step], and its shares.
 struct PaPlan {
-    int total;   // units
+    int total;   // steps
     int groups;  // workgroups that have some
+    int base, more;  // steps of a workgroup; the first `more` of them have one more
+    int nw;      // waves of a workgroup that take shares
+    bool empty;  // lane: a sequence of its has no positions
     int per;     // sequences per lane of the sums
-    int before;  // lane: units before its sequences
+    int len;     // lane: length of its sequence, where per is 1
+    int before;  // lane: steps before its sequences
 };
 
-template <int UNIT>
+// The CUs are filled before the waves of a workgroup: a CU alone takes ~1 us for 8 steps.
+template <int STEP, int NW>
 __device__ __forceinline__ PaPlan pa_plan(const PagedAttnArgs &a, int groups) {
     PaPlan p;
     p.per = (a.n_seqs + 63) / 64;
+    p.len = 0;
+    p.empty = false;
     const int s0 = lane_id() * p.per;
     int sum = 0;
     for (int i = 0; i < p.per; i++)
-        if (s0 + i < a.n_seqs) sum += (seq_len(a, s0 + i) + UNIT - 1) / UNIT;
+        if (s0 + i < a.n_seqs) {
+            p.len = seq_len(a, s0 + i);
+            p.empty |= p.len == 0;
+            sum += (p.len + STEP - 1) / STEP;
+        }
     sum *= a.c.nkv;
     const int incl = wave_scan(sum);
     p.total = __builtin_amdgcn_readlane(incl, 63);
     p.before = incl - sum;
-    p.groups = min(groups, p.total);
+    p.groups = max(min(groups, p.total), 1);
+    p.base = p.total / p.groups;
+    p.more = p.total - p.base * p.groups;
+    p.nw = min(p.base + 1, NW);
     return p;
 }
 
-// First unit of workgroup w, and the workgroup of unit u.
-__device__ __forceinline__ int pa_first(const PaPlan &p, int w) { return (int)((long long)w * p.total / p.groups); }
+// First step of workgroup g (the end of the row from g = groups on), and the workgroup of step u.
+__device__ __forceinline__ int pa_first(const PaPlan &p, int g) {
+    return g >= p.groups ? p.total : g * p.base + min(g, p.more);
+}
 __device__ __forceinline__ int pa_group(const PaPlan &p, int u) {
-    return (int)(((long long)(u + 1) * p.groups - 1) / p.total);
+    const int cut = p.more * (p.base + 1);
+    return u < cut ? u / (p.base + 1) : p.more + (u - cut) / p.base;
 }
 
-// The sequence, KV head and unit within them of unit u; len: of the sequence.
-template <int UNIT>
-__device__ __forceinline__ void pa_find(const PagedAttnArgs &a, const PaPlan &p, int u, int &seq, int &kvh, int &unit,
+// The sequence, its length, the KV head and the step within them of step u.
+template <int STEP>
+__device__ __forceinline__ void pa_find(const PagedAttnArgs &a, const PaPlan &p, int u, int &seq, int &kvh, int &step,
                                         int &len) {
     const int lane = lane_id();
-    const int L = __popcll(__ballot(p.before <= u)) - 1;  // the last lane that begins at or before u holds it
-    const int base = __builtin_amdgcn_readlane(p.before, L);
-    const int s = L * p.per + lane;
-    const int ln = lane < p.per && s < a.n_seqs ? seq_len(a, s) : 0;
-    const int n = (ln + UNIT - 1) / UNIT * a.c.nkv;
-    const int before = base + wave_scan(n) - n;
-    const int j = __popcll(__ballot(lane < p.per && before <= u)) - 1;
-    seq = L * p.per + j;
-    len = __builtin_amdgcn_readlane(ln, j);
-    const int at = u - __builtin_amdgcn_readlane(before, j), nu = (len + UNIT - 1) / UNIT;
-    kvh = at / nu;
-    unit = at % nu;
+    // the last lane that begins at or before u holds it (lanes without steps share their successor's beginning)
+    const int L = __popcll(__ballot(p.before <= u)) - 1;
+    int at = u - __builtin_amdgcn_readlane(p.before, L);
+    if (p.per == 1) {
+        seq = L;
+        len = __builtin_amdgcn_readlane(p.len, L);
+    } else {
+        const int s = L * p.per + lane;
+        const int ln = lane < p.per && s < a.n_seqs ? seq_len(a, s) : 0;
+        const int n = (ln + STEP - 1) / STEP * a.c.nkv;
+        const int before = wave_scan(n) - n;
+        const int j = __popcll(__ballot(lane < p.per && before <= at)) - 1;
+        seq = L * p.per + j;
+        len = __builtin_amdgcn_readlane(ln, j);
+        at -= __builtin_amdgcn_readlane(before, j);
+    }
+    const int steps = (len + STEP - 1) / STEP;
+    kvh = at / steps;
+    step = at % steps;
 }
 
 // max over the four lanes that share a head (lane % 16), in all of them
@@ -144,32 +172,33 @@ __device__ __forceinline__ h8 cvt8(uint32_t a, uint32_t b) {
 }
 
 template <int KV, int HD>
-__global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kernel(PagedAttnArgs a) {
+__global__ void __launch_bounds__((PaShape<KV, HD>::kThreads)) paged_attn_kernel(PagedAttnArgs a) {
     using S = PaShape<KV, HD>;
-    constexpr int STEP = S::kStep, UNIT = S::kUnit, NT = S::kTiles, KS = S::kKs, ND = S::kNd;
+    constexpr int STEP = S::kStep, NT = S::kTiles, KS = S::kKs, ND = S::kNd, NW = S::kWaves;
     constexpr int EB = KV == kKvF16 ? 2 : 1;
     constexpr int PV = STEP / 32;  // position steps of O
-    __shared__ __align__(16) float lo[kPaWaves][kPaRows][HD + 4];
-    __shared__ float lm[kPaWaves][kPaRows], ll[kPaWaves][kPaRows];
+    // pieces of cut (sequence, KV head)s: [.][0] one that began before the wave's share, [.][1] one
+    // that begins in it and goes on
+    __shared__ __align__(16) float lo[NW][2][kPaRows][HD + 4];
+    __shared__ float lm[NW][2][kPaRows], ll[NW][2][kPaRows];
+    __shared__ int pair_of[NW][2], ends[NW];  // the pieces' seq * n_kv + kvh (-1: none); whether piece 0 ends there
     const int lane = lane_id(), r = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ps = a.c.ps, psl = 31 - __builtin_clz(ps);
 
-    // rows with no positions
-    for (int s = blockIdx.x; s < a.n_seqs; s += gridDim.x)
-        if (seq_len(a, s) == 0)
-            for (int i = threadIdx.x; i < a.nh * HD; i += kPaThreads) a.out[(size_t)s * a.nh * HD + i] = 0.0f;
+    const PaPlan plan = pa_plan<STEP, NW>(a, gridDim.x);
+    // the workgroup's steps, shared out to its waves in the same way
+    const int g0 = pa_first(plan, blockIdx.x), gn = pa_first(plan, blockIdx.x + 1) - g0;
+    const int each = gn / plan.nw, odd = gn - each * plan.nw;
+    int at = g0 + wave * each + min(wave, odd);
+    const int end = wave < plan.nw ? at + each + (wave < odd) : at;
+    if (lane < 2) pair_of[wave][lane] = -1;
+    int seq = 0, kvh = 0, step = 0, len = 0;
+    if (at < end) pa_find<STEP>(a, plan, at, seq, kvh, step, len);
 
-    const PaPlan plan = pa_plan<UNIT>(a, gridDim.x);
-    if ((int)blockIdx.x >= plan.groups) return;
-    int at = pa_first(plan, blockIdx.x);
-    const int end = pa_first(plan, blockIdx.x + 1);
-    int seq, kvh, unit, len;
-    pa_find<UNIT>(a, plan, at, seq, kvh, unit, len);
-
-    while (true) {
-        const int nu = (len + UNIT - 1) / UNIT, n = min(end - at, nu - unit);
-        const int p_end = min(len, (unit + n) * UNIT);
+    while (at < end) {
+        const int steps = (len + STEP - 1) / STEP, n = min(end - at, steps - step);
+        const int p_end = min(len, (step + n) * STEP);
         const int *table = a.table + (size_t)seq * a.max_pages;
         const uint8_t *kc = (const uint8_t *)a.c.k, *vc = (const uint8_t *)a.c.v;
 
@@ -214,8 +243,8 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
         float m = -INFINITY, l = 0.0f;  // reference (log2) of the lane's head, sum over the lane's positions
         float vref = 0x1p-126f;
         f4 o[ND] = {};
-        int p0 = unit * UNIT + wave * STEP;
-        if (p0 < p_end) {
+        int p0 = step * STEP;
+        {
             Pages cur = entries(p0);
             // ---- Q: dims of slot j of dim step st as the K fragments have them
             float q[KS][8];
@@ -228,7 +257,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
             }
             load_k(p0, cur.k);
             if (KV == kKvInt8) load_scales(p0, cur.v);
-            int next = p0 + UNIT;
+            int next = p0 + STEP;
             Pages nxt = entries(min(next, len - 1));
             load_v(p0, cur.v);
             float qm = 0.0f;
@@ -323,7 +352,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
                         plo[t / 2][4 * (t & 1) + i] = (_Float16)(w - (float)hi);
                     }
                 if (KV == kKvInt8 && more) load_scales(next, nxt.v);
-                const Pages after = entries(min(next + UNIT, len - 1));
+                const Pages after = entries(min(next + STEP, len - 1));
                 // ---- O^T
                 if (KV == kKvF16 && !full) {
                     // what lies past the end may be no number, which a weight of 0 does not hide
@@ -350,154 +379,214 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
                 if (!more) break;
                 load_v(next, nxt.v);
                 p0 = next;
-                next += UNIT;
+                next += STEP;
                 cur = nxt;
                 nxt = after;
             }
         }
-        // ---- the four waves' results meet in LDS
         l = sum_heads(l);
-        if (kg == 0) {
-            lm[wave][r] = m;
-            ll[wave][r] = l;
-        }
+        const bool begins = step == 0, finishes = step + n == steps;
+        if (begins && finishes) {
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            float *out = a.out + ((size_t)seq * a.nh + kvh * a.gqa + r) * HD + 4 * kg;
+            if (r < a.gqa) {
 #pragma unroll
-        for (int i = 0; i < ND; i++) {
-            f4 x = o[i];
-            if (KV == kKvInt8) x *= vref;
-            __builtin_memcpy(&lo[wave][r][16 * i + 4 * kg], &x, 16);
-        }
-        __syncthreads();
-        const bool whole = unit == 0 && n == nu;  // finished here
-        // a partial goes to the first slot when the (sequence, KV head) began in an earlier workgroup
-        float *part = a.ws + (size_t)(2 * blockIdx.x + (unit == 0)) * (kPaRows * (HD + 2));
-        for (int e = threadIdx.x; e < a.gqa * (HD / 4); e += kPaThreads) {
-            const int h = e / (HD / 4), d = 4 * (e % (HD / 4));
-            float mm = lm[0][h];
-#pragma unroll
-            for (int w = 1; w < kPaWaves; w++) mm = fmaxf(mm, lm[w][h]);
-            f4 x = {};
-            float sum = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kPaWaves; w++) {
-                const float f = mm == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lm[w][h] - mm);
-                f4 y;
-                __builtin_memcpy(&y, &lo[w][h][d], 16);
-                x += y * f;
-                sum = fmaf(ll[w][h], f, sum);
-            }
-            if (whole) {
-                x = sum == 0.0f ? f4{0.f, 0.f, 0.f, 0.f} : x / sum;
-                __builtin_memcpy(a.out + ((size_t)seq * a.nh + kvh * a.gqa + h) * HD + d, &x, 16);
-            } else {
-                __builtin_memcpy(part + 2 * kPaRows + h * HD + d, &x, 16);
-                if (d == 0) {
-                    part[h] = mm;
-                    part[kPaRows + h] = sum;
+                for (int i = 0; i < ND; i++) {
+                    const f4 x = o[i] * (KV == kKvInt8 ? vref * inv : inv);
+                    __builtin_memcpy(out + 16 * i, &x, 16);
                 }
+            }
+        } else {
+            if (lane == 0) {
+                pair_of[wave][begins] = seq * a.c.nkv + kvh;
+                if (!begins) ends[wave] = finishes;
+            }
+            if (kg == 0) {
+                lm[wave][begins][r] = m;
+                ll[wave][begins][r] = l;
+            }
+#pragma unroll
+            for (int i = 0; i < ND; i++) {
+                f4 x = o[i];
+                if (KV == kKvInt8) x *= vref;
+                __builtin_memcpy(&lo[wave][begins][r][16 * i + 4 * kg], &x, 16);
             }
         }
         at += n;
-        if (at >= end) return;
-        __syncthreads();  // the sums are read
-        unit = 0;
-        if (++kvh == a.c.nkv) {
+        step = 0;
+        if (at < end && ++kvh == a.c.nkv) {
             kvh = 0;
             do len = seq_len(a, ++seq);
-            while (len == 0);  // a unit is left, so a sequence with positions is
+            while (len == 0);  // a step is left, so a sequence with positions is
+        }
+    }
+    if (__any(plan.empty))
+        for (int s = blockIdx.x * NW + wave; s < a.n_seqs; s += gridDim.x * NW)
+            if (seq_len(a, s) == 0)
+                for (int i = lane; i < a.nh * HD; i += 64) a.out[(size_t)s * a.nh * HD + i] = 0.0f;
+
+    // ---- pieces of one (sequence, KV head), from consecutive waves, are merged.  Lane i holds piece
+    // (i / 2, i % 2).  A chain begins with a piece 1, or with piece 0 of the first wave, and takes in
+    // the pieces 0 of the waves that follow, up to the next beginning.
+    __syncthreads();
+    const int pair = lane < 2 * NW ? pair_of[lane >> 1][lane & 1] : -1;
+    const bool closes = lane < 2 * NW && !(lane & 1) && pair >= 0 && ends[lane >> 1];
+    const uint32_t pieces = (uint32_t)__ballot(pair >= 0), closed = (uint32_t)__ballot(closes);
+    const uint32_t starts = pieces & (0xaaaaaaaau | 1u);
+    const int per = a.gqa * (HD / 4);  // elements of four dims
+    for (int e = threadIdx.x; e < __popc(starts) * per; e += S::kThreads) {
+        const int c = e / per, h = e % per / (HD / 4), d = 4 * (e % (HD / 4));
+        uint32_t from = starts;  // from its c-th bit on
+        for (int i = 0; i < c; i++) from &= from - 1;
+        const int first = __ffs((int)from) - 1;
+        const uint32_t rest = from & (from - 1);
+        // its pieces: pieces 0 between its beginning and the next one
+        const uint32_t in = pieces & 0x55555555u & ~((2u << first) - 1) & (rest ? (rest & (0u - rest)) - 1 : ~0u);
+        const int w = first >> 1, k = first & 1, n = __popc(in);
+        const bool whole = k == 1 && (in & closed);
+        float mm = lm[w][k][h], sum = ll[w][k][h];
+        f4 x;
+        __builtin_memcpy(&x, &lo[w][k][h][d], 16);
+        for (int i = 1; i <= n; i++) {
+            const float pm = lm[w + i][0][h], mn = fmaxf(mm, pm);
+            f4 y;
+            __builtin_memcpy(&y, &lo[w + i][0][h][d], 16);
+            if (mn == -INFINITY) continue;
+            const float fa = __builtin_amdgcn_exp2f(mm - mn), fb = __builtin_amdgcn_exp2f(pm - mn);
+            x = x * fa + y * fb;
+            sum = fmaf(sum, fa, ll[w + i][0][h] * fb);
+            mm = mn;
+        }
+        const int pr = pair_of[w][k];
+        if (whole) {
+            x *= sum == 0.0f ? 0.0f : 1.0f / sum;
+            __builtin_memcpy(a.out + ((size_t)(pr / a.c.nkv) * a.nh + pr % a.c.nkv * a.gqa + h) * HD + d, &x, 16);
+        } else {
+            float *part = a.ws + (size_t)(2 * blockIdx.x + k) * (kPaRows * (HD + 2));
+            __builtin_memcpy(part + 2 * kPaRows + h * HD + d, &x, 16);
+            if (d == 0) {
+                part[h] = mm;
+                part[kPaRows + h] = sum;
+            }
         }
     }
 }
 
 // Merges the partials of the (sequence, KV head)s that several workgroups share.  Workgroup x looks
-// after the one that begins in share x and goes on behind it (BY_SHARE), or after (sequence, KV head)
-// x itself.  32 x 8 threads: HD / 32 dims each of every eighth partial, then over the eight.
-template <int UNIT, int HD, bool BY_SHARE>
+// after the one that begins in workgroup x's share and goes on behind it (BY_SHARE), or after
+// (sequence, KV head) x itself.  256 threads are HD / 4 lanes of four dims, times CHAIN threads that
+// divide the partials among them, times heads.
+template <int STEP, int HD, int NW, int CHAIN, bool BY_SHARE>
 __global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnArgs a, int groups) {
-    constexpr int D = HD / 32;
-    __shared__ float so[8][HD], sm[8], sl[8];
-    const PaPlan plan = pa_plan<UNIT>(a, groups);
+    constexpr int D4 = HD / 4, HEADS = 256 / (D4 * CHAIN), BATCH = 4;
+    __shared__ __align__(16) float so[CHAIN > 1 ? CHAIN : 1][HEADS][HD];
+    __shared__ float sm[CHAIN][HEADS], sl[CHAIN][HEADS];
+    const PaPlan plan = pa_plan<STEP, NW>(a, groups);
     int seq, kvh, first, last, len;
     if (BY_SHARE) {
-        if ((int)blockIdx.x + 1 >= plan.groups) return;
-        const int u = pa_first(plan, blockIdx.x + 1) - 1;  // the last unit of the share
-        int unit;
-        pa_find<UNIT>(a, plan, u, seq, kvh, unit, len);
-        const int nu = (len + UNIT - 1) / UNIT;
-        if (unit + 1 == nu || u - unit < pa_first(plan, blockIdx.x)) return;
-        first = u - unit;
-        last = first + nu - 1;
+        const int u = pa_first(plan, blockIdx.x + 1) - 1;  // the last step of the share
+        if (u + 1 == plan.total) return;                          // nothing goes on behind it
+        int step;
+        pa_find<STEP>(a, plan, u, seq, kvh, step, len);
+        const int steps = (len + STEP - 1) / STEP;
+        first = u - step;
+        last = first + steps - 1;
+        if (last == u || first < pa_first(plan, blockIdx.x)) return;
     } else {
         seq = blockIdx.x / a.c.nkv;
         kvh = blockIdx.x % a.c.nkv;
         len = seq_len(a, seq);
         if (len == 0) return;
-        const int nu = (len + UNIT - 1) / UNIT;
-        const int L = seq / plan.per;
-        int before = __builtin_amdgcn_readlane(plan.before, L);
-        int mine = 0;
-        const int s = L * plan.per + lane_id();
-        if (s < seq) mine = (seq_len(a, s) + UNIT - 1) / UNIT * a.c.nkv;
-        before += __builtin_amdgcn_readlane(wave_scan(mine), 63);
-        first = before + kvh * nu;
-        last = first + nu - 1;
+        const int steps = (len + STEP - 1) / STEP, L = seq / plan.per;
+        first = __builtin_amdgcn_readlane(plan.before, L) + kvh * steps;
+        if (plan.per > 1) {
+            const int s = L * plan.per + lane_id();
+            const int mine = s < seq ? (seq_len(a, s) + STEP - 1) / STEP * a.c.nkv : 0;
+            first += __builtin_amdgcn_readlane(wave_scan(mine), 63);
+        }
+        last = first + steps - 1;
     }
     const int w0 = pa_group(plan, first), w1 = pa_group(plan, last);
     if (w0 == w1) return;
-    const int dl = threadIdx.x & 31, g = threadIdx.x >> 5;
+    const int dl = threadIdx.x % D4, g = threadIdx.x / D4 % CHAIN, hh = threadIdx.x / (D4 * CHAIN);
     constexpr int PART = kPaRows * (HD + 2);
-    for (int h = blockIdx.y; h < a.gqa; h += gridDim.y) {
-        float m = -INFINITY, l = 0.0f, o[D] = {};
-        for (int w = w0 + g; w <= w1; w += 8) {
-            // the first share holds its beginning in its second slot, the others in the first
-            const float *p = a.ws + (size_t)(2 * w + (w == w0)) * PART;
-            const float pm = p[h], pl = p[kPaRows + h];
-            float x[D];
-            __builtin_memcpy(x, p + 2 * kPaRows + h * HD + D * dl, 4 * D);
-            const float mn = fmaxf(m, pm);
-            if (mn == -INFINITY) continue;
-            const float fa = __builtin_amdgcn_exp2f(m - mn), fb = __builtin_amdgcn_exp2f(pm - mn);
-            l = l * fa + pl * fb;
+    for (int h0 = blockIdx.y * HEADS; h0 < a.gqa; h0 += gridDim.y * HEADS) {
+        const int h = min(h0 + hh, a.gqa - 1);
+        float m = -INFINITY, l = 0.0f;
+        f4 o = {};
+        for (int w = w0 + g; w <= w1; w += CHAIN * BATCH) {
+            float pm[BATCH], pl[BATCH];
+            f4 x[BATCH];
 #pragma unroll
-            for (int i = 0; i < D; i++) o[i] = o[i] * fa + x[i] * fb;
+            for (int i = 0; i < BATCH; i++) {  // all loads of a batch go out together
+                const int v = min(w + CHAIN * i, w1);
+                // the first workgroup holds its beginning in its second slot, the others in the first
+                const float *p = a.ws + (size_t)(2 * v + (v == w0)) * PART;
+                pm[i] = w + CHAIN * i <= w1 ? p[h] : -INFINITY;
+                pl[i] = p[kPaRows + h];
+                __builtin_memcpy(&x[i], p + 2 * kPaRows + h * HD + 4 * dl, 16);
+            }
+            float mn = m;
+#pragma unroll
+            for (int i = 0; i < BATCH; i++) mn = fmaxf(mn, pm[i]);
+            if (mn == -INFINITY) continue;
+            const float fa = __builtin_amdgcn_exp2f(m - mn);
+            l *= fa;
+            o *= fa;
+#pragma unroll
+            for (int i = 0; i < BATCH; i++) {
+                const float f = __builtin_amdgcn_exp2f(pm[i] - mn);
+                l = fmaf(pl[i], f, l);
+                o += x[i] * f;
+            }
             m = mn;
         }
-        __syncthreads();  // the last head's sums are read
-        __builtin_memcpy(&so[g][D * dl], o, 4 * D);
-        if (dl == 0) {
-            sm[g] = m;
-            sl[g] = l;
-        }
-        __syncthreads();
-        if ((int)threadIdx.x < HD) {
-            float mm = sm[0];
-#pragma unroll
-            for (int i = 1; i < 8; i++) mm = fmaxf(mm, sm[i]);
-            float sum = 0.0f, x = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float f = mm == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[i] - mm);
-                sum = fmaf(sl[i], f, sum);
-                x = fmaf(so[i][threadIdx.x], f, x);
+        if (CHAIN > 1) {
+            __syncthreads();  // the last heads' sums are read
+            __builtin_memcpy(&so[g][hh][4 * dl], &o, 16);
+            if (dl == 0) {
+                sm[g][hh] = m;
+                sl[g][hh] = l;
             }
-            a.out[((size_t)seq * a.nh + kvh * a.gqa + h) * HD + threadIdx.x] = sum == 0.0f ? 0.0f : x / sum;
+            __syncthreads();
+            if (g > 0) continue;
+            float mm = sm[0][hh];
+#pragma unroll
+            for (int i = 1; i < CHAIN; i++) mm = fmaxf(mm, sm[i][hh]);
+            l = 0.0f;
+            o = f4{};
+#pragma unroll
+            for (int i = 0; i < CHAIN; i++) {
+                const float f = mm == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[i][hh] - mm);
+                f4 y;
+                __builtin_memcpy(&y, &so[i][hh][4 * dl], 16);
+                l = fmaf(sl[i][hh], f, l);
+                o += y * f;
+            }
+        }
+        if (h0 + hh < a.gqa) {
+            o *= l == 0.0f ? 0.0f : 1.0f / l;
+            __builtin_memcpy(a.out + ((size_t)seq * a.nh + kvh * a.gqa + h) * HD + 4 * dl, &o, 16);
         }
     }
 }
 
 template <int KV, int HD>
 static void launch_pa(const PagedAttnArgs &a, hipStream_t s) {
-    constexpr int UNIT = PaShape<KV, HD>::kUnit;
+    using S = PaShape<KV, HD>;
+    constexpr int CHAIN = 1024 / HD;  // 256 threads for one head
     const long long pairs = (long long)a.n_seqs * a.c.nkv;
-    const long long most = pairs * (((long long)a.max_pages * a.c.ps + UNIT - 1) / UNIT);  // units, whatever the lengths
-    const int groups = (int)(most < kPaMaxGroups ? most : kPaMaxGroups);
-    hipLaunchKernelGGL((paged_attn_kernel<KV, HD>), dim3(groups), dim3(kPaThreads), 0, s, a);
-    if (pairs < groups) {
-        const int y = (int)(1024 / pairs < a.gqa ? (1024 / pairs < 1 ? 1 : 1024 / pairs) : a.gqa);
-        hipLaunchKernelGGL((paged_merge_kernel<UNIT, HD, false>), dim3((int)pairs, y), dim3(256), 0, s, a, groups);
-    } else if (most > pairs) {  // else no (sequence, KV head) has a second unit
-        hipLaunchKernelGGL((paged_merge_kernel<UNIT, HD, true>), dim3(groups, 1), dim3(256), 0, s, a, groups);
-    }
+    const long long most = pairs * (((long long)a.max_pages * a.c.ps + S::kStep - 1) / S::kStep);  // steps
+    const int groups = (int)(most < kPaGroups ? most : kPaGroups);
+    hipLaunchKernelGGL((paged_attn_kernel<KV, HD>), dim3(groups), dim3(S::kThreads), 0, s, a);
+    if (groups == 1) return;
+    // few (sequence, KV head)s: long chains, a workgroup for each head; many: short ones, found by the shares' ends
+    if (pairs < groups)
+        hipLaunchKernelGGL((paged_merge_kernel<S::kStep, HD, S::kWaves, CHAIN, false>), dim3((int)pairs, a.gqa), dim3(256),
+                           0, s, a, groups);
+    else
+        hipLaunchKernelGGL((paged_merge_kernel<S::kStep, HD, S::kWaves, 1, true>), dim3(groups - 1, 1), dim3(256), 0, s, a,
+                           groups);
 }
 
 int launch_paged_attention(const PagedAttnArgs &a, hipStream_t s) {
