@@ -774,8 +774,8 @@ int mnemo_logits_process(const float *logits, float *out, int n_rows, int vocab,
                          const int *history_lens, const int *prompt_lens, int max_history, const float *repetition,
                          const float *frequency, const float *presence, const int *bias_ids, const float *bias,
                          int n_bias, const unsigned *allowed, hipStream_t s) {
-    if (n_rows < 0 || n_rows > 65535 || vocab <= 0)
-        return set_error(kErrBadArg, "logits_process: need 0 <= n_rows <= 65535 and vocab > 0");
+    if (n_rows < 0 || n_rows > 65535 || vocab <= 0 || vocab > 1 << 30)
+        return set_error(kErrBadArg, "logits_process: need 0 <= n_rows <= 65535 and 1 <= vocab <= 2^30");
     if (history && (!history_lens || !prompt_lens || !repetition || !frequency || !presence || max_history < 0))
         return set_error(kErrBadArg, "logits_process: a history needs its lengths and the three penalties");
     if (bias_ids && (!bias || n_bias < 0)) return set_error(kErrBadArg, "logits_process: bias_ids needs bias");

@@ -103,7 +103,7 @@ def logits(L, *, z=A, out=A, n=2, vocab=100, hist=A, hl=A, pl=A, max_hist=8, rep
                                   None)
 
 
-@pytest.mark.parametrize("bad", [dict(z=None), dict(out=None), dict(n=-1), dict(n=65536), dict(vocab=0), dict(hl=None),
+@pytest.mark.parametrize("bad", [dict(z=None), dict(out=None), dict(n=-1), dict(n=65536), dict(vocab=0), dict(vocab=(1 << 30) + 1), dict(hl=None),
                                  dict(pl=None), dict(rep=None), dict(freq=None), dict(pres=None), dict(max_hist=-1),
                                  dict(bias=None), dict(nb=-1)])
 def test_logits_refuses(L, bad, capfd):
