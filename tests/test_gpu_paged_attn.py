@@ -365,6 +365,46 @@ def test_prep(gpu, hd, ps, nkv, nh, norm, int8):
         assert np.array_equal(new[~hit].view(np.uint8), old[~hit].view(np.uint8))
 
 
+@pytest.mark.parametrize("hd,ps,nkv,nh", [(128, 64, 4, 8), (64, 16, 12, 12), (256, 32, 3, 3), (128, 128, 8, 16)])
+@pytest.mark.parametrize("int8", [False, True])
+def test_prep_of_many_tokens(gpu, hd, ps, nkv, nh, int8):
+    """A call of many tokens equals calls of few, bit for bit: runs that begin anywhere in a page, runs of under
+    eight, two sequences' tokens in turn, a run backwards, padding and absent pages within a run."""
+    rng = np.random.default_rng(hd + ps + nkv)
+    n_seqs, width = 6, 1200 // ps + 2
+    n_pages = n_seqs * width
+    table = rng.permutation(n_pages).astype(np.int32).reshape(n_seqs, width)
+    table[2, 1] = -1
+    seq, pos = [], []
+    for s, p in [(0, range(3, 503)), (1, range(8, 13)), (1, range(16, 24)), (2, range(0, 300)), (3, range(400, 200, -1)),
+                 (4, [x for i in range(100) for x in (i, -1)]), (1, range(100, 101)), (5, range(64, 1000))]:
+        seq += [s] * len(p)
+        pos += list(p)
+    a = np.arange(200)  # two sequences in turn
+    seq += list(np.where(a % 2, 0, 3))
+    pos += list(600 + a // 2)
+    seq, pos = np.array(seq, np.int32), np.array(pos, np.int32)
+    pos[1100:1103] = -1
+    T = len(seq)
+    assert T * nkv >= 2048
+    q, k, v = (rng.standard_normal((T, h, hd)).astype(np.float32) for h in (nh, nkv, nkv))
+    w = dev(np.ones(hd, np.float32))
+    start = pool(rng, n_pages, nkv, ps, hd, int8)
+    qd, kd, vd, td, sd, pd = dev(q), dev(k), dev(v), dev(table), dev(seq), dev(pos)
+    got = []
+    for step in (T, 100):
+        p = [opt(x) for x in start]
+        qo = torch.zeros((T, nh, hd), device="cuda")
+        case(f"paged prep of {T} tokens by {step}, hd={hd} ps={ps} nkv={nkv} int8={int8}")
+        for t in range(0, T, step):
+            at = slice(t, t + step)
+            gpu.ops.paged_attn_prep(qd[at], kd[at], vd[at], w, w, 1e-6, 1e6, p[0], p[1], td, qo[at], pd[at], sd[at], p[2], p[3])
+        got.append([qo] + [x for x in p if x is not None])
+    for x, y in zip(*got):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    assert not torch.equal(got[0][1].view(torch.uint8), opt(start[0]).view(torch.uint8))
+
+
 @pytest.mark.parametrize("theta", [1e6, 1e4, 1.0])
 def test_prep_far_positions(gpu, theta):
     """Positions to 2^31 - 1: the angle loses nothing."""
