@@ -408,7 +408,7 @@ int mnemo_kv_pages_free(int *block_table, int *seq_lens, int *page_refs, const i
 /* fork: every row with parents[s] >= 0 becomes a copy of that row as it was before the call (the
  * row must be empty and the parent not; refused otherwise).  Full pages are shared; a partly
  * filled last page is copied to a page of its own, in all n_layers layers of the caches
- * ([n_layers][n_pages]...).  workspace: mnemo_kv_pages_workspace_bytes(n_seqs, n_pages) bytes,
+ * ([n_layers][n_pages]..., n_layers <= 4096).  workspace: mnemo_kv_pages_workspace_bytes(n_seqs, n_pages) bytes,
  * 16-byte aligned, no initialisation; calls sharing it must not overlap. */
 size_t mnemo_kv_pages_workspace_bytes(int n_seqs, int n_pages);
 int mnemo_kv_pages_fork(int *block_table, int *seq_lens, int *page_refs, const int *parents, int n_seqs,

@@ -725,7 +725,7 @@ int mnemo_kv_pages_free(int *block_table, int *seq_lens, int *page_refs, const i
 static int check_moving(const char *what, const PagedCache &c, int n_layers, const void *ws, size_t ws_bytes,
                         size_t need) {
     if (int rc = check_cache(what, c)) return rc;
-    if (n_layers <= 0) return set_error(kErrBadArg, "%s: need n_layers > 0", what);
+    if (n_layers <= 0 || n_layers > 4096) return set_error(kErrBadArg, "%s: need 1 <= n_layers <= 4096", what);
     if (need && (!ws || (uintptr_t)ws % 16 || ws_bytes < need))
         return set_error(kErrBadArg, "%s: workspace NULL, not 16-byte aligned, or %zu < %zu bytes", what, ws_bytes,
                          need);

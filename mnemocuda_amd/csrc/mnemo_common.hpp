@@ -154,6 +154,19 @@ __device__ __forceinline__ float sum32_lane31(float v) {
     v += dpp_f<kDppRowBcast15, 0xA>(v);
     return v;
 }
+// Inclusive sum of whole numbers over the lower lanes of the wave.
+__device__ __forceinline__ int wave_scan(int v) {
+#define MNEMO_SCAN(CTRL, ROWS) v += __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false)
+    MNEMO_SCAN(0x111, 0xF);  // row_shr 1, 2, 4, 8: lanes that would read past their row of 16 add 0
+    MNEMO_SCAN(0x112, 0xF);
+    MNEMO_SCAN(0x114, 0xF);
+    MNEMO_SCAN(0x118, 0xF);
+    MNEMO_SCAN(kDppRowBcast15, 0xA);
+    MNEMO_SCAN(kDppRowBcast31, 0xC);
+#undef MNEMO_SCAN
+    return v;
+}
+
 // Max over aligned groups of 8 lanes; every lane of the group gets the max.
 __device__ __forceinline__ float max8(float v) {
     v = fmaxf(v, dpp_f<kDppXor1>(v));

@@ -54,19 +54,6 @@ constexpr int kPaGroups = 256;  // one per CU
 static int part_floats(int hd) { return kPaRows * (hd + 2); }
 size_t paged_attn_workspace_bytes(int, int hd) { return (size_t)2 * kPaGroups * part_floats(hd) * sizeof(float); }
 
-// Inclusive sum over the lower lanes.
-__device__ __forceinline__ int wave_scan(int v) {
-#define MNEMO_SCAN(CTRL, ROWS) v += __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false)
-    MNEMO_SCAN(0x111, 0xF);  // row_shr 1, 2, 4, 8: lanes that would read past their row of 16 add 0
-    MNEMO_SCAN(0x112, 0xF);
-    MNEMO_SCAN(0x114, 0xF);
-    MNEMO_SCAN(0x118, 0xF);
-    MNEMO_SCAN(kDppRowBcast15, 0xA);
-    MNEMO_SCAN(kDppRowBcast31, 0xC);
-#undef MNEMO_SCAN
-    return v;
-}
-
 __device__ __forceinline__ int seq_len(const PagedAttnArgs &a, int s) {
     return min(max(a.lens[s], 0), a.max_pages * a.c.ps);
 }

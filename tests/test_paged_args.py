@@ -80,7 +80,7 @@ def copy(L, *, src=A, dst=A, n=2, n_pages=8, ps=64, kp=A, vp=A, ks=None, vs=None
 STATE = [dict(table=None), dict(refs=None), dict(n_seqs=0), dict(n_seqs=4097), dict(max_pages=0), dict(n_pages=0),
          dict(ps=24), dict(max_pages=1 << 25), dict(n_seqs=4096, max_pages=1 << 19, ps=16)]
 ROWS = STATE + [dict(lens=None), dict(new=None)]
-MOVING = CACHE + [dict(layers=0)]
+MOVING = CACHE + [dict(layers=0), dict(layers=4097)]
 WS = [dict(ws=None), dict(ws=A + 4), dict(wsb=16)]
 
 
