@@ -25,7 +25,8 @@ def _dev(t: torch.Tensor, name: str, dtype: torch.dtype | None = None) -> int:
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    # torch.cuda.current_stream().cuda_stream without the Stream object (2.8 us a call)
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def row_bytes(type_id: int, n_cols: int) -> int:
@@ -486,39 +487,62 @@ def paged_cache_bytes(n_pages: int, page_size: int, n_kv_heads: int, head_dim: i
     return int(load_library().mnemo_paged_cache_bytes(n_pages, page_size, n_kv_heads, head_dim, kv_type))
 
 
-def _need(t, n: int, name: str) -> None:
-    if t.numel() < n:
-        raise MnemoError(f"{name}: {t.numel()} elements < {n}")
+_gpus = 0  # visible GPUs, asked for once
+
+
+def _arg(t, name: str, dtype: torch.dtype | None = None, n: int = 0) -> int:
+    """The address of a contiguous tensor on the current GPU with at least n elements."""
+    try:
+        # the order of the checks is that of their use; each costs ~0.06 us, a call has up to 20 tensors
+        if t.is_cuda and (dtype is None or t.dtype is dtype) and t.is_contiguous() and t.numel() >= n:
+            if _gpus == 1 or t.get_device() == _current_gpu():
+                return t.data_ptr()
+            raise MnemoError(f"{name} must be on the current GPU")
+    except AttributeError:
+        pass
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise MnemoError(f"{name} must be a GPU tensor")
+    if dtype is not None and t.dtype != dtype:
+        raise MnemoError(f"{name} must be {dtype}, got {t.dtype}")
+    if not t.is_contiguous():
+        raise MnemoError(f"{name} must be contiguous")
+    raise MnemoError(f"{name}: {t.numel()} elements < {n}")
+
+
+def _current_gpu() -> int:
+    global _gpus
+    _gpus = torch.cuda.device_count()
+    return torch._C._cuda_getDevice()
+
+
+def _opt_arg(t, name: str, dtype: torch.dtype | None = None, n: int = 0) -> int | None:
+    return None if t is None else _arg(t, name, dtype, n)
 
 
 def _pages(k, v, ks, vs, layers: bool):
     """The arguments (pointers, kv_type) and shape (n_layers, n_pages, n_kv_heads, page_size, head_dim) of cache
     pages k [..., n_kv_heads, page_size, head_dim] and v [..., n_kv_heads, head_dim, page_size]."""
-    nd = 5 if layers else 4
-    if k.dtype not in (torch.float16, torch.int8) or v.dtype != k.dtype:
-        raise MnemoError(f"pages must be float16 or int8, got {k.dtype} and {v.dtype}")
-    if k.dim() != nd or tuple(v.shape) != (*k.shape[:-2], k.shape[-1], k.shape[-2]):
-        raise MnemoError(f"pages: k {tuple(k.shape)} and v {tuple(v.shape)} do not fit ({nd} dimensions, v transposed)")
-    kv_type = int(k.dtype == torch.int8)
-    if kv_type:
-        if ks is None or vs is None:
-            raise MnemoError("int8 pages need scales")
-        _need(ks, k.numel() // k.shape[-1], "k_scales")
-        _need(vs, k.numel() // k.shape[-1], "v_scales")
-    n_layers = k.shape[0] if layers else 1
-    ptrs = (_dev(k, "k_pages"), _dev(v, "v_pages"), _opt(ks if kv_type else None, "k_scales", F32),
-            _opt(vs if kv_type else None, "v_scales", F32), kv_type)
-    return ptrs, (n_layers, *k.shape[-4:])
+    shape = k.shape
+    if len(shape) != (5 if layers else 4) or v.shape != (*shape[:-2], shape[-1], shape[-2]):
+        raise MnemoError(f"pages: k {tuple(shape)} and v {tuple(v.shape)} do not fit ({5 if layers else 4} dimensions, "
+                         "v transposed)")
+    if k.dtype == torch.float16:
+        return (_arg(k, "k_pages"), _arg(v, "v_pages", torch.float16), None, None, 0), (shape[0] if layers else 1,
+                                                                                        *shape[-4:])
+    if k.dtype != torch.int8:
+        raise MnemoError(f"pages must be float16 or int8, got {k.dtype}")
+    if ks is None or vs is None:
+        raise MnemoError("int8 pages need scales")
+    n = k.numel() // max(shape[-1], 1)
+    return (_arg(k, "k_pages"), _arg(v, "v_pages", torch.int8), _arg(ks, "k_scales", F32, n),
+            _arg(vs, "v_scales", F32, n), 1), (shape[0] if layers else 1, *shape[-4:])
 
 
-def _rows(table, *per_row):
-    """(n_seqs, max_pages) of a block table; per_row: (tensor, name) with one int32 per row."""
+def _rows(table):
+    """(address, n_seqs, max_pages) of a block table."""
     if table.dim() != 2:
         raise MnemoError(f"block_table must have 2 dimensions, got {table.dim()}")
-    for t, name in per_row:
-        _dev(t, name, I32)
-        _need(t, table.shape[0], name)
-    return table.shape
+    return _arg(table, "block_table", I32), *table.shape
 
 
 def paged_attn_prep(q, k, v, qw, kw, eps: float, theta: float, k_pages, v_pages, block_table, q_out, positions=None,
@@ -528,21 +552,17 @@ def paged_attn_prep(q, k, v, qw, kw, eps: float, theta: float, k_pages, v_pages,
     row seq_ids[t] of the block table; without them it is the last position of row t (seq_lens[t] - 1)."""
     lib = load_library()
     ptrs, (_, n_pages, nkv, ps, hd) = _pages(k_pages, v_pages, ks, vs, False)
-    n_seqs, max_pages = _rows(block_table, *(((seq_lens, "seq_lens"),) if seq_lens is not None else ()))
-    T, nh = q.shape[0], q.shape[1]
-    if tuple(q.shape) != (T, nh, hd) or tuple(k.shape) != (T, nkv, hd) or v.shape != k.shape or q_out.shape != q.shape:
+    table, n_seqs, max_pages = _rows(block_table)
+    if q.dim() != 3 or q.shape[2] != hd or k.shape != (q.shape[0], nkv, hd) or v.shape != k.shape \
+            or q_out.shape != q.shape:
         raise MnemoError("paged_attn_prep: q, k, v and q_out must be [T, heads, head_dim]")
-    for t, name in ((positions, "positions"), (seq_ids, "seq_ids")):
-        if t is not None:
-            _need(t, T, name)
-    for t, name in ((qw, "qw"), (kw, "kw")):
-        if t is not None:
-            _need(t, hd, name)
+    T, nh = q.shape[0], q.shape[1]
     rc = lib.mnemo_paged_attn_prep(
-        _dev(q, "q", F32), _dev(k, "k", F32), _dev(v, "v", F32), _opt(qw, "qw", F32), _opt(kw, "kw", F32), float(eps),
-        float(theta), T, nh, hd, nkv, _opt(positions, "positions", I32), _opt(seq_ids, "seq_ids", I32),
-        _dev(block_table, "block_table", I32), _opt(seq_lens, "seq_lens", I32), n_seqs, max_pages, *ptrs, n_pages, ps,
-        _dev(q_out, "q_out", F32), _stream())
+        _arg(q, "q", F32), _arg(k, "k", F32), _arg(v, "v", F32), _opt_arg(qw, "qw", F32, hd),
+        _opt_arg(kw, "kw", F32, hd), float(eps), float(theta), T, nh, hd, nkv,
+        _opt_arg(positions, "positions", I32, T), _opt_arg(seq_ids, "seq_ids", I32, T), table,
+        _opt_arg(seq_lens, "seq_lens", I32, n_seqs), n_seqs, max_pages, *ptrs, n_pages, ps, _arg(q_out, "q_out", F32),
+        _stream())
     _check_rc(lib, rc, "mnemo_paged_attn_prep")
 
 
@@ -555,33 +575,33 @@ def paged_attention_decode(q, k_pages, v_pages, block_table, seq_lens, out, scal
     table holds (zeros for an empty row)."""
     lib = load_library()
     ptrs, (_, n_pages, nkv, ps, hd) = _pages(k_pages, v_pages, ks, vs, False)
-    n_seqs, max_pages = _rows(block_table, (seq_lens, "seq_lens"))
+    table, n_seqs, max_pages = _rows(block_table)
     if q.dim() != 3 or q.shape[0] != n_seqs or q.shape[2] != hd or out.shape != q.shape:
         raise MnemoError("paged_attention_decode: q and out must be [n_seqs, n_heads, head_dim]")
     rc = lib.mnemo_paged_attention_decode(
-        _dev(q, "q", F32), *ptrs, _dev(out, "out", F32), n_seqs, q.shape[1], hd, nkv, n_pages, ps,
-        _dev(block_table, "block_table", I32), max_pages, seq_lens.data_ptr(), float(scale), _dev(ws, "ws"),
-        ws.numel() * ws.element_size(), _stream())
+        _arg(q, "q", F32), *ptrs, _arg(out, "out", F32), n_seqs, q.shape[1], hd, nkv, n_pages, ps, table, max_pages,
+        _arg(seq_lens, "seq_lens", I32, n_seqs), float(scale), _arg(ws, "ws"), ws.numel() * ws.element_size(),
+        _stream())
     _check_rc(lib, rc, "mnemo_paged_attention_decode")
 
 
 def kv_pages_extend(block_table, seq_lens, page_refs, new_lens, page_size: int, status=None):
     """Gives pages to every row with new_lens > seq_lens; status[0] = rows that could not be served."""
     lib = load_library()
-    n_seqs, max_pages = _rows(block_table, (seq_lens, "seq_lens"), (new_lens, "new_lens"))
-    rc = lib.mnemo_kv_pages_extend(_dev(block_table, "block_table", I32), seq_lens.data_ptr(),
-                                   _dev(page_refs, "page_refs", I32), new_lens.data_ptr(), n_seqs, max_pages,
-                                   page_refs.numel(), int(page_size), _opt(status, "status", I32), _stream())
+    table, n_seqs, max_pages = _rows(block_table)
+    rc = lib.mnemo_kv_pages_extend(table, _arg(seq_lens, "seq_lens", I32, n_seqs), _arg(page_refs, "page_refs", I32),
+                                   _arg(new_lens, "new_lens", I32, n_seqs), n_seqs, max_pages, page_refs.numel(),
+                                   int(page_size), _opt_arg(status, "status", I32, 1), _stream())
     _check_rc(lib, rc, "mnemo_kv_pages_extend")
 
 
 def kv_pages_free(block_table, seq_lens, page_refs, gone, page_size: int):
     """Drops the pages of every row with gone != 0."""
     lib = load_library()
-    n_seqs, max_pages = _rows(block_table, (seq_lens, "seq_lens"), (gone, "gone"))
-    rc = lib.mnemo_kv_pages_free(_dev(block_table, "block_table", I32), seq_lens.data_ptr(),
-                                 _dev(page_refs, "page_refs", I32), gone.data_ptr(), n_seqs, max_pages,
-                                 page_refs.numel(), int(page_size), _stream())
+    table, n_seqs, max_pages = _rows(block_table)
+    rc = lib.mnemo_kv_pages_free(table, _arg(seq_lens, "seq_lens", I32, n_seqs), _arg(page_refs, "page_refs", I32),
+                                 _arg(gone, "gone", I32, n_seqs), n_seqs, max_pages, page_refs.numel(),
+                                 int(page_size), _stream())
     _check_rc(lib, rc, "mnemo_kv_pages_free")
 
 
@@ -594,12 +614,12 @@ def kv_pages_fork(block_table, seq_lens, page_refs, parents, k_pages, v_pages, s
     copied in all layers of k_pages / v_pages [n_layers, n_pages, ...]; status[0] = rows that could not be served."""
     lib = load_library()
     ptrs, (n_layers, n_pages, nkv, ps, hd) = _pages(k_pages, v_pages, ks, vs, True)
-    n_seqs, max_pages = _rows(block_table, (seq_lens, "seq_lens"), (parents, "parents"))
-    _need(page_refs, n_pages, "page_refs")
-    rc = lib.mnemo_kv_pages_fork(_dev(block_table, "block_table", I32), seq_lens.data_ptr(),
-                                 _dev(page_refs, "page_refs", I32), parents.data_ptr(), n_seqs, max_pages, *ptrs,
-                                 n_layers, n_pages, ps, nkv, hd, _opt(status, "status", I32), _dev(ws, "ws"),
-                                 ws.numel() * ws.element_size(), _stream())
+    table, n_seqs, max_pages = _rows(block_table)
+    rc = lib.mnemo_kv_pages_fork(table, _arg(seq_lens, "seq_lens", I32, n_seqs),
+                                 _arg(page_refs, "page_refs", I32, n_pages), _arg(parents, "parents", I32, n_seqs),
+                                 n_seqs, max_pages, *ptrs, n_layers, n_pages, ps, nkv, hd,
+                                 _opt_arg(status, "status", I32, 1), _arg(ws, "ws"), ws.numel() * ws.element_size(),
+                                 _stream())
     _check_rc(lib, rc, "mnemo_kv_pages_fork")
 
 
@@ -607,11 +627,10 @@ def kv_pages_compact(block_table, page_refs, k_pages, v_pages, n_live, ws, ks=No
     """Moves the pages in use to the front of the pool, in all layers; n_live[0] = their number."""
     lib = load_library()
     ptrs, (n_layers, n_pages, nkv, ps, hd) = _pages(k_pages, v_pages, ks, vs, True)
-    n_seqs, max_pages = _rows(block_table)
-    _need(page_refs, n_pages, "page_refs")
-    rc = lib.mnemo_kv_pages_compact(_dev(block_table, "block_table", I32), _dev(page_refs, "page_refs", I32), n_seqs,
-                                    max_pages, *ptrs, n_layers, n_pages, ps, nkv, hd, _opt(n_live, "n_live", I32),
-                                    _dev(ws, "ws"), ws.numel() * ws.element_size(), _stream())
+    table, n_seqs, max_pages = _rows(block_table)
+    rc = lib.mnemo_kv_pages_compact(table, _arg(page_refs, "page_refs", I32, n_pages), n_seqs, max_pages, *ptrs,
+                                    n_layers, n_pages, ps, nkv, hd, _opt_arg(n_live, "n_live", I32, 1),
+                                    _arg(ws, "ws"), ws.numel() * ws.element_size(), _stream())
     _check_rc(lib, rc, "mnemo_kv_pages_compact")
 
 
@@ -621,7 +640,7 @@ def kv_pages_copy(src, dst, k_pages, v_pages, ks=None, vs=None):
     ptrs, (n_layers, n_pages, nkv, ps, hd) = _pages(k_pages, v_pages, ks, vs, True)
     if src.numel() != dst.numel():
         raise MnemoError("kv_pages_copy: src and dst differ in length")
-    rc = lib.mnemo_kv_pages_copy(_dev(src, "src", I32), _dev(dst, "dst", I32), src.numel(), *ptrs, n_layers, n_pages,
+    rc = lib.mnemo_kv_pages_copy(_arg(src, "src", I32), _arg(dst, "dst", I32), src.numel(), *ptrs, n_layers, n_pages,
                                  ps, nkv, hd, _stream())
     _check_rc(lib, rc, "mnemo_kv_pages_copy")
 
@@ -636,25 +655,19 @@ def logits_process(logits, out, history=None, history_lens=None, prompt_lens=Non
     if logits.dim() != 2 or out.shape != logits.shape:
         raise MnemoError("logits_process: logits and out must be [n, vocab]")
     n, vocab = logits.shape
-    max_history = n_bias = 0
+    h = (None, None, None, 0, None, None, None)
     if history is not None:
         if history.dim() != 2 or history.shape[0] != n:
             raise MnemoError("logits_process: history must be [n, max_history]")
-        max_history = history.shape[1]
-        for t, name in ((history_lens, "history_lens"), (prompt_lens, "prompt_lens"), (repetition, "repetition"),
-                        (frequency, "frequency"), (presence, "presence")):
-            if t is None:
-                raise MnemoError(f"logits_process: history needs {name}")
-            _need(t, n, name)
+        h = (_arg(history, "history", I32), _arg(history_lens, "history_lens", I32, n),
+             _arg(prompt_lens, "prompt_lens", I32, n), history.shape[1], _arg(repetition, "repetition", F32, n),
+             _arg(frequency, "frequency", F32, n), _arg(presence, "presence", F32, n))
+    b = (None, None, 0)
     if bias_ids is not None:
         if bias is None or bias_ids.dim() != 2 or bias_ids.shape[0] != n or bias.shape != bias_ids.shape:
             raise MnemoError("logits_process: bias_ids and bias must be [n, n_bias]")
-        n_bias = bias_ids.shape[1]
-    if allowed is not None:
-        _need(allowed, n * ((vocab + 31) // 32), "allowed")
+        b = (_arg(bias_ids, "bias_ids", I32), _arg(bias, "bias", F32), bias_ids.shape[1])
     rc = lib.mnemo_logits_process(
-        _dev(logits, "logits", F32), _dev(out, "out", F32), n, vocab, _opt(history, "history", I32),
-        _opt(history_lens, "history_lens", I32), _opt(prompt_lens, "prompt_lens", I32), max_history,
-        _opt(repetition, "repetition", F32), _opt(frequency, "frequency", F32), _opt(presence, "presence", F32),
-        _opt(bias_ids, "bias_ids", I32), _opt(bias, "bias", F32), n_bias, _opt(allowed, "allowed", I32), _stream())
+        _arg(logits, "logits", F32), _arg(out, "out", F32), n, vocab, *h, *b,
+        _opt_arg(allowed, "allowed", I32, n * ((vocab + 31) // 32)), _stream())
     _check_rc(lib, rc, "mnemo_logits_process")
