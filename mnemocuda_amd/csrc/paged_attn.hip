@@ -159,7 +159,7 @@ __device__ __forceinline__ h8 cvt8(uint32_t a, uint32_t b) {
 }
 
 template <int KV, int HD>
-__global__ void __launch_bounds__((PaShape<KV, HD>::kThreads)) paged_attn_kernel(PagedAttnArgs a) {
+__global__ void __launch_bounds__((PaShape<KV, HD>::kThreads)) paged_attn_kernel(PagedAttnArgs a, int whole_pairs) {
     using S = PaShape<KV, HD>;
     constexpr int STEP = S::kStep, NT = S::kTiles, KS = S::kKs, ND = S::kNd, NW = S::kWaves;
     constexpr int EB = KV == kKvF16 ? 2 : 1;
@@ -175,12 +175,22 @@ __global__ void __launch_bounds__((PaShape<KV, HD>::kThreads)) paged_attn_kernel
 
     const PaPlan plan = pa_plan<STEP, NW>(a, gridDim.x);
     // the workgroup's steps, shared out to its waves in the same way
-    const int g0 = pa_first(plan, blockIdx.x), gn = pa_first(plan, blockIdx.x + 1) - g0;
-    const int each = gn / plan.nw, odd = gn - each * plan.nw;
+    int g0 = pa_first(plan, blockIdx.x), g1 = pa_first(plan, blockIdx.x + 1);
+    int nw = plan.nw, seq = 0, kvh = 0, step = 0, len = 0;
+    if (whole_pairs) {  // both ends move up to the next (sequence, KV head)'s beginning
+        nw = min(NW, 4);
+        auto up = [&](int u) {
+            if (u >= plan.total) return plan.total;
+            pa_find<STEP>(a, plan, u, seq, kvh, step, len);
+            return step > 0 ? u + (len + STEP - 1) / STEP - step : u;
+        };
+        g0 = up(g0);
+        g1 = up(g1);
+    }
+    const int each = (g1 - g0) / nw, odd = g1 - g0 - each * nw;
     int at = g0 + wave * each + min(wave, odd);
-    const int end = wave < plan.nw ? at + each + (wave < odd) : at;
+    const int end = wave < nw ? at + each + (wave < odd) : at;
     if (lane < 2) pair_of[wave][lane] = -1;
-    int seq = 0, kvh = 0, step = 0, len = 0;
     if (at < end) pa_find<STEP>(a, plan, at, seq, kvh, step, len);
 
     while (at < end) {
@@ -407,10 +417,13 @@ __global__ void __launch_bounds__((PaShape<KV, HD>::kThreads)) paged_attn_kernel
             while (len == 0);  // a step is left, so a sequence with positions is
         }
     }
-    if (__any(plan.empty))
-        for (int s = blockIdx.x * NW + wave; s < a.n_seqs; s += gridDim.x * NW)
-            if (seq_len(a, s) == 0)
-                for (int i = lane; i < a.nh * HD; i += 64) a.out[(size_t)s * a.nh * HD + i] = 0.0f;
+    if (__any(plan.empty))  // sequences with no positions: zeros, a KV head's query heads by a wave
+        for (int i = blockIdx.x * NW + wave; i < a.n_seqs * a.c.nkv; i += gridDim.x * NW)
+            if (seq_len(a, i / a.c.nkv) == 0) {
+                const f4 zero = {};
+                float *out = a.out + (size_t)i * a.gqa * HD;
+                for (int e = 4 * lane; e < a.gqa * HD; e += 256) __builtin_memcpy(out + e, &zero, 16);
+            }
 
     // ---- pieces of one (sequence, KV head), from consecutive waves, are merged.  Lane i holds piece
     // (i / 2, i % 2).  A chain begins with a piece 1, or with piece 0 of the first wave, and takes in
@@ -431,18 +444,19 @@ __global__ void __launch_bounds__((PaShape<KV, HD>::kThreads)) paged_attn_kernel
         const uint32_t in = pieces & 0x55555555u & ~((2u << first) - 1) & (rest ? (rest & (0u - rest)) - 1 : ~0u);
         const int w = first >> 1, k = first & 1, n = __popc(in);
         const bool whole = k == 1 && (in & closed);
-        float mm = lm[w][k][h], sum = ll[w][k][h];
-        f4 x;
-        __builtin_memcpy(&x, &lo[w][k][h][d], 16);
-        for (int i = 1; i <= n; i++) {
-            const float pm = lm[w + i][0][h], mn = fmaxf(mm, pm);
+        float mm = lm[w][k][h];
+#pragma unroll 4
+        for (int i = 1; i <= n; i++) mm = fmaxf(mm, lm[w + i][0][h]);
+        f4 x = {};
+        float sum = 0.0f;
+#pragma unroll 4
+        for (int i = 0; i <= n; i++) {
+            const int ki = i ? 0 : k;
+            const float f = mm == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lm[w + i][ki][h] - mm);
             f4 y;
-            __builtin_memcpy(&y, &lo[w + i][0][h][d], 16);
-            if (mn == -INFINITY) continue;
-            const float fa = __builtin_amdgcn_exp2f(mm - mn), fb = __builtin_amdgcn_exp2f(pm - mn);
-            x = x * fa + y * fb;
-            sum = fmaf(sum, fa, ll[w + i][0][h] * fb);
-            mm = mn;
+            __builtin_memcpy(&y, &lo[w + i][ki][h][d], 16);
+            x += y * f;
+            sum = fmaf(ll[w + i][ki][h], f, sum);
         }
         const int pr = pair_of[w][k];
         if (whole) {
@@ -565,8 +579,12 @@ static void launch_pa(const PagedAttnArgs &a, hipStream_t s) {
     const long long pairs = (long long)a.n_seqs * a.c.nkv;
     const long long most = pairs * (((long long)a.max_pages * a.c.ps + S::kStep - 1) / S::kStep);  // steps
     const int groups = (int)(most < kPaGroups ? most : kPaGroups);
-    hipLaunchKernelGGL((paged_attn_kernel<KV, HD>), dim3(groups), dim3(S::kThreads), 0, s, a);
-    if (groups == 1) return;
+    // Tables of up to four steps: no (sequence, KV head) is cut between workgroups, and nothing is left to merge (100
+    // sequences to 60 positions 7.0 us against 9.2 with the merge launch).  Longer ones are cut: a CU alone loads no
+    // more than ~20 GB/s, and 300 positions of one sequence take 11.3 us on 4 CUs against 8.3 on 40.
+    const bool whole_pairs = most <= 4 * pairs;
+    hipLaunchKernelGGL((paged_attn_kernel<KV, HD>), dim3(groups), dim3(S::kThreads), 0, s, a, (int)whole_pairs);
+    if (whole_pairs) return;
     // few (sequence, KV head)s: long chains, a workgroup for each head; many: short ones, found by the shares' ends
     if (pairs < groups)
         hipLaunchKernelGGL((paged_merge_kernel<S::kStep, HD, S::kWaves, CHAIN, false>), dim3((int)pairs, a.gqa), dim3(256),
