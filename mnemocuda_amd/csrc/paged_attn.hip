@@ -13,7 +13,7 @@ namespace mnemo {
 // ------------------------------------------------------------------ attention
 // out[s][h] = sum_p P_p v_p / sum_p P_p,  P_p = exp(scale q.k_p - m), over the positions of row s.
 //
-// The work is cut into steps of kStep positions of one (sequence, KV head), in that order, and the
+// The work is cut into steps of STEP positions of one (sequence, KV head), in that order, and the
 // waves of the launch take equal shares of the row of steps, whatever the lengths are: every wave
 // computes its share from the lengths itself.  A (sequence, KV head) that lies within one share
 // is finished there; pieces of one that several shares cut meet in LDS where the shares belong to
@@ -22,9 +22,15 @@ namespace mnemo {
 // A wave streams its steps with no exchange with others and no LDS: S^T = K Q^T (positions x heads)
 // comes out of the matrix instruction with a lane holding four positions of one head, which is how
 // O^T = V^T P^T (dims x heads) wants P^T, when the K rows of a tile are picked so: lane row m of
-// tile t is position (kStep/4)(m/4) + 4t + m%4, so that a lane's rows over the tiles are kStep/4
+// tile t is position (STEP/4)(m/4) + 4t + m%4, so that a lane's rows over the tiles are STEP/4
 // consecutive positions.  K fragments are 16 bytes of a K row, V fragments 16 bytes of positions of
 // one dim.
+//
+// Bound by memory: 96 sequences to 8192 positions (957 MB) take 172 us, 5.5 TB/s, where a plain read of
+// as much reaches 6.2; 3 int8 sequences to 131,072 (324 MB) 67.5 us.  A CU has room for one workgroup and
+// ~20 GB/s of loads, so shares are spread over the CUs first; what a small call takes is its chain of
+// loads: lengths, table, K, V, then the same for the merge (300 positions: 8.5 us, of which 3 are the
+// second launch).
 //
 // Precision: Q is scaled by a power of two into [1, 2) per head and split into two f16 parts, P
 // likewise split; K and V enter exactly (f16 or int8).  P is formed relative to a reference that
@@ -40,13 +46,14 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 constexpr int kPaRows = 16;
 constexpr float kSlack = 5.0f, kLift = 9.0f;  // powers of two: P <= 2^14, times a scale below 2
 
-template <int KV, int HD>
+template <int KV, int HD, int STEP>
 struct PaShape {
-    static constexpr int kStep = KV == kKvF16 ? 32 : 64;  // positions of a wave's step
-    static constexpr int kTiles = kStep / 16;
+    static constexpr int kTiles = STEP / 16;
     static constexpr int kKs = HD / 32, kNd = HD / 16;  // dim steps of S, dim tiles of O
     // one workgroup per CU; its pieces fill LDS (135 KB at head_dim 128)
-    static constexpr int kWaves = HD == 256 ? 4 : HD == 64 && KV == kKvF16 ? 16 : 8;
+    static constexpr int kWaves = HD == 256 ? 4 : 8;
+    // the parts of Q wait in LDS where registers are short
+    static constexpr bool kQInLds = HD == 128 && STEP == 64;
     static constexpr int kThreads = 64 * kWaves;
 };
 
@@ -70,7 +77,7 @@ struct PaPlan {
     int before;  // lane: steps before its sequences
 };
 
-// The CUs are filled before the waves of a workgroup: a CU alone takes ~1 us for 8 steps.
+// The CUs are filled before the waves of a workgroup: eight steps on one CU end ~4 us after a step alone.
 template <int STEP, int NW>
 __device__ __forceinline__ PaPlan pa_plan(const PagedAttnArgs &a, int groups) {
     PaPlan p;
@@ -158,11 +165,12 @@ __device__ __forceinline__ h8 cvt8(uint32_t a, uint32_t b) {
     return __builtin_shufflevector(cvt4(a), cvt4(b), 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-template <int KV, int HD>
-__global__ void __launch_bounds__((PaShape<KV, HD>::kThreads)) paged_attn_kernel(PagedAttnArgs a, int whole_pairs) {
-    using S = PaShape<KV, HD>;
-    constexpr int STEP = S::kStep, NT = S::kTiles, KS = S::kKs, ND = S::kNd, NW = S::kWaves;
+template <int KV, int HD, int STEP>
+__global__ void __launch_bounds__((PaShape<KV, HD, STEP>::kThreads)) paged_attn_kernel(PagedAttnArgs a, int whole_pairs) {
+    using S = PaShape<KV, HD, STEP>;
+    constexpr int NT = S::kTiles, KS = S::kKs, ND = S::kNd, NW = S::kWaves;
     constexpr int EB = KV == kKvF16 ? 2 : 1;
+    constexpr int VW = STEP / 4 * EB / 16;  // 16-byte words of a dim's positions per lane
     constexpr int PV = STEP / 32;  // position steps of O
     // pieces of cut (sequence, KV head)s: [.][0] one that began before the wave's share, [.][1] one
     // that begins in it and goes on
@@ -208,7 +216,7 @@ __global__ void __launch_bounds__((PaShape<KV, HD>::kThreads)) paged_attn_kernel
             e.v = table[min((p0 + STEP / 4 * kg) >> psl, last)];
             return e;
         };
-        u4 kr[NT][HD * EB / 64], vr[ND];
+        u4 kr[NT][HD * EB / 64], vr[ND][VW];
         float ksc[KV == kKvInt8 ? 16 : 1], vsc[KV == kKvInt8 ? 16 : 1];
         auto load_k = [&](int p0, int page) {
             const int row = ((p0 + STEP / 4 * (r >> 2)) & (ps - 1)) + (r & 3);
@@ -224,7 +232,9 @@ __global__ void __launch_bounds__((PaShape<KV, HD>::kThreads)) paged_attn_kernel
             page = (unsigned)page < (unsigned)a.c.n_pages ? page : 0;
             const uint8_t *base = vc + ((((size_t)page * a.c.nkv + kvh) * HD + r) * ps + off) * EB;
 #pragma unroll
-            for (int i = 0; i < ND; i++) __builtin_memcpy(&vr[i], base + (size_t)16 * i * ps * EB, 16);
+            for (int i = 0; i < ND; i++)
+#pragma unroll
+                for (int j = 0; j < VW; j++) __builtin_memcpy(&vr[i][j], base + (size_t)16 * i * ps * EB + 16 * j, 16);
         };
         auto load_scales = [&](int p0, int page) {
             const int off = (p0 + STEP / 4 * kg) & (ps - 1);
@@ -267,22 +277,33 @@ __global__ void __launch_bounds__((PaShape<KV, HD>::kThreads)) paged_attn_kernel
             const float qs = ldexpf(1.0f, -qe);
             const float c = ldexpf(a.scale * 1.44269504088896341f, qe);
             h8 qhi[KS], qlo[KS];
+            // in LDS they wait where the wave's last piece goes in the end
+            uint8_t *ql = (uint8_t *)&lo[wave][1][0][0] + 16 * lane;
 #pragma unroll
-            for (int st = 0; st < KS; st++)
+            for (int st = 0; st < KS; st++) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const float x = q[st][j] * qs;
                     qhi[st][j] = (_Float16)x;
                     qlo[st][j] = (_Float16)(x - (float)qhi[st][j]);
                 }
+                if (S::kQInLds) {
+                    __builtin_memcpy(ql + 2048 * st, &qhi[st], 16);
+                    __builtin_memcpy(ql + 2048 * st + 1024, &qlo[st], 16);
+                }
+            }
             for (;;) {
                 // ---- S^T: lane: head r, positions p0 + STEP/4 kg + 4t + i
-                f4 s[NT];
+                f4 s[NT] = {};
 #pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    s[t] = f4{0.f, 0.f, 0.f, 0.f};
+                for (int st = 0; st < KS; st++) {
+                    if (S::kQInLds) {
+                        asm volatile("" ::: "memory");  // read again every step
+                        __builtin_memcpy(&qhi[st], ql + 2048 * st, 16);
+                        __builtin_memcpy(&qlo[st], ql + 2048 * st + 1024, 16);
+                    }
 #pragma unroll
-                    for (int st = 0; st < KS; st++) {
+                    for (int t = 0; t < NT; t++) {
                         h8 kf;
                         if (KV == kKvF16) kf = __builtin_bit_cast(h8, kr[t][st]);
                         else kf = cvt8(kr[t][st >> 1][2 * (st & 1)], kr[t][st >> 1][2 * (st & 1) + 1]);
@@ -356,11 +377,11 @@ __global__ void __launch_bounds__((PaShape<KV, HD>::kThreads)) paged_attn_kernel
 #pragma unroll
                     for (int i = 0; i < ND; i++)
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            uint32_t w = vr[i][j];
+                        for (int j = 0; j < 4 * VW; j++) {
+                            uint32_t w = vr[i][j / 4][j % 4];
                             if (!ok || live <= 2 * j) w = 0;
                             else if (live == 2 * j + 1) w &= 0xffffu;
-                            vr[i][j] = w;
+                            vr[i][j / 4][j % 4] = w;
                         }
                 }
 #pragma unroll
@@ -368,8 +389,8 @@ __global__ void __launch_bounds__((PaShape<KV, HD>::kThreads)) paged_attn_kernel
 #pragma unroll
                     for (int k = 0; k < PV; k++) {
                         h8 vf;
-                        if (KV == kKvF16) vf = __builtin_bit_cast(h8, vr[i]);
-                        else vf = cvt8(vr[i][2 * k], vr[i][2 * k + 1]);
+                        if (KV == kKvF16) vf = __builtin_bit_cast(h8, vr[i][k]);
+                        else vf = cvt8(vr[i][0][2 * k], vr[i][0][2 * k + 1]);
                         o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, phi[k], o[i], 0, 0, 0);
                         o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, plo[k], o[i], 0, 0, 0);
                     }
@@ -572,38 +593,39 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnArgs a, int g
     }
 }
 
-template <int KV, int HD>
+template <int KV, int HD, int STEP>
 static void launch_pa(const PagedAttnArgs &a, hipStream_t s) {
-    using S = PaShape<KV, HD>;
+    using S = PaShape<KV, HD, STEP>;
     constexpr int CHAIN = 1024 / HD;  // 256 threads for one head
     const long long pairs = (long long)a.n_seqs * a.c.nkv;
-    const long long most = pairs * (((long long)a.max_pages * a.c.ps + S::kStep - 1) / S::kStep);  // steps
+    const long long most = pairs * (((long long)a.max_pages * a.c.ps + STEP - 1) / STEP);  // steps
     const int groups = (int)(most < kPaGroups ? most : kPaGroups);
     // Tables of up to four steps: no (sequence, KV head) is cut between workgroups, and nothing is left to merge (100
     // sequences to 60 positions 7.0 us against 9.2 with the merge launch).  Longer ones are cut: a CU alone loads no
     // more than ~20 GB/s, and 300 positions of one sequence take 11.3 us on 4 CUs against 8.3 on 40.
     const bool whole_pairs = most <= 4 * pairs;
-    hipLaunchKernelGGL((paged_attn_kernel<KV, HD>), dim3(groups), dim3(S::kThreads), 0, s, a, (int)whole_pairs);
+    hipLaunchKernelGGL((paged_attn_kernel<KV, HD, STEP>), dim3(groups), dim3(S::kThreads), 0, s, a, (int)whole_pairs);
     if (whole_pairs) return;
     // few (sequence, KV head)s: long chains, a workgroup for each head; many: short ones, found by the shares' ends
     if (pairs < groups)
-        hipLaunchKernelGGL((paged_merge_kernel<S::kStep, HD, S::kWaves, CHAIN, false>), dim3((int)pairs, a.gqa), dim3(256),
+        hipLaunchKernelGGL((paged_merge_kernel<STEP, HD, S::kWaves, CHAIN, false>), dim3((int)pairs, a.gqa), dim3(256),
                            0, s, a, groups);
     else
-        hipLaunchKernelGGL((paged_merge_kernel<S::kStep, HD, S::kWaves, 1, true>), dim3(groups - 1, 1), dim3(256), 0, s, a,
+        hipLaunchKernelGGL((paged_merge_kernel<STEP, HD, S::kWaves, 1, true>), dim3(groups - 1, 1), dim3(256), 0, s, a,
                            groups);
 }
 
 int launch_paged_attention(const PagedAttnArgs &a, hipStream_t s) {
-#define MNEMO_PA(HD_)                                      \
-    do {                                                   \
-        if (a.c.kv_type == kKvF16) launch_pa<kKvF16, HD_>(a, s); \
-        else launch_pa<kKvInt8, HD_>(a, s);                \
-    } while (0)
-    if (a.c.hd == 64) MNEMO_PA(64);
-    else if (a.c.hd == 128) MNEMO_PA(128);
-    else MNEMO_PA(256);
-#undef MNEMO_PA
+    const bool f16 = a.c.kv_type == kKvF16;
+    // Steps of 64 positions read whole lines of V where pages hold 64 or more, and halve what a step costs besides its
+    // loads: 96 sequences to 8192 (8 KV heads of 128) 173.7 us against 188.0 with steps of 32, one of 32,768 20.7
+    // against 23.2.  Few steps are spread thinner by 32: 300 positions 8.4 us against 9.3, 100 sequences to 60
+    // positions 7.2 against 8.0; 40 to 250, 2 KV heads of 256, 11.3 against 16.2 (to 8192: 37.1 against 33.9).
+    const bool few = (long long)a.n_seqs * a.c.nkv * a.max_pages * a.c.ps <= 32 * 1024;
+    if (a.c.hd == 64) f16 ? launch_pa<kKvF16, 64, 64>(a, s) : launch_pa<kKvInt8, 64, 64>(a, s);
+    else if (!f16) a.c.hd == 128 ? launch_pa<kKvInt8, 128, 64>(a, s) : launch_pa<kKvInt8, 256, 64>(a, s);
+    else if (a.c.hd == 128) few ? launch_pa<kKvF16, 128, 32>(a, s) : launch_pa<kKvF16, 128, 64>(a, s);
+    else few ? launch_pa<kKvF16, 256, 32>(a, s) : launch_pa<kKvF16, 256, 64>(a, s);
     return check_launch("paged_attention_decode");
 }
 

@@ -87,10 +87,11 @@ EDGES = [0, 1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 257, 6
     (128, 64, 4, 16, False), (128, 64, 4, 16, True), (128, 16, 2, 5, False), (128, 16, 2, 5, True),
     (128, 32, 1, 1, False), (128, 128, 3, 8, True), (64, 16, 2, 7, False), (64, 64, 12, 1, False),
     (64, 32, 2, 16, True), (256, 16, 1, 16, False), (256, 64, 2, 3, False), (256, 128, 1, 4, True)])
-def test_attention_at_the_edges(gpu, hd, ps, nkv, G, int8):
+@pytest.mark.parametrize("wide", [False, True])  # tables far wider than the lengths: the kernels of long ones
+def test_attention_at_the_edges(gpu, hd, ps, nkv, G, int8, wide):
     rng = np.random.default_rng(hd + ps + G)
     lens = np.array(EDGES, np.int32)
-    width = -(-max(EDGES) // ps)
+    width = -(-max(EDGES) // ps) + (32768 // ps if wide else 0)
     n_pages = sum(-(-max(n, 0) // ps) for n in EDGES) + 5
     k, v, ks, vs = pool(rng, n_pages, nkv, ps, hd, int8)
     table = block_table(rng, EDGES, ps, width, n_pages)
@@ -107,7 +108,27 @@ def test_attention_at_the_edges(gpu, hd, ps, nkv, G, int8):
 
 
 @pytest.mark.parametrize("int8", [False, True])
-@pytest.mark.parametrize("seqs,hi,nkv,G,ps", [(1, 5000, 4, 16, 64), (1, 70001, 1, 4, 16), (9, 3000, 2, 6, 32),
+@pytest.mark.parametrize("seqs,hi,nkv,hd,ps", [(70, 112, 2, 128, 16), (400, 128, 4, 128, 64), (90, 100, 12, 64, 32),
+                                               (130, 128, 3, 256, 128), (4096, 30, 1, 64, 16), (1, 1, 1, 128, 16)])
+def test_short_tables(gpu, seqs, hi, nkv, hd, ps, int8):
+    """Tables of a few steps, which no workgroup shares with another; more sequences than a wave has lanes."""
+    rng = np.random.default_rng(seqs)
+    lens = rng.integers(0, hi + 1, seqs).astype(np.int32)
+    lens[-1] = hi
+    n_pages = int(sum(-(-lens // ps))) + 1
+    k, v, ks, vs = pool(rng, n_pages, nkv, ps, hd, int8)
+    table = block_table(rng, lens, ps, -(-hi // ps), n_pages)
+    q = rng.standard_normal((seqs, nkv * 3, hd)).astype(np.float32)
+    case(f"paged attention, short tables seqs={seqs} hi={hi} nkv={nkv} hd={hd} ps={ps} int8={int8}")
+    got = host(attend(gpu, q, k, v, ks, vs, table, lens, hd ** -0.5))
+    want = reference(q, k, v, ks, vs, table, lens, hd ** -0.5)
+    assert not got[lens == 0].any()
+    for i in np.flatnonzero(lens):
+        assert rel_l2(got[i], want[i]) <= BAR, (i, lens[i])
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("seqs,hi,nkv,G,ps", [(1000, 300, 1, 2, 16), (1, 5000, 4, 16, 64), (1, 70001, 1, 4, 16), (9, 3000, 2, 6, 32),
                                               (70, 400, 4, 8, 64), (3, 40000, 8, 2, 128)])
 def test_attention_split_over_the_length(gpu, seqs, hi, nkv, G, ps, int8):
     rng = np.random.default_rng(hi + seqs)
