@@ -357,38 +357,42 @@ int mnemo_attention_decode_prep(const float *q, const float *k, const float *v,
  * kv_type 0 f16, 1 int8; head_dim 64, 128 or 256; all four arrays 16-byte aligned.
  * block_table [n_seqs][max_pages]: row s lists the pages of sequence s in order, position p is
  * at entry p / page_size, row p % page_size.  seq_lens [n_seqs]: positions held; a row with
- * length 0 is empty.  n_seqs <= 4096, max_pages * page_size and n_seqs * max_pages <= 2^30.
+ * length 0 is empty.  n_pages <= 2^30, n_seqs <= 4096, max_pages * page_size <= 2^30 and
+ * n_seqs * max_pages <= 2^30.
  * Table, lengths and ids live in device memory and are read by the kernels, so that captured
  * graphs serve every step.  A page id outside 0..n_pages-1 is never followed: attention takes
  * its positions as absent, stores and copies to it are dropped. */
 /* bytes of the K (or V) pages of one layer */
-size_t mnemo_paged_cache_bytes(int n_pages, int page_size, int n_kv_heads, int head_dim, int kv_type);
+size_t mnemo_paged_cache_bytes(int n_pages, int page_size, int n_kv_heads, int head_dim,
+                               int kv_type);
 /* Prepares n_tokens new tokens: QK norm (when both weights are given) and RoPE of q
  * [n_tokens][n_heads][head_dim] into q_out (which may be q) and of k [n_tokens][n_kv_heads]
  * [head_dim], and the store of k and v at their positions (int8: with per-row absmax scales,
  * as mnemo_attn_prep).  k and v are not modified.  Token t is position positions[t] of sequence
  * seq_ids[t]; with both NULL, token t < n_tokens <= n_seqs is the last position of sequence t,
  * seq_lens[t] - 1 (seq_lens may otherwise be NULL).  A token with a negative position is padding:
- * neither read nor written.  A position beyond the table, or a seq_id outside it, is prepared but
+ * nothing of it is written.  A position beyond the table, or a seq_id outside it, is prepared but
  * not stored.  No two tokens may share a position of a sequence, nor may stored pages be shared
- * by rows.  Angles are exact at any position (mnemo_attn_prep forms them in fp32, as the reference
- * does: its angle at position p is off by up to p * 2^-24). */
+ * by rows.  theta >= 1, n_tokens <= 4,194,304.  Angles are exact at any position (mnemo_attn_prep
+ * forms them in fp32, as the reference does: its angle at position p is off by up to p * 2^-24). */
 int mnemo_paged_attn_prep(const float *q, const float *k, const float *v, const float *q_norm_w,
                           const float *k_norm_w, float eps, float theta, int n_tokens, int n_heads,
                           int head_dim, int n_kv_heads, const int *positions, const int *seq_ids,
                           const int *block_table, const int *seq_lens, int n_seqs, int max_pages,
-                          void *k_pages, void *v_pages, float *k_scales, float *v_scales, int kv_type,
-                          int n_pages, int page_size, float *q_out, hipStream_t stream);
+                          void *k_pages, void *v_pages, float *k_scales, float *v_scales,
+                          int kv_type, int n_pages, int page_size, float *q_out,
+                          hipStream_t stream);
 /* Attention of one new token per sequence, n_heads = gqa * n_kv_heads with gqa <= 16:
  * out[s][h] = softmax_p(scale q[s][h] . k_p) v_p over the positions p < seq_lens[s] (at most
  * max_pages * page_size), q and out [n_seqs][n_heads][head_dim] fp32.  A sequence with no
- * positions gets zeros.  n_seqs * n_kv_heads * max_pages * page_size < 2^38.  workspace: mnemo_paged_attention_workspace_bytes(...) bytes, 16-byte
+ * positions gets zeros.  n_seqs * n_kv_heads * max_pages * page_size < 2^36.
+ * out must not overlap q.  workspace: mnemo_paged_attention_workspace_bytes(...) bytes, 16-byte
  * aligned, no initialisation; calls sharing it must not overlap. */
 size_t mnemo_paged_attention_workspace_bytes(int n_heads, int n_kv_heads, int head_dim);
 int mnemo_paged_attention_decode(const float *q, const void *k_pages, const void *v_pages,
-                                 const float *k_scales, const float *v_scales, int kv_type, float *out,
-                                 int n_seqs, int n_heads, int head_dim, int n_kv_heads, int n_pages,
-                                 int page_size, const int *block_table, int max_pages,
+                                 const float *k_scales, const float *v_scales, int kv_type,
+                                 float *out, int n_seqs, int n_heads, int head_dim, int n_kv_heads,
+                                 int n_pages, int page_size, const int *block_table, int max_pages,
                                  const int *seq_lens, float scale, void *workspace,
                                  size_t workspace_bytes, hipStream_t stream);
 /* Page upkeep.  page_refs [n_pages] counts the rows that hold a page; 0 is free.  A row holds its
@@ -403,25 +407,26 @@ int mnemo_kv_pages_extend(int *block_table, int *seq_lens, int *page_refs, const
                           int n_seqs, int max_pages, int n_pages, int page_size, int *status,
                           hipStream_t stream);
 /* free: every row with gone[s] != 0 drops its pages and becomes empty. */
-int mnemo_kv_pages_free(int *block_table, int *seq_lens, int *page_refs, const int *gone, int n_seqs,
-                        int max_pages, int n_pages, int page_size, hipStream_t stream);
+int mnemo_kv_pages_free(int *block_table, int *seq_lens, int *page_refs, const int *gone,
+                        int n_seqs, int max_pages, int n_pages, int page_size, hipStream_t stream);
 /* fork: every row with parents[s] >= 0 becomes a copy of that row as it was before the call (the
  * row must be empty and the parent not; refused otherwise).  Full pages are shared; a partly
  * filled last page is copied to a page of its own, in all n_layers layers of the caches
- * ([n_layers][n_pages]..., n_layers <= 4096).  workspace: mnemo_kv_pages_workspace_bytes(n_seqs, n_pages) bytes,
- * 16-byte aligned, no initialisation; calls sharing it must not overlap. */
+ * ([n_layers][n_pages]..., n_layers <= 4096).  workspace: mnemo_kv_pages_workspace_bytes(n_seqs,
+ * n_pages) bytes, 16-byte aligned, no initialisation; calls sharing it must not overlap. */
 size_t mnemo_kv_pages_workspace_bytes(int n_seqs, int n_pages);
-int mnemo_kv_pages_fork(int *block_table, int *seq_lens, int *page_refs, const int *parents, int n_seqs,
-                        int max_pages, void *k_pages, void *v_pages, float *k_scales, float *v_scales,
-                        int kv_type, int n_layers, int n_pages, int page_size, int n_kv_heads,
-                        int head_dim, int *status, void *workspace, size_t workspace_bytes,
-                        hipStream_t stream);
+int mnemo_kv_pages_fork(int *block_table, int *seq_lens, int *page_refs, const int *parents,
+                        int n_seqs, int max_pages, void *k_pages, void *v_pages, float *k_scales,
+                        float *v_scales, int kv_type, int n_layers, int n_pages, int page_size,
+                        int n_kv_heads, int head_dim, int *status, void *workspace,
+                        size_t workspace_bytes, hipStream_t stream);
 /* compact: the pages in use, n of them, become pages 0..n-1 (those at n and above move to the free
  * ones below, in order), in all layers; table and references follow, *n_live = n (may be NULL). */
-int mnemo_kv_pages_compact(int *block_table, int *page_refs, int n_seqs, int max_pages, void *k_pages,
-                           void *v_pages, float *k_scales, float *v_scales, int kv_type, int n_layers,
-                           int n_pages, int page_size, int n_kv_heads, int head_dim, int *n_live,
-                           void *workspace, size_t workspace_bytes, hipStream_t stream);
+int mnemo_kv_pages_compact(int *block_table, int *page_refs, int n_seqs, int max_pages,
+                           void *k_pages, void *v_pages, float *k_scales, float *v_scales,
+                           int kv_type, int n_layers, int n_pages, int page_size, int n_kv_heads,
+                           int head_dim, int *n_live, void *workspace, size_t workspace_bytes,
+                           hipStream_t stream);
 /* copy: page src[i] to page dst[i], i < n, in all layers.  A destination may appear only once and
  * must not be a source of another copy. */
 int mnemo_kv_pages_copy(const int *src, const int *dst, int n, void *k_pages, void *v_pages,
@@ -444,8 +449,8 @@ int mnemo_kv_pages_copy(const int *src, const int *dst, int n, void *k_pages, vo
 int mnemo_logits_process(const float *logits, float *out, int n_rows, int vocab, const int *history,
                          const int *history_lens, const int *prompt_lens, int max_history,
                          const float *repetition, const float *frequency, const float *presence,
-                         const int *bias_ids, const float *bias, int n_bias, const unsigned *allowed,
-                         hipStream_t stream);
+                         const int *bias_ids, const float *bias, int n_bias,
+                         const unsigned *allowed, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -3,6 +3,7 @@
 // Each wrapper validates its arguments, fills a launch descriptor and returns; errors are
 // printed (as the reference's KERNEL_LAUNCH_CHECK does, kernels.cu:1062-1067) and kept
 // per host thread for mnemo_last_error().
+#include <cfloat>
 #include <climits>
 #include <cstdarg>
 #include <cstdio>
@@ -595,8 +596,8 @@ int mnemo_moe_decode_rmsnorm_noalloc(const float *router_w, const void *experts,
 // ------------------------------------------------------------------ paged cache
 static int check_pages(const char *what, const KvPagesArgs &a) {
     if (!a.table || !a.lens || !a.refs) return set_error(kErrBadArg, "%s: NULL block table, lengths or references", what);
-    if (a.n_seqs <= 0 || a.n_seqs > kMaxSeqs || a.max_pages <= 0 || a.n_pages <= 0)
-        return set_error(kErrBadArg, "%s: need 1 <= n_seqs <= %d, max_pages > 0 and n_pages > 0", what, kMaxSeqs);
+    if (a.n_seqs <= 0 || a.n_seqs > kMaxSeqs || a.max_pages <= 0 || a.n_pages <= 0 || a.n_pages > 1 << 30)
+        return set_error(kErrBadArg, "%s: need 1 <= n_seqs <= %d, max_pages > 0 and 1 <= n_pages <= 2^30", what, kMaxSeqs);
     if (a.ps != 16 && a.ps != 32 && a.ps != 64 && a.ps != 128)
         return set_error(kErrBadArg, "%s: page_size %d (16, 32, 64, 128)", what, a.ps);
     if ((long long)a.max_pages * a.ps > 1 << 30 || (long long)a.n_seqs * a.max_pages > 1 << 30)
@@ -612,8 +613,8 @@ static int check_cache(const char *what, const PagedCache &c) {
         return set_error(kErrBadArg, "%s: head_dim %d (64, 128, 256)", what, c.hd);
     if (c.ps != 16 && c.ps != 32 && c.ps != 64 && c.ps != 128)
         return set_error(kErrBadArg, "%s: page_size %d (16, 32, 64, 128)", what, c.ps);
-    if (c.nkv <= 0 || c.nkv > 4096 || c.n_pages <= 0)
-        return set_error(kErrBadArg, "%s: need 1 <= n_kv_heads <= 4096 and n_pages > 0", what);
+    if (c.nkv <= 0 || c.nkv > 4096 || c.n_pages <= 0 || c.n_pages > 1 << 30)
+        return set_error(kErrBadArg, "%s: need 1 <= n_kv_heads <= 4096 and 1 <= n_pages <= 2^30", what);
     if (((uintptr_t)c.k | (uintptr_t)c.v | (c.kv_type == kKvInt8 ? (uintptr_t)c.ksc | (uintptr_t)c.vsc : 0)) % 16)
         return set_error(kErrBadArg, "%s: pages and scales must be 16-byte aligned", what);
     return 0;
@@ -638,7 +639,7 @@ int mnemo_paged_attn_prep(const float *q, const float *k, const float *v, const 
     if (n_seqs <= 0 || n_seqs > kMaxSeqs || max_pages <= 0 || (long long)max_pages * page_size > 1 << 30)
         return set_error(kErrBadArg, "%s: need 1 <= n_seqs <= %d and 1 <= max_pages * page_size <= 2^30", what, kMaxSeqs);
     if (n_heads <= 0 || n_heads > 65536) return set_error(kErrBadArg, "%s: n_heads must be in 1..65536", what);
-    if (!(theta > 0.0f)) return set_error(kErrBadArg, "%s: theta must be positive", what);
+    if (!(theta >= 1.0f && theta <= FLT_MAX)) return set_error(kErrBadArg, "%s: theta must be at least 1", what);
     if (n_tokens == 0) return kOk;
     if (n_tokens < 0 || n_tokens > 1 << 22)
         return set_error(kErrBadArg, "%s: n_tokens must be in 0..%d", what, 1 << 22);
@@ -683,8 +684,8 @@ int mnemo_paged_attention_decode(const float *q, const void *k_pages, const void
         return set_error(kErrBadArg, "%s: n_heads must be 1 to 16 times n_kv_heads", what);
     if (n_seqs <= 0 || n_seqs > kMaxSeqs || max_pages <= 0 || (long long)max_pages * page_size > 1 << 30)
         return set_error(kErrBadArg, "%s: need 1 <= n_seqs <= %d and 1 <= max_pages * page_size <= 2^30", what, kMaxSeqs);
-    if ((long long)n_seqs * n_kv_heads * max_pages * page_size >= 1LL << 38)
-        return set_error(kErrBadArg, "%s: n_seqs * n_kv_heads * max_pages * page_size must be below 2^38", what);
+    if ((long long)n_seqs * n_kv_heads * max_pages * page_size >= 1LL << 36)  // its steps are counted in an int
+        return set_error(kErrBadArg, "%s: n_seqs * n_kv_heads * max_pages * page_size must be below 2^36", what);
     if ((uintptr_t)workspace % 16 || workspace_bytes < paged_attn_workspace_bytes(n_kv_heads, head_dim))
         return set_error(kErrBadArg, "%s: workspace not 16-byte aligned, or %zu < %zu bytes", what, workspace_bytes,
                          paged_attn_workspace_bytes(n_kv_heads, head_dim));
@@ -765,7 +766,8 @@ int mnemo_kv_pages_copy(const int *src, const int *dst, int n, void *k_pages, vo
                         int head_dim, hipStream_t s) {
     const PagedCache c = {k_pages, v_pages, k_scales, v_scales, kv_type, n_pages, page_size, n_kv_heads, head_dim};
     if (int rc = check_moving("kv_pages_copy", c, n_layers, nullptr, 0, 0)) return rc;
-    if (n < 0 || (n > 0 && (!src || !dst))) return set_error(kErrBadArg, "kv_pages_copy: n < 0, or src or dst NULL");
+    if (n < 0 || n > 1 << 30 || (n > 0 && (!src || !dst)))
+        return set_error(kErrBadArg, "kv_pages_copy: n not in 0..2^30, or src or dst NULL");
     return launch_kv_copy(c, n_layers, src, dst, n, s);
 }
 

@@ -858,17 +858,12 @@ __global__ void __launch_bounds__(256) paged_prep_kernel(PagedPrepArgs a, int v_
 
 int launch_paged_prep(PagedPrepArgs &a, double theta, hipStream_t s) {
     const int hd = a.c.hd;
-    // theta^(-2j/hd) / (2 pi) of a turn per position, in units of 2^-64: repeated products, in whole numbers
-    // (2^-64 of a turn is lost by each, 2^-28 in all at position 2^30) where the factor is at most 1
-    const long double step = powl(theta, -2.0L / hd), turn0 = 0x1p64L / (2.0L * 3.14159265358979323846264338327950288L);
-    if (step <= 1.0L) {
-        const uint64_t f = step < 1.0L ? (uint64_t)(step * 0x1p64L) : UINT64_MAX;
-        uint64_t t = (uint64_t)turn0;
-        for (int j = 0; j < hd / 2; j++, t = (uint64_t)(((unsigned __int128)t * f) >> 64)) a.turn[j] = t;
-    } else {
-        long double t = turn0;
-        for (int j = 0; j < hd / 2; j++, t *= step) a.turn[j] = (uint64_t)fmodl(t, 0x1p64L);
-    }
+    // theta^(-2j/hd) / (2 pi) of a turn per position, in units of 2^-64, by repeated products in whole numbers: each
+    // loses up to 2^-64 of a turn, all of them 2^-27 at position 2^30
+    const long double step = powl(theta, -2.0L / hd);  // <= 1
+    const uint64_t f = step < 1.0L ? (uint64_t)(step * 0x1p64L) : UINT64_MAX;
+    uint64_t t = (uint64_t)(0x1p64L / (2.0L * 3.14159265358979323846264338327950288L));
+    for (int j = 0; j < hd / 2; j++, t = (uint64_t)(((unsigned __int128)t * f) >> 64)) a.turn[j] = t;
     // V through tiles where runs of tokens can be expected (a call by lengths has one token per sequence) and
     // there are enough tiles to hide their two phases behind the other blocks: 4 KV heads of 128, f16, 256
     // tokens 6.4 us with tiles against 5.8, 400 7.6 against 7.7, 1899 22.6 against 25.7; 12 heads of 64, 2000

@@ -637,9 +637,9 @@ def kv_pages_compact(block_table, page_refs, k_pages, v_pages, n_live, ws, ks=No
 def kv_pages_copy(src, dst, k_pages, v_pages, ks=None, vs=None):
     """Copies page src[i] to page dst[i] in all layers (int32 device tensors; destinations distinct, no source)."""
     lib = load_library()
-    ptrs, (n_layers, n_pages, nkv, ps, hd) = _pages(k_pages, v_pages, ks, vs, True)
     if src.numel() != dst.numel():
         raise MnemoError("kv_pages_copy: src and dst differ in length")
+    ptrs, (n_layers, n_pages, nkv, ps, hd) = _pages(k_pages, v_pages, ks, vs, True)
     rc = lib.mnemo_kv_pages_copy(_arg(src, "src", I32), _arg(dst, "dst", I32), src.numel(), *ptrs, n_layers, n_pages,
                                  ps, nkv, hd, _stream())
     _check_rc(lib, rc, "mnemo_kv_pages_copy")
