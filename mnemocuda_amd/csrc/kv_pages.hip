@@ -296,12 +296,12 @@ size_t kv_pages_workspace_bytes(int n_seqs, int n_pages) {
 
 __global__ void __launch_bounds__(kPlanThreads) kv_fork_plan_kernel(KvPagesArgs a, const int *__restrict__ parents,
                                                                     int *status, int *ws) {
-    __shared__ int start[kMaxSeqs];
+    __shared__ int copy_of[kMaxSeqs], last_page[kMaxSeqs];  // of each copy: its row, its source
     __shared__ uint16_t list[kScanPages];
     __shared__ int waves[kPlanThreads / 64], n_refused;
     int *parent = ws + 4, *tail = parent + a.n_seqs, *src = tail + a.n_seqs, *dst = src + a.n_seqs;
     const int per = (a.n_seqs + kPlanThreads - 1) / kPlanThreads, r0 = (int)threadIdx.x * per;
-    int need[kPlanRows], from[kPlanRows], len[kPlanRows], sum = 0, total, refused = 0;
+    int need[kPlanRows], from[kPlanRows], len[kPlanRows], page[kPlanRows], sum = 0, total, refused = 0;
     FreePages fp;
     fp.load(a.refs, a.n_pages);
     if (threadIdx.x == 0) n_refused = 0;
@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_fork_plan_kernel(KvPagesArgs 
     for (int i = 0; i < kPlanRows; i++) {
         const int r = r0 + i;
         need[i] = len[i] = 0;
-        from[i] = -1;
+        from[i] = page[i] = -1;
         if (i < per && r < a.n_seqs) {
             const int p = parents[r];
             if (p >= 0) {
@@ -320,6 +320,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_fork_plan_kernel(KvPagesArgs 
                     len[i] = pl;
                     need[i] = pl % a.ps != 0;
                     sum += need[i];
+                    if (need[i]) page[i] = a.table[(size_t)p * a.max_pages + pl / a.ps];
                 }
             }
         }
@@ -331,7 +332,10 @@ __global__ void __launch_bounds__(kPlanThreads) kv_fork_plan_kernel(KvPagesArgs 
     for (int i = 0; i < kPlanRows; i++) {
         const int r = r0 + i;
         if (i < per && r < a.n_seqs) {
-            start[r] = at;
+            if (need[i]) {
+                copy_of[at] = r;
+                last_page[at] = page[i];
+            }
             at += need[i];
             const bool served = from[i] >= 0 && at <= fp.n;
             if (from[i] >= 0 && !served) refused++;
@@ -341,17 +345,15 @@ __global__ void __launch_bounds__(kPlanThreads) kv_fork_plan_kernel(KvPagesArgs 
         }
     }
     if (refused) atomicAdd(&n_refused, refused);
-    __syncthreads();  // start and the count are whole
+    __syncthreads();  // the copies and the count are whole
     if (threadIdx.x == 0) {
         ws[0] = min(total, fp.n);
         if (status) *status = n_refused;
     }
     // a free page for each copy: rank k of the free pages is the k-th copy's
     if (total > 0) fp.give(min(total, fp.n), waves, list, [&](int page, int rank) {
-        const int r = row_of(start, a.n_seqs, rank);
-        const int p = parents[r];
-        tail[r] = page;
-        src[rank] = a.table[(size_t)p * a.max_pages + pages_of(a.lens[p], a.ps) - 1];
+        tail[copy_of[rank]] = page;
+        src[rank] = last_page[rank];
         dst[rank] = page;
         a.refs[page] = 1;
     });
