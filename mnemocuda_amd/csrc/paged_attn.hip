@@ -58,8 +58,16 @@ struct PaShape {
 };
 
 constexpr int kPaGroups = 256;  // one per CU
-static int part_floats(int hd) { return kPaRows * (hd + 2); }
-size_t paged_attn_workspace_bytes(int, int hd) { return (size_t)2 * kPaGroups * part_floats(hd) * sizeof(float); }
+// Workspace: two partials per workgroup (max [16], sum [16], O [16][hd]) and what they are: begun[g] is the
+// (sequence, KV head) that begins in workgroup g's share and goes on behind it (its second partial), taken[g]
+// the one that it goes on with from the workgroup before (its first), -1 for none.
+__host__ __device__ constexpr int part_floats(int hd) { return kPaRows * (hd + 2); }
+size_t paged_attn_workspace_bytes(int, int hd) {
+    return (size_t)2 * kPaGroups * (part_floats(hd) * sizeof(float) + sizeof(int));
+}
+__device__ __forceinline__ int *pa_begun(const PagedAttnArgs &a) {
+    return (int *)(a.ws + (size_t)2 * kPaGroups * part_floats(a.c.hd));
+}
 
 __device__ __forceinline__ int seq_len(const PagedAttnArgs &a, int s) {
     return min(max(a.lens[s], 0), a.max_pages * a.c.ps);
@@ -103,13 +111,9 @@ __device__ __forceinline__ PaPlan pa_plan(const PagedAttnArgs &a, int groups) {
     return p;
 }
 
-// First step of workgroup g (the end of the row from g = groups on), and the workgroup of step u.
+// First step of workgroup g (the end of the row from g = groups on).
 __device__ __forceinline__ int pa_first(const PaPlan &p, int g) {
     return g >= p.groups ? p.total : g * p.base + min(g, p.more);
-}
-__device__ __forceinline__ int pa_group(const PaPlan &p, int u) {
-    const int cut = p.more * (p.base + 1);
-    return u < cut ? u / (p.base + 1) : p.more + (u - cut) / p.base;
 }
 
 // The sequence, its length, the KV head and the step within them of step u.
@@ -454,6 +458,12 @@ __global__ void __launch_bounds__((PaShape<KV, HD, STEP>::kThreads)) paged_attn_
     const bool closes = lane < 2 * NW && !(lane & 1) && pair >= 0 && ends[lane >> 1];
     const uint32_t pieces = (uint32_t)__ballot(pair >= 0), closed = (uint32_t)__ballot(closes);
     const uint32_t starts = pieces & (0xaaaaaaaau | 1u);
+    if (threadIdx.x == 0) {
+        const int last = 31 - __builtin_clz(starts | 1u), after = ~((2u << last) - 1);
+        const bool goes_on = (starts & 2 * 0x55555555u) && (last & 1) && !(closed & after);
+        pa_begun(a)[blockIdx.x] = goes_on ? pair_of[last >> 1][1] : -1;
+        pa_begun(a)[kPaGroups + blockIdx.x] = pair_of[0][0];
+    }
     const int per = a.gqa * (HD / 4);  // elements of four dims
     for (int e = threadIdx.x; e < __popc(starts) * per; e += S::kThreads) {
         const int c = e / per, h = e % per / (HD / 4), d = 4 * (e % (HD / 4));
@@ -484,7 +494,7 @@ __global__ void __launch_bounds__((PaShape<KV, HD, STEP>::kThreads)) paged_attn_
             x *= sum == 0.0f ? 0.0f : 1.0f / sum;
             __builtin_memcpy(a.out + ((size_t)(pr / a.c.nkv) * a.nh + pr % a.c.nkv * a.gqa + h) * HD + d, &x, 16);
         } else {
-            float *part = a.ws + (size_t)(2 * blockIdx.x + k) * (kPaRows * (HD + 2));
+            float *part = a.ws + (size_t)(2 * blockIdx.x + k) * part_floats(HD);
             __builtin_memcpy(part + 2 * kPaRows + h * HD + d, &x, 16);
             if (d == 0) {
                 part[h] = mm;
@@ -498,40 +508,31 @@ __global__ void __launch_bounds__((PaShape<KV, HD, STEP>::kThreads)) paged_attn_
 // after the one that begins in workgroup x's share and goes on behind it (BY_SHARE), or after
 // (sequence, KV head) x itself.  256 threads are HD / 4 lanes of four dims, times CHAIN threads that
 // divide the partials among them, times heads.
-template <int STEP, int HD, int NW, int CHAIN, bool BY_SHARE>
+template <int HD, int CHAIN, bool BY_SHARE>
 __global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnArgs a, int groups) {
     constexpr int D4 = HD / 4, HEADS = 256 / (D4 * CHAIN), BATCH = 4;
+    static_assert(kPaGroups == 256, "a lane reads four entries");
     __shared__ __align__(16) float so[CHAIN > 1 ? CHAIN : 1][HEADS][HD];
     __shared__ float sm[CHAIN][HEADS], sl[CHAIN][HEADS];
-    const PaPlan plan = pa_plan<STEP, NW>(a, groups);
-    int seq, kvh, first, last, len;
-    if (BY_SHARE) {
-        const int u = pa_first(plan, blockIdx.x + 1) - 1;  // the last step of the share
-        if (u + 1 == plan.total) return;                          // nothing goes on behind it
-        int step;
-        pa_find<STEP>(a, plan, u, seq, kvh, step, len);
-        const int steps = (len + STEP - 1) / STEP;
-        first = u - step;
-        last = first + steps - 1;
-        if (last == u || first < pa_first(plan, blockIdx.x)) return;
-    } else {
-        seq = blockIdx.x / a.c.nkv;
-        kvh = blockIdx.x % a.c.nkv;
-        len = seq_len(a, seq);
-        if (len == 0) return;
-        const int steps = (len + STEP - 1) / STEP, L = seq / plan.per;
-        first = __builtin_amdgcn_readlane(plan.before, L) + kvh * steps;
-        if (plan.per > 1) {
-            const int s = L * plan.per + lane_id();
-            const int mine = s < seq ? (seq_len(a, s) + STEP - 1) / STEP * a.c.nkv : 0;
-            first += __builtin_amdgcn_readlane(wave_scan(mine), 63);
+    const int *begun = pa_begun(a);
+    int b[4], t[4], pair = blockIdx.x, w0 = blockIdx.x, n = 0;
+    __builtin_memcpy(t, begun + kPaGroups + 4 * lane_id(), 16);
+    if (BY_SHARE) pair = begun[blockIdx.x];
+    else {
+        __builtin_memcpy(b, begun + 4 * lane_id(), 16);
+        w0 = -1;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint64_t at = __ballot(4 * lane_id() + i < groups && b[i] == pair);
+            if (at) w0 = 4 * (__ffsll((unsigned long long)at) - 1) + i;
         }
-        last = first + steps - 1;
     }
-    const int w0 = pa_group(plan, first), w1 = pa_group(plan, last);
-    if (w0 == w1) return;
+    if (pair < 0 || w0 < 0) return;  // nothing, or finished in one workgroup
+#pragma unroll
+    for (int i = 0; i < 4; i++) n += __popcll(__ballot(4 * lane_id() + i < groups && t[i] == pair));
+    const int w1 = w0 + n, seq = pair / a.c.nkv, kvh = pair % a.c.nkv;
     const int dl = threadIdx.x % D4, g = threadIdx.x / D4 % CHAIN, hh = threadIdx.x / (D4 * CHAIN);
-    constexpr int PART = kPaRows * (HD + 2);
+    constexpr int PART = part_floats(HD);
     for (int h0 = blockIdx.y * HEADS; h0 < a.gqa; h0 += gridDim.y * HEADS) {
         const int h = min(h0 + hh, a.gqa - 1);
         float m = -INFINITY, l = 0.0f;
@@ -608,10 +609,10 @@ static void launch_pa(const PagedAttnArgs &a, hipStream_t s) {
     if (whole_pairs) return;
     // few (sequence, KV head)s: long chains, a workgroup for each head; many: short ones, found by the shares' ends
     if (pairs < groups)
-        hipLaunchKernelGGL((paged_merge_kernel<STEP, HD, S::kWaves, CHAIN, false>), dim3((int)pairs, a.gqa), dim3(256),
+        hipLaunchKernelGGL((paged_merge_kernel<HD, CHAIN, false>), dim3((int)pairs, a.gqa), dim3(256),
                            0, s, a, groups);
     else
-        hipLaunchKernelGGL((paged_merge_kernel<STEP, HD, S::kWaves, 1, true>), dim3(groups - 1, 1), dim3(256), 0, s, a,
+        hipLaunchKernelGGL((paged_merge_kernel<HD, 1, true>), dim3(groups - 1, 1), dim3(256), 0, s, a,
                            groups);
 }
 
