@@ -215,6 +215,7 @@ struct PagedPrepArgs {
     const int *table, *lens;
     const int *pos, *seq;  // of each token; both NULL: token t is position lens[t] - 1 of sequence t
     int n_tokens, n_seqs, max_pages, nh;
+    int q_streams;  // q_out is stored past the caches
     float eps;
     uint64_t turn[128];  // theta^(-2j/hd) / (2 pi) in units of 2^-64
 };

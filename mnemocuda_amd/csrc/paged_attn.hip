@@ -699,6 +699,7 @@ __device__ __forceinline__ void store_v(const PagedCache &c, const CacheRow<KV> 
 
 constexpr int kVTokens = 64;  // tokens of a tile of V, at head_dim 64 and 128; half of that at 256
 constexpr int kFewBlocks = 2048;  // resident at once
+typedef f4 f4a4 __attribute__((aligned(4)));
 
 // With V_TILES the first v_blocks take kVTokens tokens of one V head through LDS: V pages hold the
 // positions of a dim side by side, so eight tokens in a row that fill a group of eight positions are
@@ -778,8 +779,13 @@ __global__ void __launch_bounds__(256) paged_prep_kernel(PagedPrepArgs a, int v_
             }
             if (is_q) {
                 float *dst = a.q_out + ((size_t)t * a.nh + h) * HD;
-                __builtin_memcpy(dst + 4 * l, x0, 16);
-                __builtin_memcpy(dst + HALF + 4 * l, x1, 16);
+                if (a.q_streams) {
+                    __builtin_nontemporal_store(f4{x0[0], x0[1], x0[2], x0[3]}, (f4a4 *)(dst + 4 * l));
+                    __builtin_nontemporal_store(f4{x1[0], x1[1], x1[2], x1[3]}, (f4a4 *)(dst + HALF + 4 * l));
+                } else {
+                    __builtin_memcpy(dst + 4 * l, x0, 16);
+                    __builtin_memcpy(dst + HALF + 4 * l, x1, 16);
+                }
                 continue;
             }
             if (k.page < 0) continue;
@@ -874,6 +880,9 @@ int launch_paged_prep(PagedPrepArgs &a, double theta, hipStream_t s) {
     // heads of 128, 1899 tokens: 21.9 us, 25.5 with five workgroups per token, 22.5 with one).
     const int per = 2048 / hd, heads = a.nh + a.c.nkv * (tiles ? 1 : 2), parts = (heads + per - 1) / per;
     const int y = (long long)a.n_tokens * parts <= kFewBlocks ? parts : min(parts, 2);
+    // queries that outgrow an XCD's L2 (4 MB) are stored past it: 1899 tokens into an int8 cache 25.6 us where the
+    // stores through it take 31.6 and evict the pages, too; 800 tokens 9.7 against 11.6
+    a.q_streams = (long long)a.n_tokens * a.nh * hd * 4 > 4 << 20;
     const int vt = hd == 256 ? kVTokens / 2 : kVTokens;
     const int v_blocks = tiles ? ((a.n_tokens + vt - 1) / vt * a.c.nkv + y - 1) / y : 0;
     const dim3 grid(a.n_tokens + v_blocks, y);
