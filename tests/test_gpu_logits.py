@@ -74,7 +74,8 @@ def run(gpu, a, out=None):
 @pytest.mark.parametrize("n,V,H,B,mask", [
     (1, 1, 4, 1, True), (3, 31, 10, 5, True), (2, 33, 1, 0, True), (2, 4095, 300, 9, True), (2, 4096, 300, 9, False),
     (3, 4097, 300, 9, True), (5, 10007, 0, 3, True), (4, 8195, None, 40, True), (4, 20001, 5000, 0, False),
-    (1, 151936, 131072, 300, True), (9, 151937, 900, 2000, True), (700, 50, 77, 3, True), (2, 262144, 10, 1, True)])
+    (1, 151936, 131072, 300, True), (9, 151937, 900, 2000, True), (700, 50, 77, 3, True), (2, 262144, 10, 1, True),
+    (20, 151937, 3000, 90, True), (41, 151935, 9000, 40, True), (2100, 2001, 33, 2, False)])  # larger slices
 def test_against_the_formula(gpu, n, V, H, B, mask):
     rng = np.random.default_rng(n + V)
     a = inputs(rng, n, V, H, B, mask)

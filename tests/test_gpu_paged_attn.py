@@ -148,6 +148,64 @@ def test_attention_split_over_the_length(gpu, seqs, hi, nkv, G, ps, int8):
 
 
 @pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("seqs,hi,nkv,hd,G,ps", [(90, 700, 3, 64, 2, 16), (300, 260, 1, 256, 3, 32), (40, 900, 8, 128, 4, 128),
+                                                 (30, 400, 12, 64, 1, 64), (2, 20000, 2, 256, 16, 64), (5, 9000, 3, 64, 9, 128)])
+def test_many_and_few_sequences_of_every_head_size(gpu, seqs, hi, nkv, hd, G, ps, int8):
+    """More (sequence, KV head)s than workgroups, and far fewer, with shares that cut them."""
+    rng = np.random.default_rng(seqs + hd)
+    lens = rng.integers(0, hi + 1, seqs).astype(np.int32)
+    lens[seqs // 2] = hi
+    n_pages = int(sum(-(-lens // ps))) + 1
+    k, v, ks, vs = pool(rng, n_pages, nkv, ps, hd, int8)
+    table = block_table(rng, lens, ps, -(-hi // ps) + 1, n_pages)
+    q = rng.standard_normal((seqs, nkv * G, hd)).astype(np.float32)
+    case(f"paged attention seqs={seqs} hi={hi} nkv={nkv} hd={hd} gqa={G} ps={ps} int8={int8}")
+    got = attend(gpu, q, k, v, ks, vs, table, lens, hd ** -0.5)
+    assert torch.equal(got, attend(gpu, q, k, v, ks, vs, table, lens, hd ** -0.5))
+    want = reference(q, k, v, ks, vs, table, lens, hd ** -0.5)
+    for i in range(seqs):
+        if lens[i] == 0:
+            assert not host(got)[i].any()
+        else:
+            assert rel_l2(host(got)[i], want[i]) <= BAR, (i, lens[i])
+
+
+def test_rows_behind_the_last_are_left(gpu):
+    """The C entry points write n_seqs, n_tokens and n_rows rows and nothing behind them."""
+    import ctypes as C
+    lib = gpu.load_library()
+    rng = np.random.default_rng(21)
+    p = lambda t: C.c_void_p(t.data_ptr())  # noqa: E731
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    k, v, _, _ = pool(rng, 40, 2, 16, 64, False)
+    kd, vd = dev(k), dev(v)
+    lens = np.array([100, 0, 33, 5], np.int32)
+    table, ld = dev(block_table(rng, lens, 16, 8, 40)), dev(lens)
+    q, out = dev(rng.standard_normal((4, 6, 64)).astype(np.float32)), torch.full((4, 6, 64), 3.0, device="cuda")
+    n = gpu.ops.paged_attention_workspace_bytes(6, 2, 64)
+    ws = torch.full((n + 256,), 0x5A, dtype=torch.uint8, device="cuda")
+    case("rows behind the last")
+    assert lib.mnemo_paged_attention_decode(p(q), p(kd), p(vd), None, None, 0, p(out), 3, 6, 64, 2, 40, 16, p(table), 8, p(ld),
+                                            0.1, p(ws), n, stream) == 0
+    o = host(out)
+    assert (o[3] == 3.0).all() and not o[1].any() and (o[0] != 3.0).all()
+    assert (host(ws)[n:] == 0x5A).all()
+    kn = dev(rng.standard_normal((4, 2, 64)).astype(np.float32))
+    before = [x.clone() for x in (kd, vd)]
+    out.fill_(3.0)
+    assert lib.mnemo_paged_attn_prep(p(q), p(kn), p(kn), None, None, 1e-6, 1e4, 3, 6, 64, 2, None, None, p(table), p(ld), 4, 8,
+                                     p(kd), p(vd), None, None, 0, 40, 16, p(out), stream) == 0
+    o, t = host(out), host(table)
+    assert (o[3] == 3.0).all() and (o[1] == 3.0).all() and (o[0] != 3.0).all() and (o[2] != 3.0).all()
+    changed = (kd != before[0]).any(-1).nonzero().tolist()
+    assert sorted(set((a, c) for a, _, c in changed)) == sorted([(t[0, 6], 3), (t[2, 2], 0)])
+    z, zo = torch.randn((3, 77), device="cuda"), torch.full((3, 77), 3.0, device="cuda")
+    assert lib.mnemo_logits_process(p(z), p(zo), 2, 77, None, None, None, 0, None, None, None, None, None, 0, None, stream) == 0
+    assert torch.equal(zo[:2], z[:2]) and (host(zo)[2] == 3.0).all()
+    lib.mnemo_last_error()
+
+
+@pytest.mark.parametrize("int8", [False, True])
 @pytest.mark.parametrize("ps", [16, 64])
 def test_positions_past_the_end_are_not_looked_at(gpu, ps, int8):
     """NaN and infinities in the unused rest of a last page, in pages that nothing names, and in the table's rest."""
