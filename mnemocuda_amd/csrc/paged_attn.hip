@@ -873,11 +873,11 @@ int launch_paged_prep(PagedPrepArgs &a, double theta, hipStream_t s) {
     for (int j = 0; j < hd / 2; j++, t = (uint64_t)(((unsigned __int128)t * f) >> 64)) a.turn[j] = t;
     // V through tiles where runs of tokens can be expected (a call by lengths has one token per sequence) and
     // there are enough tiles to hide their two phases behind the other blocks: 4 KV heads of 128, f16, 256
-    // tokens 6.4 us with tiles against 5.8, 400 7.6 against 7.7, 1899 22.6 against 25.7; 12 heads of 64, 2000
-    // tokens 7.7 against 15.6; 2 heads of 256, 1000 tokens 10.9 against 10.7.
+    // tokens 5.7 us with tiles against 5.3, 400 6.5 either way, 1899 21.9 against 25.7; 12 heads of 64, 2000
+    // tokens 7.2 against 15.0; 2 heads of 256, 1000 tokens 9.1 against 8.9.
     const bool tiles = a.pos && (long long)a.n_tokens * a.c.nkv >= 2048;
     // Few tokens: a workgroup for every pass of heads; many: two per token, whose passes overlap (64 + 4
-    // heads of 128, 1899 tokens: 21.9 us, 25.5 with five workgroups per token, 22.5 with one).
+    // heads of 128, 1899 tokens: 21.9 us, 23.8 with five workgroups per token, 22.8 with one).
     const int per = 2048 / hd, heads = a.nh + a.c.nkv * (tiles ? 1 : 2), parts = (heads + per - 1) / per;
     const int y = (long long)a.n_tokens * parts <= kFewBlocks ? parts : min(parts, 2);
     // queries that outgrow an XCD's L2 (4 MB) are stored past it: 1899 tokens into an int8 cache 25.6 us where the
