@@ -217,7 +217,7 @@ struct PagedPrepArgs {
     int n_tokens, n_seqs, max_pages, nh;
     int q_streams;  // q_out is stored past the caches
     float eps;
-    uint64_t turn[128];  // theta^(-2j/hd) / (2 pi) in units of 2^-64
+    uint64_t turn0, step[7];  // 1 / (2 pi) and theta^(-2 2^i / hd), in units of 2^-64
 };
 int launch_paged_prep(PagedPrepArgs &a, double theta, hipStream_t s);
 

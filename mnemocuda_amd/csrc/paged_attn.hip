@@ -632,7 +632,7 @@ int launch_paged_attention(const PagedAttnArgs &a, hipStream_t s) {
 
 // ------------------------------------------------------------------ preparation of new tokens
 // HD / 8 lanes own a head, four rotated pairs (j, j + HD/2) each.  The angle of pair j at position p
-// is p turn[j] in units of 2^-64 of a turn, formed in integers (the product keeps its low 64 bits,
+// is p turn(j) in units of 2^-64 of a turn, formed in integers (the product keeps its low 64 bits,
 // whole turns fall off), so that it is as exact at position 10^6 as at 1: fp32 angles are off by
 // p 2^-24.
 //
@@ -730,7 +730,12 @@ __global__ void __launch_bounds__(256) paged_prep_kernel(PagedPrepArgs a, int v_
             __builtin_memcpy(u, src + 4 * l, 16);
             __builtin_memcpy(v, src + HALF + 4 * l, 16);
         };
-        const uint64_t turn = a.turn[tid % HALF];
+        uint64_t turn = a.turn0;  // of pair tid
+#pragma unroll
+        for (int i = 0; (1 << i) < HALF; i++) {
+            const uint64_t next = __umul64hi(turn, a.step[i]);
+            turn = tid >> i & 1 ? next : turn;
+        }
         load(blockIdx.y * PER, x0, x1);
         const Token k = token_of(a, t);
         if (k.pos < 0) return;
@@ -865,12 +870,14 @@ __global__ void __launch_bounds__(256) paged_prep_kernel(PagedPrepArgs a, int v_
 
 int launch_paged_prep(PagedPrepArgs &a, double theta, hipStream_t s) {
     const int hd = a.c.hd;
-    // theta^(-2j/hd) / (2 pi) of a turn per position, in units of 2^-64, by repeated products in whole numbers: each
-    // loses up to 2^-64 of a turn, all of them 2^-27 at position 2^30
-    const long double step = powl(theta, -2.0L / hd);  // <= 1
-    const uint64_t f = step < 1.0L ? (uint64_t)(step * 0x1p64L) : UINT64_MAX;
-    uint64_t t = (uint64_t)(0x1p64L / (2.0L * 3.14159265358979323846264338327950288L));
-    for (int j = 0; j < hd / 2; j++, t = (uint64_t)(((unsigned __int128)t * f) >> 64)) a.turn[j] = t;
+    // a turn per position is theta^(-2j/hd) / (2 pi) for pair j: the kernel forms it from the powers 2^i of the step, in
+    // whole numbers of 2^-64 (with the squarings' roundings at most 48 of them, 2^-28 of a turn at position 2^30)
+    long double step = powl(theta, -2.0L / hd);  // <= 1
+    a.turn0 = (uint64_t)(0x1p64L / (2.0L * 3.14159265358979323846264338327950288L));
+    for (uint64_t &p : a.step) {
+        p = step < 1.0L ? (uint64_t)(step * 0x1p64L) : UINT64_MAX;
+        step *= step;
+    }
     // V through tiles where runs of tokens can be expected (a call by lengths has one token per sequence) and
     // there are enough tiles to hide their two phases behind the other blocks: 4 KV heads of 128, f16, 256
     // tokens 5.7 us with tiles against 5.3, 400 6.5 either way, 1899 21.9 against 25.7; 12 heads of 64, 2000

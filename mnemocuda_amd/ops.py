@@ -494,7 +494,7 @@ def _arg(t, name: str, dtype: torch.dtype | None = None, n: int = 0) -> int:
     """The address of a contiguous tensor on the current GPU with at least n elements."""
     try:
         # the order of the checks is that of their use; each costs ~0.06 us, a call has up to 20 tensors
-        if t.is_cuda and (dtype is None or t.dtype is dtype) and t.is_contiguous() and t.numel() >= n:
+        if t.is_cuda and (dtype is None or t.dtype is dtype) and t.is_contiguous() and (not n or t.numel() >= n):
             if _gpus == 1 or t.get_device() == _current_gpu():
                 return t.data_ptr()
             raise MnemoError(f"{name} must be on the current GPU")
@@ -522,27 +522,35 @@ def _opt_arg(t, name: str, dtype: torch.dtype | None = None, n: int = 0) -> int 
 def _pages(k, v, ks, vs, layers: bool):
     """The arguments (pointers, kv_type) and shape (n_layers, n_pages, n_kv_heads, page_size, head_dim) of cache
     pages k [..., n_kv_heads, page_size, head_dim] and v [..., n_kv_heads, head_dim, page_size]."""
-    shape = k.shape
-    if len(shape) != (5 if layers else 4) or v.shape != (*shape[:-2], shape[-1], shape[-2]):
-        raise MnemoError(f"pages: k {tuple(shape)} and v {tuple(v.shape)} do not fit ({5 if layers else 4} dimensions, "
+    try:
+        if layers:
+            L, n, h, p, d = k.shape
+            fits = v.shape == (L, n, h, d, p)
+        else:
+            n, h, p, d = k.shape
+            L, fits = 1, v.shape == (n, h, d, p)
+    except ValueError:
+        fits = False
+    if not fits:
+        raise MnemoError(f"pages: k {tuple(k.shape)} and v {tuple(v.shape)} do not fit ({5 if layers else 4} dimensions, "
                          "v transposed)")
-    if k.dtype == torch.float16:
-        return (_arg(k, "k_pages"), _arg(v, "v_pages", torch.float16), None, None, 0), (shape[0] if layers else 1,
-                                                                                        *shape[-4:])
-    if k.dtype != torch.int8:
+    if k.dtype is torch.float16:
+        return (_arg(k, "k_pages"), _arg(v, "v_pages", torch.float16), None, None, 0), (L, n, h, p, d)
+    if k.dtype is not torch.int8:
         raise MnemoError(f"pages must be float16 or int8, got {k.dtype}")
     if ks is None or vs is None:
         raise MnemoError("int8 pages need scales")
-    n = k.numel() // max(shape[-1], 1)
-    return (_arg(k, "k_pages"), _arg(v, "v_pages", torch.int8), _arg(ks, "k_scales", F32, n),
-            _arg(vs, "v_scales", F32, n), 1), (shape[0] if layers else 1, *shape[-4:])
+    rows = L * n * h * p
+    return (_arg(k, "k_pages"), _arg(v, "v_pages", torch.int8), _arg(ks, "k_scales", F32, rows),
+            _arg(vs, "v_scales", F32, rows), 1), (L, n, h, p, d)
 
 
 def _rows(table):
     """(address, n_seqs, max_pages) of a block table."""
-    if table.dim() != 2:
-        raise MnemoError(f"block_table must have 2 dimensions, got {table.dim()}")
-    return _arg(table, "block_table", I32), *table.shape
+    shape = table.shape
+    if len(shape) != 2:
+        raise MnemoError(f"block_table must have 2 dimensions, got {len(shape)}")
+    return _arg(table, "block_table", I32), shape[0], shape[1]
 
 
 def paged_attn_prep(q, k, v, qw, kw, eps: float, theta: float, k_pages, v_pages, block_table, q_out, positions=None,
@@ -553,10 +561,10 @@ def paged_attn_prep(q, k, v, qw, kw, eps: float, theta: float, k_pages, v_pages,
     lib = load_library()
     ptrs, (_, n_pages, nkv, ps, hd) = _pages(k_pages, v_pages, ks, vs, False)
     table, n_seqs, max_pages = _rows(block_table)
-    if q.dim() != 3 or q.shape[2] != hd or k.shape != (q.shape[0], nkv, hd) or v.shape != k.shape \
-            or q_out.shape != q.shape:
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != hd or k.shape != (shape[0], nkv, hd) or v.shape != k.shape or q_out.shape != shape:
         raise MnemoError("paged_attn_prep: q, k, v and q_out must be [T, heads, head_dim]")
-    T, nh = q.shape[0], q.shape[1]
+    T, nh = shape[0], shape[1]
     rc = lib.mnemo_paged_attn_prep(
         _arg(q, "q", F32), _arg(k, "k", F32), _arg(v, "v", F32), _opt_arg(qw, "qw", F32, hd),
         _opt_arg(kw, "kw", F32, hd), float(eps), float(theta), T, nh, hd, nkv,
@@ -576,10 +584,11 @@ def paged_attention_decode(q, k_pages, v_pages, block_table, seq_lens, out, scal
     lib = load_library()
     ptrs, (_, n_pages, nkv, ps, hd) = _pages(k_pages, v_pages, ks, vs, False)
     table, n_seqs, max_pages = _rows(block_table)
-    if q.dim() != 3 or q.shape[0] != n_seqs or q.shape[2] != hd or out.shape != q.shape:
+    shape = q.shape
+    if len(shape) != 3 or shape[0] != n_seqs or shape[2] != hd or out.shape != shape:
         raise MnemoError("paged_attention_decode: q and out must be [n_seqs, n_heads, head_dim]")
     rc = lib.mnemo_paged_attention_decode(
-        _arg(q, "q", F32), *ptrs, _arg(out, "out", F32), n_seqs, q.shape[1], hd, nkv, n_pages, ps, table, max_pages,
+        _arg(q, "q", F32), *ptrs, _arg(out, "out", F32), n_seqs, shape[1], hd, nkv, n_pages, ps, table, max_pages,
         _arg(seq_lens, "seq_lens", I32, n_seqs), float(scale), _arg(ws, "ws"), ws.numel() * ws.element_size(),
         _stream())
     _check_rc(lib, rc, "mnemo_paged_attention_decode")
