@@ -398,8 +398,9 @@ int mnemo_paged_attention_decode(const float *q, const void *k_pages, const void
 /* Page upkeep.  page_refs [n_pages] counts the rows that hold a page; 0 is free.  A row holds its
  * first ceil(seq_lens / page_size) entries.  An empty state is table -1, lengths 0, references 0.
  * Pages are given out lowest first, to the rows in order.  A row is served when the free pages
- * suffice for it and all rows before it that need some; the others stay as they were, and their
- * number goes to *status (device memory, may be NULL).
+ * suffice for it and all rows before it that need some; from the first row that they do not suffice
+ * for, none is (one that needs no page neither).  The others stay as they were, and their number
+ * goes to *status (device memory, may be NULL).
  *
  * extend: every row with new_lens[s] > seq_lens[s] gets the pages it needs and that length (a
  * length beyond the table is refused).  The new positions hold nothing yet. */

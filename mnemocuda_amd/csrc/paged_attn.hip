@@ -703,8 +703,9 @@ typedef f4 f4a4 __attribute__((aligned(4)));
 
 // With V_TILES the first v_blocks take kVTokens tokens of one V head through LDS: V pages hold the
 // positions of a dim side by side, so eight tokens in a row that fill a group of eight positions are
-// one store per dim instead of eight of one element each.  Tokens outside such groups are stored singly.  The other blocks take one token each and gridDim.y-th parts of its
-// heads: q heads, then k, then (V_TILES false) v.
+// one store per dim instead of eight of one element each.  Tokens outside such groups are stored
+// singly.  The other blocks take one token each and gridDim.y-th parts of its heads: q heads, then k,
+// then (V_TILES false) v.
 template <int KV, int HD, bool V_TILES>
 __global__ void __launch_bounds__(256) paged_prep_kernel(PagedPrepArgs a, int v_blocks) {
     constexpr int LPH = HD / 8, HALF = HD / 2, EB = KV == kKvF16 ? 2 : 1;
@@ -871,7 +872,7 @@ __global__ void __launch_bounds__(256) paged_prep_kernel(PagedPrepArgs a, int v_
 int launch_paged_prep(PagedPrepArgs &a, double theta, hipStream_t s) {
     const int hd = a.c.hd;
     // a turn per position is theta^(-2j/hd) / (2 pi) for pair j: the kernel forms it from the powers 2^i of the step, in
-    // whole numbers of 2^-64 (with the squarings' roundings at most 48 of them, 2^-28 of a turn at position 2^30)
+    // whole numbers of 2^-64 (off by up to 8 of them for theta from 1 to 3e38: 2^-31 of a turn at position 2^30)
     long double step = powl(theta, -2.0L / hd);  // <= 1
     a.turn0 = (uint64_t)(0x1p64L / (2.0L * 3.14159265358979323846264338327950288L));
     for (uint64_t &p : a.step) {
