@@ -445,8 +445,8 @@ int mnemo_kv_pages_copy(const int *src, const int *dst, int n, void *k_pages, vo
  * 0..max_history), or NULL: no penalties, its other arguments unused.  bias_ids / bias
  * [n_rows][n_bias], or NULL: the bias of token bias_ids[r][i] (ids outside the vocabulary are
  * ignored; of several entries for a token the last counts).  allowed [n_rows][ceil(vocab / 32)],
- * or NULL: all are.  A row whose mask allows nothing is all -inf.  n_rows <= 65535,
- * vocab <= 2^30. */
+ * or NULL: all are.  A row whose mask allows nothing is all -inf.  n_rows <= 65535; vocab,
+ * max_history and n_bias <= 2^30. */
 int mnemo_logits_process(const float *logits, float *out, int n_rows, int vocab, const int *history,
                          const int *history_lens, const int *prompt_lens, int max_history,
                          const float *repetition, const float *frequency, const float *presence,

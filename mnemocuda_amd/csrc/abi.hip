@@ -781,6 +781,9 @@ int mnemo_logits_process(const float *logits, float *out, int n_rows, int vocab,
     if (history && (!history_lens || !prompt_lens || !repetition || !frequency || !presence || max_history < 0))
         return set_error(kErrBadArg, "logits_process: a history needs its lengths and the three penalties");
     if (bias_ids && (!bias || n_bias < 0)) return set_error(kErrBadArg, "logits_process: bias_ids needs bias");
+    // the kernel steps over both in 32-bit counters
+    if ((history && max_history > 1 << 30) || (bias_ids && n_bias > 1 << 30))
+        return set_error(kErrBadArg, "logits_process: max_history and n_bias must be at most 2^30");
     if (n_rows == 0) return kOk;
     if (!logits || !out) return set_error(kErrBadArg, "logits_process: logits or out is NULL");
     LogitsArgs a = {};

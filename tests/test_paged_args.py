@@ -155,3 +155,12 @@ def test_wrappers_refuse_host_tensors_and_shapes(L):
         ops.logits_process(z(2, 50), z(2, 50), i(3, 4))
     with pytest.raises(MnemoError, match="GPU tensor"):
         ops.logits_process(z(2, 50), z(2, 50))
+
+
+
+@pytest.mark.parametrize("bad", [dict(max_hist=(1 << 30) + 1), dict(max_hist=(1 << 31) - 1), dict(nb=(1 << 30) + 1),
+                                 dict(nb=(1 << 31) - 1)])
+def test_logits_refuses_lengths_that_its_steps_would_leave_the_range_with(L, bad, capfd):
+    """The kernel walks the history 4096 entries and the biases 256 at a time in 32-bit counters."""
+    assert logits(L, z=None, out=None, n=0, **{k: v for k, v in bad.items()}) == 1
+    assert "logits_process" in capfd.readouterr().err
