@@ -552,13 +552,14 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnArgs a, int g
             float mn = m;
 #pragma unroll
             for (int i = 0; i < BATCH; i++) mn = fmaxf(mn, pm[i]);
-            if (mn == -INFINITY) continue;
-            const float fa = __builtin_amdgcn_exp2f(m - mn);
+            // partials without a maximum are taken in, too: their sums are 0, or NaN where every score is one
+            const float ref = mn == -INFINITY ? 0.0f : mn;
+            const float fa = __builtin_amdgcn_exp2f(m - ref);
             l *= fa;
             o *= fa;
 #pragma unroll
             for (int i = 0; i < BATCH; i++) {
-                const float f = __builtin_amdgcn_exp2f(pm[i] - mn);
+                const float f = __builtin_amdgcn_exp2f(pm[i] - ref);
                 l = fmaf(pl[i], f, l);
                 o += x[i] * f;
             }

@@ -544,3 +544,33 @@ def test_int8_rows_of_zeros_and_of_tiny_values(gpu):
     for p, s in ((host(kp)[0, 0, :3], host(ks)), (host(vp)[0, 0, :, :3].T, host(vs))):
         assert not p[:2].any() and not s[0, 0, :2].any()
         assert np.abs(p[2]).max() == 127
+
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("lens,nkv,hd,ps", [([10, 5000, 300, 64, 20000], 2, 128, 64), ([7, 900, 4000], 1, 256, 32),
+                                            (list(range(1, 1400, 14)), 3, 64, 16)])
+def test_queries_that_are_no_number(gpu, lens, nkv, hd, ps, int8):
+    """A query head that holds a NaN or an infinity gives NaN, whether its sequence lies in one workgroup's share or in
+    several (few and many sequences: both kinds of merge); the other heads are not touched."""
+    rng = np.random.default_rng(hd)
+    lens = np.array(lens, np.int32)
+    n_pages = int(sum(-(-lens // ps))) + 1
+    k, v, ks, vs = pool(rng, n_pages, nkv, ps, hd, int8)
+    table = block_table(rng, lens, ps, -(-int(lens.max()) // ps) + 2, n_pages)
+    nh = 3 * nkv
+    q = rng.standard_normal((len(lens), nh, hd)).astype(np.float32)
+    want = reference(q, k, v, ks, vs, table, lens, hd ** -0.5)
+    bad = np.zeros((len(lens), nh), bool)
+    for i in range(len(lens)):
+        bad[i, [i % nh, (i + 4) % nh]] = True
+        q[i, i % nh, (5 * i) % hd] = np.nan
+        q[i, (i + 4) % nh, (7 * i) % hd] = (np.inf, np.nan)[i % 2]
+    case(f"paged attention, NaN queries, {len(lens)} sequences nkv={nkv} hd={hd} int8={int8}")
+    got = host(attend(gpu, q, k, v, ks, vs, table, lens, hd ** -0.5))
+    for i in range(len(lens)):
+        for h in range(nh):
+            if bad[i, h]:
+                assert np.isnan(got[i, h]).all(), (i, h, lens[i])
+            else:
+                assert rel_l2(got[i, h], want[i, h]) <= 2 * BAR, (i, h, lens[i])  # one head: two deviations
