@@ -35,8 +35,10 @@ namespace mnemo {
 // Precision: Q is scaled by a power of two into [1, 2) per head and split into two f16 parts, P
 // likewise split; K and V enter exactly (f16 or int8).  P is formed relative to a reference that
 // follows the maximum only when a score exceeds it by 2^kSlack, and is 2^kLift at the reference:
-// its smallest f16 step, 2^-24, is then 2^-33 of the largest weight.  int8 value scales multiply
-// P relative to a power of two that follows the largest of them in the same way.
+// its smallest f16 step, 2^-24, is then 2^-33 of the largest weight.  int8: what is split is P times
+// the value's scale, relative to a power of two (wref) that follows the largest such product in the
+// same way, not the largest scale: a large scale of no weight leaves the others their bits.  The
+// reference of P is a whole power there, so that O and its unit are rescaled without rounding.
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -44,7 +46,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int kPaRows = 16;
-constexpr float kSlack = 5.0f, kLift = 9.0f;  // powers of two: P <= 2^14, times a scale below 2
+constexpr float kSlack = 5.0f, kLift = 9.0f;  // powers of two: P <= 2^14 (int8: 2^5, P times scale below 2^15 wref)
 
 template <int KV, int HD, int STEP>
 struct PaShape {
@@ -252,7 +254,7 @@ __global__ void __launch_bounds__((PaShape<KV, HD, STEP>::kThreads)) paged_attn_
         };
 
         float m = -INFINITY, l = 0.0f;  // reference (log2) of the lane's head, sum over the lane's positions
-        float vref = 0x1p-126f;
+        float wref = 0x1p-126f;  // of the lane's head
         f4 o[ND] = {};
         int p0 = step * STEP;
         {
@@ -321,7 +323,7 @@ __global__ void __launch_bounds__((PaShape<KV, HD, STEP>::kThreads)) paged_attn_
                 const int live = min(max(len - (p0 + STEP / 4 * kg), 0), STEP / 4);  // of the lane's positions
                 const bool ok = (unsigned)cur.v < (unsigned)a.c.n_pages;
                 const bool full = __all(ok && live == STEP / 4);  // uniform
-                float smax = -INFINITY, vmax = 0.0f;
+                float smax = -INFINITY;
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -335,37 +337,57 @@ __global__ void __launch_bounds__((PaShape<KV, HD, STEP>::kThreads)) paged_attn_
                         }
                         s[t][i] = x;
                         smax = fmaxf(smax, x);
-                        if (KV == kKvInt8) vmax = fmaxf(vmax, fabsf(vsc[4 * t + i]));
                     }
-                if (__any(smax > m + kSlack || (KV == kKvInt8 && vmax >= 2.0f * vref))) {
-                    const float mn = fmaxf(m, max_heads(smax));
-                    const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-                    float f = al;
-                    if (KV == kKvInt8) {
-                        float vm = vmax;
-#pragma unroll
-                        for (int x = 1; x < 64; x <<= 1) vm = fmaxf(vm, __shfl_xor(vm, x));
-                        // the power of two at or below vm (at most 2^126, so that its inverse is a float)
-                        const uint32_t e = min(__builtin_bit_cast(uint32_t, vm) & 0x7f800000u, 0x7e800000u);
-                        const float vn = fmaxf(vref, __builtin_bit_cast(float, e));
-                        f = al * (vref * inverse2(vn));
-                        vref = vn;
+                if (__any(smax > m + kSlack)) {
+                    float mn = max_heads(smax), al, f;
+                    if (KV == kKvF16) {
+                        mn = fmaxf(m, mn);
+                        f = al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+                    } else {
+                        mn = fmaxf(m, ceilf(mn));
+                        al = mn == -INFINITY ? 1.0f : ldexpf(1.0f, (int)fmaxf(m - mn, -256.0f));
+                        // O stays as it is while its unit, 2^m wref, can
+                        const float w = wref * al;
+                        wref = fmaxf(w, 0x1p-126f);
+                        f = w * inverse2(wref);
                     }
                     l *= al;
 #pragma unroll
                     for (int i = 0; i < ND; i++) o[i] *= f;
                     m = mn;
                 }
-                const float ref = m == -INFINITY ? 0.0f : m - kLift;
-                const float vi = inverse2(vref);
+                const float ref = m == -INFINITY ? 0.0f : KV == kKvF16 ? m - kLift : m;
+                float wi = 1.0f;
+                if (KV == kKvInt8) {
+                    float wmax = 0.0f;
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float p = __builtin_amdgcn_exp2f(s[t][i] - ref);
+                            l += p;
+                            s[t][i] = p * vsc[4 * t + i];
+                            wmax = fmaxf(wmax, fabsf(s[t][i]));
+                        }
+                    if (__any(wmax >= 0x1p15f * wref)) {
+                        // the power of two at or below the largest (at most 2^126) becomes 2^kLift
+                        const uint32_t e = min(__builtin_bit_cast(uint32_t, max_heads(wmax)) & 0x7f800000u, 0x7e800000u);
+                        const float wn = fmaxf(wref, __builtin_bit_cast(float, e) * exp2f(-kLift));
+                        const float f = wref * inverse2(wn);
+#pragma unroll
+                        for (int i = 0; i < ND; i++) o[i] *= f;
+                        wref = wn;
+                    }
+                    wi = inverse2(wref);
+                }
                 h8 phi[PV], plo[PV];
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const float p = __builtin_amdgcn_exp2f(s[t][i] - ref);
-                        l += p;
-                        float w = KV == kKvInt8 ? p * (vsc[4 * t + i] * vi) : p;
+                        float w;
+                        if (KV == kKvF16) l += w = __builtin_amdgcn_exp2f(s[t][i] - ref);
+                        else w = s[t][i] * wi;
                         // one fp32 value for both parts: a product folded into one of the conversions
                         // would round differently there
                         asm("" : "+v"(w));
@@ -414,7 +436,8 @@ __global__ void __launch_bounds__((PaShape<KV, HD, STEP>::kThreads)) paged_attn_
             if (r < a.gqa) {
 #pragma unroll
                 for (int i = 0; i < ND; i++) {
-                    const f4 x = o[i] * (KV == kKvInt8 ? vref * inv : inv);
+                    f4 x = o[i] * inv;
+                    if (KV == kKvInt8) x *= wref;
                     __builtin_memcpy(out + 16 * i, &x, 16);
                 }
             }
@@ -430,7 +453,7 @@ __global__ void __launch_bounds__((PaShape<KV, HD, STEP>::kThreads)) paged_attn_
 #pragma unroll
             for (int i = 0; i < ND; i++) {
                 f4 x = o[i];
-                if (KV == kKvInt8) x *= vref;
+                if (KV == kKvInt8) x *= wref;
                 __builtin_memcpy(&lo[wave][begins][r][16 * i + 4 * kg], &x, 16);
             }
         }

@@ -574,3 +574,51 @@ def test_queries_that_are_no_number(gpu, lens, nkv, hd, ps, int8):
                 assert np.isnan(got[i, h]).all(), (i, h, lens[i])
             else:
                 assert rel_l2(got[i, h], want[i, h]) <= 2 * BAR, (i, h, lens[i])  # one head: two deviations
+
+
+
+# Scores of these tests: K rows and queries of equal signs, so that a head's products are one power of two and their sum is
+# exact; scale, log2(e) and the key's scale are four roundings of the score S, its difference to the maximum another
+# (2^-24 each, of S at most), exp2 and the weight's three products and its sum 16 at most of the weight itself.  So a
+# weight is off by (6 S + 16) 2^-24 of itself, numerator and denominator both; a sum over n positions by n 2^-24 of the
+# sizes that it adds; and the two f16 parts of a weight times scale by 2^-33 of the largest of them per position.
+@pytest.mark.parametrize("order", ["random", "scores rise", "scores fall", "one large", "one large at last"])
+@pytest.mark.parametrize("n,nkv,hd,ps", [(64, 1, 128, 16), (150, 2, 64, 32), (3000, 2, 128, 64), (900, 1, 256, 128)])
+def test_value_scales_within_a_sequence(gpu, n, nkv, hd, ps, order):
+    """int8 value scales that differ by many orders of magnitude within one sequence, also where the largest of them has
+    next to no weight."""
+    rng = np.random.default_rng(n + len(order))
+    width = -(-n // ps)
+    u = rng.choice(np.array([-1, 1], np.int8), hd)
+    k = np.broadcast_to(u, (width, nkv, ps, hd)).copy()
+    v = rng.integers(-127, 128, (width, nkv, hd, ps)).astype(np.int8)
+    a = np.array([1.0, 0.5, 0.25, 1.0])
+    q = np.tile((a[:, None] * u).astype(np.float32), (nkv, 1))[None]
+    for trial in range(4):
+        if order.startswith("one"):  # the other scales 1e-6, 1e-8, 1e-12 and 1e-20 of it
+            s = rng.uniform(0, 3, (nkv, width * ps))
+            vs = rng.uniform(0.5, 1.5, s.shape) * (1e-6, 1e-8, 1e-12, 1e-20)[trial]
+            at = n - 1 if order.endswith("last") else n // 2
+            s[:, at], vs[:, at] = -50.0, 1.0
+        else:
+            s = rng.uniform(-30, 30, (nkv, width * ps))
+            if order != "random":
+                s[:, :n] = np.sort(s[:, :n], -1)[:, ::1 if order == "scores rise" else -1]
+            vs = 10 ** rng.uniform(-15, 15, s.shape)
+            if trial % 2:  # large scales on small scores
+                vs = np.exp(-s * (0.5 + 0.5 * trial)) * rng.uniform(0.5, 1.5, s.shape)
+        ks = np.ascontiguousarray(s.astype(np.float32).reshape(nkv, width, ps).transpose(1, 0, 2))
+        vs = np.ascontiguousarray(vs.astype(np.float32).reshape(nkv, width, ps).transpose(1, 0, 2))
+        table, lens = np.arange(width, dtype=np.int32)[None], np.array([n], np.int32)
+        case(f"paged attention, value scales within a sequence n={n} nkv={nkv} hd={hd} {order} {trial}")
+        got = host(attend(gpu, q, k, v, ks, vs, table, lens, 1.0 / hd))[0]
+        for h in range(4 * nkv):
+            g = h // 4
+            sc = a[h % 4] * ks[:, g].astype(np.float64).flatten()[:n]
+            w = np.exp(sc - sc.max())
+            sizes = w * vs[:, g].astype(np.float64).flatten()[:n]
+            V = v[:, g].transpose(0, 2, 1).reshape(-1, hd)[:n].astype(np.float64)
+            want = sizes @ V / w.sum()
+            eps = 2 * (6 * np.abs(sc).max() + 16 + n) * 2.0 ** -24
+            bound = (eps * (sizes @ np.abs(V)) + n * 2.0 ** -33 * 127 * sizes.max()) / w.sum()
+            assert (np.abs(got[h] - want) <= bound).all(), (trial, h, np.abs(got[h] - want).max(), bound.max())
