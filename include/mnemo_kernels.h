@@ -369,10 +369,16 @@ size_t mnemo_paged_cache_bytes(int n_pages, int page_size, int n_kv_heads, int h
  * [n_tokens][n_heads][head_dim] into q_out (which may be q) and of k [n_tokens][n_kv_heads]
  * [head_dim], and the store of k and v at their positions (int8: with per-row absmax scales,
  * as mnemo_attn_prep).  k and v are not modified.  Token t is position positions[t] of sequence
- * seq_ids[t]; with both NULL, token t < n_tokens <= n_seqs is the last position of sequence t,
- * seq_lens[t] - 1 (seq_lens may otherwise be NULL).  A token with a negative position is padding:
- * nothing of it is written.  A position beyond the table, or a seq_id outside it, is prepared but
- * not stored.  No two tokens may share a position of a sequence, nor may stored pages be shared
+ * seq_ids[t].  A token with a negative position is padding: nothing of it is written.  A position
+ * beyond the table, a seq_id outside it, and, where seq_lens is given (else NULL), a position at
+ * seq_lens[seq_ids[t]] or beyond is prepared but not stored.  A step that extends its rows first gives
+ * positions[s] = new_lens[s] - 1 (-1 for a row that takes no token) and seq_lens: a row that
+ * mnemo_kv_pages_extend refused then keeps its pages as they are.
+ * With positions and seq_ids both NULL, token t < n_tokens <= n_seqs is the last position of
+ * sequence t, seq_lens[t] - 1, whether or not the row grew: this is for steps in which every row
+ * that is not empty took a token.  A refused or paused row's last position would be overwritten,
+ * in a page that other rows may share.
+ * No two tokens may share a position of a sequence, nor may stored pages be shared
  * by rows.  theta >= 1, n_tokens <= 4,194,304.  Angles are exact at any position (mnemo_attn_prep
  * forms them in fp32, as the reference does: its angle at position p is off by up to p * 2^-24). */
 int mnemo_paged_attn_prep(const float *q, const float *k, const float *v, const float *q_norm_w,
@@ -400,7 +406,8 @@ int mnemo_paged_attention_decode(const float *q, const void *k_pages, const void
  * Pages are given out lowest first, to the rows in order.  A row is served when the free pages
  * suffice for it and all rows before it that need some; from the first row that they do not suffice
  * for, none is (one that needs no page neither).  The others stay as they were, and their number
- * goes to *status (device memory, may be NULL).
+ * goes to *status (device memory, may be NULL); which ones they are shows in seq_lens, which is
+ * then not what was asked for.
  *
  * extend: every row with new_lens[s] > seq_lens[s] gets the pages it needs and that length (a
  * length beyond the table is refused).  The new positions hold nothing yet. */

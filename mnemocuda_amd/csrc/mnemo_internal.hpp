@@ -213,7 +213,8 @@ struct PagedPrepArgs {
     float *q_out;
     PagedCache c;
     const int *table, *lens;
-    const int *pos, *seq;  // of each token; both NULL: token t is position lens[t] - 1 of sequence t
+    // of each token (with lens: not stored from lens[seq] on); both NULL: token t is position lens[t] - 1 of sequence t
+    const int *pos, *seq;
     int n_tokens, n_seqs, max_pages, nh;
     int q_streams;  // q_out is stored past the caches
     float eps;

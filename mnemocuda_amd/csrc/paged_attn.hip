@@ -696,7 +696,8 @@ __device__ __forceinline__ CacheRow<KV> cache_row(const float (&x0)[4], const fl
     return r;
 }
 
-// Sequence and position of token t (position -1: padding, sequence -1: not stored), and its page.
+// Sequence and position of token t (position -1: padding, sequence -1: not stored), and its page.  Where positions come
+// with lengths, a token at its row's length or behind it is not stored: the row was not extended for it.
 struct Token { int seq, pos, page; };
 __device__ __forceinline__ Token token_of(const PagedPrepArgs &a, int t) {
     Token k;
@@ -705,6 +706,7 @@ __device__ __forceinline__ Token token_of(const PagedPrepArgs &a, int t) {
     const int i = k.pos / a.c.ps;
     const bool in = (unsigned)k.seq < (unsigned)a.n_seqs && k.pos >= 0 && i < a.max_pages;
     k.page = in ? a.table[(size_t)k.seq * a.max_pages + i] : -1;
+    if (in && a.pos && a.lens && k.pos >= a.lens[k.seq]) k.page = -1;
     if ((unsigned)k.page >= (unsigned)a.c.n_pages) k.page = -1;
     return k;
 }

@@ -557,7 +557,9 @@ def paged_attn_prep(q, k, v, qw, kw, eps: float, theta: float, k_pages, v_pages,
                     seq_ids=None, ks=None, vs=None, seq_lens=None):
     """QK norm (when qw/kw are given) + RoPE of the new tokens q [T, n_heads, head_dim] (into q_out, which may be q)
     and k [T, n_kv_heads, head_dim], and the store of k and v into the pages.  Token t is position positions[t] of
-    row seq_ids[t] of the block table; without them it is the last position of row t (seq_lens[t] - 1)."""
+    row seq_ids[t] of the block table (with seq_lens: not stored unless it lies before the row's end, as in a row that
+    could not be extended); without them it is the last position of row t (seq_lens[t] - 1), also if the row did not
+    grow."""
     lib = load_library()
     ptrs, (_, n_pages, nkv, ps, hd) = _pages(k_pages, v_pages, ks, vs, False)
     table, n_seqs, max_pages = _rows(block_table)

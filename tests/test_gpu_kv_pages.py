@@ -269,3 +269,68 @@ def test_upkeep_in_a_graph(gpu):
         restore()
         step()
         same(d, m, "eager")
+
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("graph", [False, True])
+def test_step_of_a_pool_that_runs_out(gpu, int8, graph):
+    """Extend and prep as a server's step calls them, the tokens named by their positions (-1: a row that takes none) and
+    the lengths: a row that could not be extended, its sibling on the same full pages and a paused row keep their pages
+    bit for bit."""
+    ps, nkv, hd, S = 16, 2, 64, 6
+    m = Model(S, 4, 9, ps, layers=1, nkv=nkv, hd=hd, int8=int8, seed=5)
+    d = Device(gpu, m)
+    # row 0: two full pages, row 1 its fork; rows 2 (paused), 3 and 5 partly filled; row 4 empty
+    for call, arg in (("extend", [32, 0, 20, 21, 0, 3]), ("fork", [-1, 0, -1, -1, -1, -1])):
+        assert getattr(d, call)(i32(arg)) == getattr(m, call)(i32(arg)) == 0
+    same(d, m, "begin")
+    assert len(m.free_pages()) == 2 and m.table[0, 1] == m.table[1, 1]
+    rng = np.random.default_rng(1)
+    new, pos, seq = dev(np.zeros(S, np.int32)), dev(np.zeros(S, np.int32)), dev(np.arange(S, dtype=np.int32))
+    active = dev(i32([1, 1, 0, 1, 0, 1]))
+    q = dev(rng.standard_normal((S, 4, hd)).astype(np.float32))
+    k, v = (dev(rng.standard_normal((S, nkv, hd)).astype(np.float32)) for _ in range(2))
+    q_out = torch.zeros_like(q)
+
+    def step():
+        torch.add(d.lens, active, out=new)
+        torch.mul(new, active, out=pos)
+        pos.sub_(1)
+        d.o.kv_pages_extend(*d.state(), new, ps, d.st)
+        d.o.paged_attn_prep(q, k, v, None, None, 1e-6, 1e4, d.arr[0][0], d.arr[1][0], d.table, q_out, pos, seq,
+                            d.arr[2][0] if int8 else None, d.arr[3][0] if int8 else None, seq_lens=d.lens)
+
+    case(f"a step of a pool that runs out int8={int8} graph={graph}")
+    run = step
+    if graph:
+        start = [t.clone() for t in (*d.state(), *d.arr)]
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            step()
+            side.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                step()
+        for t, x in zip((*d.state(), *d.arr), start):
+            t.copy_(x)
+        torch.cuda.synchronize()
+        run = g.replay
+    on = np.array([1, 1, 0, 1, 0, 1])
+    refused = []
+    for i in range(14):  # rows 0 and 1 take the two pages that are left; row 3 is stopped at its page's end, with it row 5
+        before, old = [host(a).copy() for a in d.arr], m.lens.copy()
+        n = m.extend(i32(m.lens + on))
+        run()
+        torch.cuda.synchronize()
+        assert int(host(d.st)[0]) == n
+        assert np.array_equal(host(d.lens), m.lens) and np.array_equal(host(d.table), m.table) and np.array_equal(host(d.refs), m.refs)
+        wrote = {(int(m.table[r, (m.lens[r] - 1) // ps]), int((m.lens[r] - 1) % ps)) for r in range(S) if m.lens[r] > old[r]}
+        refused.append(n)
+        for t, (a, b) in enumerate(zip(d.arr, before)):
+            x = host(a)[0] != b[0]
+            x = x.any(1) if t > 1 else x.any((1, 2)) if t == 1 else x.any((1, 3))  # [page][position]
+            assert {(int(p), int(o)) for p, o in np.argwhere(x)} <= wrote, (i, t)
+            if t < 2:
+                assert {(int(p), int(o)) for p, o in np.argwhere(x)} == wrote, (i, t)
+    assert refused[0] == 0 and max(refused) == 2

@@ -622,3 +622,30 @@ def test_value_scales_within_a_sequence(gpu, n, nkv, hd, ps, order):
             eps = 2 * (6 * np.abs(sc).max() + 16 + n) * 2.0 ** -24
             bound = (eps * (sizes @ np.abs(V)) + n * 2.0 ** -33 * 127 * sizes.max()) / w.sum()
             assert (np.abs(got[h] - want) <= bound).all(), (trial, h, np.abs(got[h] - want).max(), bound.max())
+
+
+
+def test_prep_stores_nothing_past_the_lengths(gpu):
+    """With positions and lengths, a token at or past its row's length (a row that could not be extended) is prepared
+    but not stored."""
+    rng = np.random.default_rng(17)
+    lens = np.array([5, 0, 20, 33], np.int32)
+    table = np.arange(16, dtype=np.int32).reshape(4, 4)
+    seq = np.array([0, 0, 1, 2, 2, 2, 3, 3, -1, 4], np.int32)
+    pos = np.array([4, 5, 0, 18, 20, 63, 31, 33, 2, 2], np.int32)
+    q, k, v = (rng.standard_normal((10, h, 64)).astype(np.float32) for h in (4, 2, 2))
+    for int8 in (False, True):
+        p = [opt(x) for x in pool(rng, 16, 2, 16, 64, int8)]
+        before = [None if x is None else x.clone() for x in p]
+        alone = [None if x is None else x.clone() for x in p]
+        qo, qa = torch.zeros((10, 4, 64), device="cuda"), torch.zeros((10, 4, 64), device="cuda")
+        case(f"paged prep past the lengths int8={int8}")
+        gpu.ops.paged_attn_prep(dev(q), dev(k), dev(v), None, None, 1e-6, 1e4, p[0], p[1], dev(table), qo, dev(pos), dev(seq),
+                                p[2], p[3], seq_lens=dev(lens))
+        keep = [0, 3, 6]
+        gpu.ops.paged_attn_prep(dev(q), dev(k), dev(v), None, None, 1e-6, 1e4, alone[0], alone[1], dev(table), qa, dev(pos),
+                                dev(np.where(np.isin(np.arange(10), keep), seq, -1).astype(np.int32)), alone[2], alone[3])
+        assert torch.equal(qo, qa)
+        for x, y, b in zip(p, alone, before):
+            if x is not None:
+                assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)) and not torch.equal(x, b)
