@@ -368,7 +368,8 @@ size_t mnemo_paged_cache_bytes(int n_pages, int page_size, int n_kv_heads, int h
 /* Prepares n_tokens new tokens: QK norm (when both weights are given) and RoPE of q
  * [n_tokens][n_heads][head_dim] into q_out (which may be q) and of k [n_tokens][n_kv_heads]
  * [head_dim], and the store of k and v at their positions (int8: with per-row absmax scales,
- * as mnemo_attn_prep).  k and v are not modified.  Token t is position positions[t] of sequence
+ * as mnemo_attn_prep; a row with a NaN or an infinity reads back as NaN, where mnemo_attn_prep
+ * takes a NaN for -127 steps).  k and v are not modified.  Token t is position positions[t] of sequence
  * seq_ids[t].  A token with a negative position is padding: nothing of it is written.  A position
  * beyond the table, a seq_id outside it, and, where seq_lens is given (else NULL), a position at
  * seq_lens[seq_ids[t]] or beyond is prepared but not stored.  A step that extends its rows first gives

@@ -661,7 +661,9 @@ int launch_paged_attention(const PagedAttnArgs &a, hipStream_t s) {
 // p 2^-24.
 //
 // A row that is stored (k, v) as the cache's elements, and its int8 scale.  A row whose largest
-// value is below 1e-36 (127 / m leaves the range) is stored as zeros.
+// value is below 1e-36 (127 / m leaves the range) is stored as zeros.  The largest value is found
+// among the bits, where a NaN is the largest of all: a row with a NaN or an infinity has that for
+// its scale and zeros for elements, so that all of it reads as NaN.
 template <int KV>
 struct CacheRow {
     uint32_t w0[KV == kKvF16 ? 2 : 1], w1[KV == kKvF16 ? 2 : 1];  // elements 4l .. 4l + 3, HD/2 + 4l ..
@@ -677,13 +679,15 @@ __device__ __forceinline__ CacheRow<KV> cache_row(const float (&x0)[4], const fl
         __builtin_memcpy(r.w0, &a, 8);
         __builtin_memcpy(r.w1, &b, 8);
     } else {
-        float m = 0.0f;
+        uint32_t mb = 0;
 #pragma unroll
-        for (int i = 0; i < 4; i++) m = fmaxf(m, fmaxf(fabsf(x0[i]), fabsf(x1[i])));
+        for (int i = 0; i < 4; i++)
+            mb = max(mb, max(__builtin_bit_cast(uint32_t, fabsf(x0[i])), __builtin_bit_cast(uint32_t, fabsf(x1[i]))));
 #pragma unroll
-        for (int o = 1; o < LPH; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-        const float inv = m >= 1e-36f ? 127.0f / m : 0.0f;
-        r.scale = m >= 1e-36f ? m / 127.0f : 0.0f;
+        for (int o = 1; o < LPH; o <<= 1) mb = max(mb, (uint32_t)__shfl_xor((int)mb, o));
+        const float m = __builtin_bit_cast(float, mb);
+        const float inv = m < 1e-36f ? 0.0f : 127.0f / m;
+        r.scale = m < 1e-36f ? 0.0f : m / 127.0f;
         r.w0[0] = r.w1[0] = 0;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -692,6 +696,7 @@ __device__ __forceinline__ CacheRow<KV> cache_row(const float (&x0)[4], const fl
             r.w0[0] |= (uint32_t)(a & 255) << (8 * i);
             r.w1[0] |= (uint32_t)(b & 255) << (8 * i);
         }
+        if (mb >= 0x7f800000u) r.w0[0] = r.w1[0] = 0;
     }
     return r;
 }

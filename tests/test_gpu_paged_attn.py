@@ -649,3 +649,38 @@ def test_prep_stores_nothing_past_the_lengths(gpu):
         for x, y, b in zip(p, alone, before):
             if x is not None:
                 assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)) and not torch.equal(x, b)
+
+
+
+@pytest.mark.parametrize("hd,T", [(64, 40), (128, 40), (256, 40), (64, 2100), (128, 2100), (256, 2100)])
+def test_int8_rows_that_hold_no_number(gpu, hd, T):
+    """A row with a NaN or an infinity reads back as NaN throughout, as its definition says (the scale is the largest
+    absolute value / 127); its neighbours are as without it."""
+    rng = np.random.default_rng(hd)
+    x = rng.standard_normal((T, 1, hd)).astype(np.float32)
+    ps, width = 64, -(-T // 64)
+    outs = []
+    bad = np.zeros(T, bool)
+    bad[[0, 7, 18, 33, T - 1]] = True
+    y = x.copy()
+    y[bad, 0, rng.integers(0, hd, 5)] = [np.nan, np.inf, -np.inf, np.nan, -np.inf]
+    y[18, 0, :3] = np.nan
+    for z in (x, y):
+        kp = torch.full((width, 1, ps, hd), 9, dtype=torch.int8, device="cuda")
+        vp = torch.full((width, 1, hd, ps), 9, dtype=torch.int8, device="cuda")
+        ks, vs = torch.full((width, 1, ps), 9.0, device="cuda"), torch.full((width, 1, ps), 9.0, device="cuda")
+        case(f"paged prep, int8 rows with NaN hd={hd} T={T}")
+        gpu.ops.paged_attn_prep(dev(z), dev(z), dev(z), None, None, 1e-6, 1e4, kp, vp, torch.arange(width, dtype=torch.int32, device="cuda")[None],
+                                torch.empty((T, 1, hd), device="cuda"), torch.arange(T, dtype=torch.int32, device="cuda"),
+                                torch.zeros(T, dtype=torch.int32, device="cuda"), ks, vs)
+        with np.errstate(invalid="ignore"):
+            outs.append((host(kp)[:, 0].reshape(-1, hd)[:T] * host(ks).flatten()[:T, None],
+                         host(vp)[:, 0].transpose(0, 2, 1).reshape(-1, hd)[:T] * host(vs).flatten()[:T, None]))
+    for a, b in zip(*outs):
+        assert np.isnan(b[bad]).all()
+        assert np.array_equal(a[~bad], b[~bad])
+    # attention over such a cache says so
+    q = torch.ones((1, 2, hd), device="cuda")
+    table, n = torch.arange(width, dtype=torch.int32, device="cuda")[None], torch.tensor([T], dtype=torch.int32, device="cuda")
+    for scales in ((ks, torch.nan_to_num(vs)), (torch.nan_to_num(ks), vs)):
+        assert np.isnan(host(attend(gpu, q, kp, vp, *scales, table, n, 0.1))).all()
