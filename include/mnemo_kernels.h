@@ -380,8 +380,9 @@ size_t mnemo_paged_cache_bytes(int n_pages, int page_size, int n_kv_heads, int h
  * that is not empty took a token.  A refused or paused row's last position would be overwritten,
  * in a page that other rows may share.
  * No two tokens may share a position of a sequence, nor may stored pages be shared
- * by rows.  theta >= 1, n_tokens <= 4,194,304.  Angles are exact at any position (mnemo_attn_prep
- * forms them in fp32, as the reference does: its angle at position p is off by up to p * 2^-24). */
+ * by rows.  theta >= 1, n_tokens <= 4,194,304.  The angle at position
+ * p is off by less than 10 p * 2^-64 of a turn before it is reduced and rounded to fp32
+ * (mnemo_attn_prep forms it in fp32, as the reference does: off by up to p * 2^-24). */
 int mnemo_paged_attn_prep(const float *q, const float *k, const float *v, const float *q_norm_w,
                           const float *k_norm_w, float eps, float theta, int n_tokens, int n_heads,
                           int head_dim, int n_kv_heads, const int *positions, const int *seq_ids,

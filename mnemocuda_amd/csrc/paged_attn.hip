@@ -657,8 +657,8 @@ int launch_paged_attention(const PagedAttnArgs &a, hipStream_t s) {
 // ------------------------------------------------------------------ preparation of new tokens
 // HD / 8 lanes own a head, four rotated pairs (j, j + HD/2) each.  The angle of pair j at position p
 // is p turn(j) in units of 2^-64 of a turn, formed in integers (the product keeps its low 64 bits,
-// whole turns fall off), so that it is as exact at position 10^6 as at 1: fp32 angles are off by
-// p 2^-24.
+// whole turns fall off): off by less than 10 p 2^-64 of a turn, where fp32 angles are off by p 2^-24.
+// What is left of a turn is rounded to fp32 for the sine and cosine.
 //
 // A row that is stored (k, v) as the cache's elements, and its int8 scale.  A row whose largest
 // value is below 1e-36 (127 / m leaves the range) is stored as zeros.  The largest value is found
@@ -902,13 +902,16 @@ __global__ void __launch_bounds__(256) paged_prep_kernel(PagedPrepArgs a, int v_
 
 int launch_paged_prep(PagedPrepArgs &a, double theta, hipStream_t s) {
     const int hd = a.c.hd;
-    // a turn per position is theta^(-2j/hd) / (2 pi) for pair j: the kernel forms it from the powers 2^i of the step, in
-    // whole numbers of 2^-64 (off by up to 8 of them for theta from 1 to 3e38: 2^-31 of a turn at position 2^30)
-    long double step = powl(theta, -2.0L / hd);  // <= 1
+    // A turn per position is theta^(-2j/hd) / (2 pi) for pair j: the kernel forms it from theta^(-2 2^i/hd), in whole
+    // numbers of 2^-64.  The largest i gives 1 / sqrt(theta), the others are its square roots, each of which halves what
+    // the last is off by (squares would double it).  Seven products cut off below 1 each, their factors are off by at
+    // most 1.5 (times a turn of 0.16 at most): together below 10 of 2^-64, 7.5 at most over 1000 values of theta from 1
+    // to 3e38 in extended precision.  At position 2^31 that is 2^-29.7 of a turn.
+    long double step = 1.0L / sqrtl(theta);  // <= 1
     a.turn0 = (uint64_t)(0x1p64L / (2.0L * 3.14159265358979323846264338327950288L));
-    for (uint64_t &p : a.step) {
-        p = step < 1.0L ? (uint64_t)(step * 0x1p64L) : UINT64_MAX;
-        step *= step;
+    for (int i = hd == 64 ? 4 : hd == 128 ? 5 : 6; i >= 0; i--) {
+        a.step[i] = step < 1.0L ? (uint64_t)rintl(step * 0x1p64L) : UINT64_MAX;
+        step = sqrtl(step);
     }
     // V through tiles where runs of tokens can be expected (a call by lengths has one token per sequence) and
     // there are enough tiles to hide their two phases behind the other blocks: 4 KV heads of 128, f16, 256

@@ -684,3 +684,30 @@ def test_int8_rows_that_hold_no_number(gpu, hd, T):
     table, n = torch.arange(width, dtype=torch.int32, device="cuda")[None], torch.tensor([T], dtype=torch.int32, device="cuda")
     for scales in ((ks, torch.nan_to_num(vs)), (torch.nan_to_num(ks), vs)):
         assert np.isnan(host(attend(gpu, q, kp, vp, *scales, table, n, 0.1))).all()
+
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("theta", [1.0 + 2.0 ** -23, 1.00009, 1.0104, 1e3, 3e38])
+def test_prep_far_positions_of_every_head_size(gpu, hd, theta):
+    """Bases next to 1, where the frequencies' factors are next to 1 as well, and the largest one."""
+    theta = float(np.float32(theta))
+    pos = np.array([3, 131071, 10 ** 7 + 1, 2 ** 30 + 1, 2 ** 31 - 1], np.int32)
+    rng = np.random.default_rng(15)
+    q = rng.standard_normal((len(pos), 2, hd)).astype(np.float32)
+    kv = torch.zeros((len(pos), 1, hd), device="cuda")
+    kp = torch.zeros((1, 1, 16, hd), dtype=torch.float16, device="cuda")
+    vp = torch.zeros((1, 1, hd, 16), dtype=torch.float16, device="cuda")
+    qd = dev(q)
+    case(f"paged prep, far positions, hd={hd} theta={theta}")
+    gpu.ops.paged_attn_prep(qd, kv, kv, None, None, 1e-6, theta, kp, vp, torch.full((1, 1), -1, dtype=torch.int32, device="cuda"),
+                            qd, dev(pos), torch.zeros(len(pos), dtype=torch.int32, device="cuda"))
+    # the angle in extended precision, whose frequencies are off by 2^-63 of themselves (4 roundings), products by as much
+    f = np.longdouble(theta) ** (-2 * np.arange(hd // 2, dtype=np.longdouble) / hd)
+    a = np.fmod(pos.astype(np.longdouble)[:, None] * f, 2 * np.arccos(np.longdouble(-1)))
+    c, s = np.cos(a)[:, None].astype(np.float64), np.sin(a)[:, None].astype(np.float64)
+    x0, x1 = q[..., :hd // 2].astype(np.float64), q[..., hd // 2:].astype(np.float64)
+    want = np.concatenate([x0 * c - x1 * s, x1 * c + x0 * s], -1)
+    # the kernel's angle: 10 p 2^-64 and, cut off when it is reduced, 2^-32 of a turn
+    off = (pos.astype(np.float64) * (2.0 ** -64 * 10 * 2 * math.pi + 2.0 ** -60) + 2.0 ** -32 * 2 * math.pi)[:, None, None]
+    assert (np.abs(host(qd) - want) <= (ROT + off) * np.abs(want).max(-1, keepdims=True)).all()
