@@ -3,6 +3,7 @@
 //
 // Pages: K [page][n_kv][ps][hd], V [page][n_kv][hd][ps] (8 consecutive positions of a dim are
 // contiguous, a matrix instruction's operand), int8 scales [page][n_kv][ps].
+#include <limits.h>
 #include <math.h>
 
 #include "mnemo_common.hpp"
@@ -338,8 +339,10 @@ __global__ void __launch_bounds__((PaShape<KV, HD, STEP>::kThreads)) paged_attn_
                         s[t][i] = x;
                         smax = fmaxf(smax, x);
                     }
-                if (__any(smax > m + kSlack)) {
-                    float mn = max_heads(smax), al, f;
+                bool rescale = __any(smax > m + kSlack);  // uniform
+                float f = 1.0f;
+                if (rescale) {
+                    float mn = max_heads(smax), al;
                     if (KV == kKvF16) {
                         mn = fmaxf(m, mn);
                         f = al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -352,8 +355,6 @@ __global__ void __launch_bounds__((PaShape<KV, HD, STEP>::kThreads)) paged_attn_
                         f = w * inverse2(wref);
                     }
                     l *= al;
-#pragma unroll
-                    for (int i = 0; i < ND; i++) o[i] *= f;
                     m = mn;
                 }
                 const float ref = m == -INFINITY ? 0.0f : KV == kKvF16 ? m - kLift : m;
@@ -373,12 +374,15 @@ __global__ void __launch_bounds__((PaShape<KV, HD, STEP>::kThreads)) paged_attn_
                         // the power of two at or below the largest (at most 2^126) becomes 2^kLift
                         const uint32_t e = min(__builtin_bit_cast(uint32_t, max_heads(wmax)) & 0x7f800000u, 0x7e800000u);
                         const float wn = fmaxf(wref, __builtin_bit_cast(float, e) * exp2f(-kLift));
-                        const float f = wref * inverse2(wn);
-#pragma unroll
-                        for (int i = 0; i < ND; i++) o[i] *= f;
+                        f *= wref * inverse2(wn);
                         wref = wn;
+                        rescale = true;
                     }
                     wi = inverse2(wref);
+                }
+                if (rescale) {
+#pragma unroll
+                    for (int i = 0; i < ND; i++) o[i] *= f;
                 }
                 h8 phi[PV], plo[PV];
 #pragma unroll
@@ -710,9 +714,10 @@ __device__ __forceinline__ Token token_of(const PagedPrepArgs &a, int t) {
     k.pos = a.pos ? a.pos[t] : a.lens[t] - 1;
     const int i = k.pos / a.c.ps;
     const bool in = (unsigned)k.seq < (unsigned)a.n_seqs && k.pos >= 0 && i < a.max_pages;
+    int end = INT_MAX;
+    if (in && a.pos && a.lens) end = a.lens[k.seq];
     k.page = in ? a.table[(size_t)k.seq * a.max_pages + i] : -1;
-    if (in && a.pos && a.lens && k.pos >= a.lens[k.seq]) k.page = -1;
-    if ((unsigned)k.page >= (unsigned)a.c.n_pages) k.page = -1;
+    if ((unsigned)k.page >= (unsigned)a.c.n_pages || k.pos >= end) k.page = -1;
     return k;
 }
 
