@@ -594,8 +594,9 @@ int mnemo_moe_decode_rmsnorm_noalloc(const float *router_w, const void *experts,
 }
 
 // ------------------------------------------------------------------ paged cache
-static int check_pages(const char *what, const KvPagesArgs &a) {
-    if (!a.table || !a.lens || !a.refs) return set_error(kErrBadArg, "%s: NULL block table, lengths or references", what);
+static int check_pages(const char *what, const KvPagesArgs &a, bool needs_lens = true) {
+    if (!a.table || !a.refs || (needs_lens && !a.lens))
+        return set_error(kErrBadArg, "%s: NULL block table, lengths or references", what);
     if (a.n_seqs <= 0 || a.n_seqs > kMaxSeqs || a.max_pages <= 0 || a.n_pages <= 0 || a.n_pages > 1 << 30)
         return set_error(kErrBadArg, "%s: need 1 <= n_seqs <= %d, max_pages > 0 and 1 <= n_pages <= 2^30", what, kMaxSeqs);
     if (a.ps != 16 && a.ps != 32 && a.ps != 64 && a.ps != 128)
@@ -666,7 +667,7 @@ int mnemo_paged_attn_prep(const float *q, const float *k, const float *v, const 
 }
 
 size_t mnemo_paged_attention_workspace_bytes(int n_heads, int n_kv_heads, int head_dim) {
-    return n_heads > 0 && n_kv_heads > 0 && head_dim > 0 ? paged_attn_workspace_bytes(n_kv_heads, head_dim) : 0;
+    return n_heads > 0 && n_kv_heads > 0 && head_dim > 0 ? paged_attn_workspace_bytes(head_dim) : 0;
 }
 
 int mnemo_paged_attention_decode(const float *q, const void *k_pages, const void *v_pages, const float *k_scales,
@@ -686,9 +687,9 @@ int mnemo_paged_attention_decode(const float *q, const void *k_pages, const void
         return set_error(kErrBadArg, "%s: need 1 <= n_seqs <= %d and 1 <= max_pages * page_size <= 2^30", what, kMaxSeqs);
     if ((long long)n_seqs * n_kv_heads * max_pages * page_size >= 1LL << 36)  // its steps are counted in an int
         return set_error(kErrBadArg, "%s: n_seqs * n_kv_heads * max_pages * page_size must be below 2^36", what);
-    if ((uintptr_t)workspace % 16 || workspace_bytes < paged_attn_workspace_bytes(n_kv_heads, head_dim))
+    if ((uintptr_t)workspace % 16 || workspace_bytes < paged_attn_workspace_bytes(head_dim))
         return set_error(kErrBadArg, "%s: workspace not 16-byte aligned, or %zu < %zu bytes", what, workspace_bytes,
-                         paged_attn_workspace_bytes(n_kv_heads, head_dim));
+                         paged_attn_workspace_bytes(head_dim));
     a.q = q;
     a.out = out;
     a.table = block_table;
@@ -699,7 +700,6 @@ int mnemo_paged_attention_decode(const float *q, const void *k_pages, const void
     a.gqa = n_heads / n_kv_heads;
     a.scale = scale;
     a.ws = (float *)workspace;
-    a.ws_bytes = workspace_bytes;
     return launch_paged_attention(a, s);
 }
 
@@ -752,9 +752,9 @@ int mnemo_kv_pages_compact(int *block_table, int *page_refs, int n_seqs, int max
                            int n_kv_heads, int head_dim, int *n_live, void *workspace, size_t workspace_bytes,
                            hipStream_t s) {
     // compaction needs no lengths: every table entry at n or above is renamed
-    const KvPagesArgs a = {block_table, block_table, page_refs, n_seqs, max_pages, n_pages, page_size};
+    const KvPagesArgs a = {block_table, nullptr, page_refs, n_seqs, max_pages, n_pages, page_size};
     const PagedCache c = {k_pages, v_pages, k_scales, v_scales, kv_type, n_pages, page_size, n_kv_heads, head_dim};
-    if (int rc = check_pages("kv_pages_compact", a)) return rc;
+    if (int rc = check_pages("kv_pages_compact", a, false)) return rc;
     if (int rc = check_moving("kv_pages_compact", c, n_layers, workspace, workspace_bytes,
                               kv_pages_workspace_bytes(n_seqs, n_pages)))
         return rc;

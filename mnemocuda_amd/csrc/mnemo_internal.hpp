@@ -202,9 +202,8 @@ struct PagedAttnArgs {
     int n_seqs, max_pages, nh, gqa;
     float scale;
     float *ws;
-    size_t ws_bytes;
 };
-size_t paged_attn_workspace_bytes(int nkv, int hd);
+size_t paged_attn_workspace_bytes(int hd);
 int launch_paged_attention(const PagedAttnArgs &a, hipStream_t s);
 
 struct PagedPrepArgs {
@@ -223,7 +222,7 @@ struct PagedPrepArgs {
 int launch_paged_prep(PagedPrepArgs &a, double theta, hipStream_t s);
 
 struct KvPagesArgs {
-    int *table, *lens, *refs;
+    int *table, *lens, *refs;  // (compaction: lens NULL)
     int n_seqs, max_pages, n_pages, ps;
 };
 int launch_kv_extend(const KvPagesArgs &a, const int *new_lens, int *status, hipStream_t s);

@@ -65,7 +65,7 @@ constexpr int kPaGroups = 256;  // one per CU
 // (sequence, KV head) that begins in workgroup g's share and goes on behind it (its second partial), taken[g]
 // the one that it goes on with from the workgroup before (its first), -1 for none.
 __host__ __device__ constexpr int part_floats(int hd) { return kPaRows * (hd + 2); }
-size_t paged_attn_workspace_bytes(int, int hd) {
+size_t paged_attn_workspace_bytes(int hd) {
     return (size_t)2 * kPaGroups * (part_floats(hd) * sizeof(float) + sizeof(int));
 }
 __device__ __forceinline__ int *pa_begun(const PagedAttnArgs &a) {
