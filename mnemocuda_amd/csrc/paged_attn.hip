@@ -28,10 +28,10 @@ namespace mnemo {
 // one dim.
 //
 // Bound by memory: 96 sequences to 8192 positions (957 MB) take 172 us, 5.5 TB/s, where a plain read of
-// as much reaches 6.2; 3 int8 sequences to 131,072 (324 MB) 67.5 us.  A CU has room for one workgroup and
-// ~20 GB/s of loads, so shares are spread over the CUs first; what a small call takes is its chain of
-// loads: lengths, table, K, V, then the same for the merge (300 positions: 8.5 us, of which 3 are the
-// second launch).
+// as much reaches 6.2; 3 int8 sequences to 131,072 (324 MB) 67.5 us.  A CU holds one workgroup, so
+// shares are spread over the CUs first (300 positions 11.3 us on 4 CUs, 8.3 on 40); what a small call
+// takes is its chain of loads: lengths, table, K, V, then the same for the merge (300 positions: 8.5 us,
+// of which 3.1 are the second launch; it takes 3.1 to 3.9 of every call that has it).
 //
 // Precision: Q is scaled by a power of two into [1, 2) per head and split into two f16 parts, P
 // likewise split; K and V enter exactly (f16 or int8).  P is formed relative to a reference that
@@ -53,7 +53,8 @@ template <int KV, int HD, int STEP>
 struct PaShape {
     static constexpr int kTiles = STEP / 16;
     static constexpr int kKs = HD / 32, kNd = HD / 16;  // dim steps of S, dim tiles of O
-    // one workgroup per CU; its pieces fill LDS (135 KB at head_dim 128)
+    // one workgroup per CU, whose pieces take most of its LDS (134 KB at head_dim 128 and 256; 70 KB at 64, where
+    // there is room for a second one that is not launched)
     static constexpr int kWaves = HD == 256 ? 4 : 8;
     // the parts of Q wait in LDS where registers are short
     static constexpr bool kQInLds = HD == 128 && STEP == 64;
@@ -630,8 +631,8 @@ static void launch_pa(const PagedAttnArgs &a, hipStream_t s) {
     const long long most = pairs * (((long long)a.max_pages * a.c.ps + STEP - 1) / STEP);  // steps
     const int groups = (int)(most < kPaGroups ? most : kPaGroups);
     // Tables of up to four steps: no (sequence, KV head) is cut between workgroups, and nothing is left to merge (100
-    // sequences to 60 positions 7.0 us against 9.2 with the merge launch).  Longer ones are cut: a CU alone loads no
-    // more than ~20 GB/s, and 300 positions of one sequence take 11.3 us on 4 CUs against 8.3 on 40.
+    // sequences to 60 positions 7.0 us against 9.2 with the merge launch).  Longer ones are cut: 300 positions of one
+    // sequence take 11.3 us on 4 CUs against 8.3 on 40, the merge launch included.
     const bool whole_pairs = most <= 4 * pairs;
     hipLaunchKernelGGL((paged_attn_kernel<KV, HD, STEP>), dim3(groups), dim3(S::kThreads), 0, s, a, (int)whole_pairs);
     if (whole_pairs) return;

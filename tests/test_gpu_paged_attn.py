@@ -711,3 +711,30 @@ def test_prep_far_positions_of_every_head_size(gpu, hd, theta):
     # the kernel's angle: 10 p 2^-64 and, cut off when it is reduced, 2^-32 of a turn
     off = (pos.astype(np.float64) * (2.0 ** -64 * 10 * 2 * math.pi + 2.0 ** -60) + 2.0 ** -32 * 2 * math.pi)[:, None, None]
     assert (np.abs(host(qd) - want) <= (ROT + off) * np.abs(want).max(-1, keepdims=True)).all()
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_tokens_of_chunks_as_rows(gpu, int8):
+    """Chunks of prompts: stored in one call, then attended with a table that has a row for every token, a copy of its
+    sequence's, and the length up to it: causal, over the pages that the rows share."""
+    rng = np.random.default_rng(31)
+    ps, nkv, G, hd = 32, 2, 4, 128
+    begin, n = np.array([0, 70, 31, 5]), np.array([130, 33, 2, 1])
+    lens = (begin + n).astype(np.int32)
+    n_pages = int(sum(-(-lens // ps))) + 2
+    pages = pool(rng, n_pages, nkv, ps, hd, int8)
+    table = block_table(rng, lens, ps, 6, n_pages)
+    seq = np.repeat(np.arange(4), n).astype(np.int32)
+    pos = np.concatenate([np.arange(b, b + m) for b, m in zip(begin, n)]).astype(np.int32)
+    T = len(seq)
+    q, k, v = (rng.standard_normal((T, h, hd)).astype(np.float32) for h in (nkv * G, nkv, nkv))
+    p = [opt(x) for x in pages]
+    qo = torch.empty((T, nkv * G, hd), device="cuda")
+    case(f"chunks as rows int8={int8}")
+    gpu.ops.paged_attn_prep(dev(q), dev(k), dev(v), None, None, 1e-6, 1e4, p[0], p[1], dev(table), qo, dev(pos), dev(seq), p[2],
+                            p[3], seq_lens=dev(lens))
+    got = host(attend(gpu, qo, *p, table[seq], pos + 1, hd ** -0.5))
+    stored = [None if x is None else host(x) for x in p]
+    want = reference(host(qo), *stored, table[seq], pos + 1, hd ** -0.5)
+    for t in range(T):
+        assert rel_l2(got[t], want[t]) <= BAR, (t, seq[t], pos[t])
