@@ -28,10 +28,10 @@ namespace mnemo {
 // one dim.
 //
 // Bound by memory: 96 sequences to 8192 positions (957 MB) take 172 us, 5.5 TB/s, where a plain read of
-// as much reaches 6.2; 3 int8 sequences to 131,072 (324 MB) 67.5 us.  A CU holds one workgroup, so
+// as much reaches 6.2; 3 int8 sequences to 131,072 (324 MB) 67.5 us.  A CU is given one workgroup, so
 // shares are spread over the CUs first (300 positions 11.3 us on 4 CUs, 8.3 on 40); what a small call
 // takes is its chain of loads: lengths, table, K, V, then the same for the merge (300 positions: 8.5 us,
-// of which 3.1 are the second launch; it takes 3.1 to 3.9 of every call that has it).
+// of which 3.1 are the second launch; 3.1 to 3.9 of five calls from 8.5 to 172 us).
 //
 // Precision: Q is scaled by a power of two into [1, 2) per head and split into two f16 parts, P
 // likewise split; K and V enter exactly (f16 or int8).  P is formed relative to a reference that
