@@ -462,6 +462,57 @@ int mnemo_logits_process(const float *logits, float *out, int n_rows, int vocab,
                          const int *bias_ids, const float *bias, int n_bias,
                          const unsigned *allowed, hipStream_t stream);
 
+/* ---- Prompts of several requests (no reference counterpart: it takes a prompt token by token,
+ * src/forward.c:1783-1830) ------------------------------------------------------------------
+ *
+ * Routing of n_tokens tokens from their router logits [n_tokens][n_experts], for mnemo_moe_prefill:
+ *   s_e = 1 / (1 + exp(-z_e)) (score 1) or exp(z_e) / sum_f exp(z_f) (score 0);  c_e = s_e + bias[e]
+ *   The experts are n_groups runs of n_experts / n_groups.  A group scores the sum of its group_best
+ *   (1 or 2) largest c; the top_groups best groups are kept (ties to the lower index).
+ *   topk_idx[t] = the k experts of largest c in the kept groups, best first, ties to the lower index
+ *   topk_w[t] = scale * s of those, divided by their sum where renormalise is not 0
+ * (bias NULL: none.)  The choice is made in 64 bits, c within 2^-42 of each other being a tie.  An expert whose logit or bias is
+ * -inf is never chosen; a slot that no expert is left for gets id -1 and weight 0 (mnemo_moe_prefill
+ * skips it).  A token whose scores hold a NaN (of a logit that is none, or +inf with score 0) gets
+ * ids -1 and weights NaN.  k <= 16, k <= n_experts <= 1024, n_experts % n_groups == 0, n_groups <= 64,
+ * n_tokens * k <= 4,194,304. */
+int mnemo_moe_route(const float *logits, int n_tokens, int n_experts, int score, const float *bias,
+                    int n_groups, int top_groups, int group_best, int k, int renormalise,
+                    float scale, int *topk_idx, float *topk_w, hipStream_t stream);
+
+/* Low-rank adapters beside a projection that all requests share:
+ *   out[t] = base[t] + scales[a] * B_a (A_a x[t]),  a = adapter_ids[t]
+ * x [n_tokens][n_in], base and out [n_tokens][n_out] fp32 (out may be base, but not overlap it or x
+ * otherwise); a_w [n_adapters][max_rank][n_in] and b_w [n_adapters][n_out][max_rank] of f16
+ * (adapter_type 0) or bf16 (1), 16-byte aligned; ranks[a] <= max_rank: what lies behind it in a_w
+ * and b_w is not used.  A token whose id lies outside 0..n_adapters-1, or whose adapter's rank is
+ * 0 or less, gets its base.  A token whose x holds a NaN or an infinity gets no numbers; no
+ * token depends on another's x or adapter.  n_in and max_rank multiples of 8, max_rank <= 256,
+ * n_in <= 1,048,576, n_tokens <= 524,288, n_adapters <= 65536.  workspace:
+ * mnemo_lora_workspace_bytes(...) bytes, 16-byte aligned, no initialisation; calls sharing it must
+ * not overlap. */
+size_t mnemo_lora_workspace_bytes(int n_tokens, int n_in, int max_rank);
+int mnemo_lora_add(const float *x, const void *a_w, const void *b_w, int adapter_type,
+                   const int *adapter_ids, const int *ranks, const float *scales, const float *base,
+                   float *out, int n_tokens, int n_in, int n_out, int n_adapters, int max_rank,
+                   void *workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* What rows of logits [n_rows][vocab] say of tokens, with log p = z - log(sum exp(z)) of a row:
+ *   logprob[r] = log p of targets[r], rank[r] = 1 + the tokens before it in the order (z falling, id
+ *   rising); a target outside the vocabulary (padding) gets 0 and rank 0
+ *   entropy[r] = -sum p log p
+ *   top_ids[r][i], top_logprobs[r][i] = the n_top likeliest tokens in that order; tokens of -inf are
+ *   none of them (id -1, -inf)
+ * targets NULL: logprob and rank are not used; rank, entropy NULL: not wanted; n_top 0: no
+ * alternatives.  A row that is -inf everywhere has log p = -inf and entropy 0; one with a NaN or +inf
+ * gets NaN, rank 0 and ids -1.  n_rows <= 65535, vocab <= 2^30, n_top <= 64.  workspace:
+ * mnemo_logprobs_workspace_bytes(...) bytes, 16-byte aligned, no initialisation; calls sharing it
+ * must not overlap. */
+size_t mnemo_logprobs_workspace_bytes(int n_rows, int vocab, int n_top);
+int mnemo_logprobs(const float *logits, const int *targets, int n_rows, int vocab, float *logprob,
+                   int *rank, float *entropy, int n_top, int *top_ids, float *top_logprobs,
+                   void *workspace, size_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -805,4 +805,118 @@ int mnemo_logits_process(const float *logits, float *out, int n_rows, int vocab,
     return launch_logits_process(a, s);
 }
 
+// ------------------------------------------------------------------ batches that hold prompts
+int mnemo_moe_route(const float *logits, int n_tokens, int n_experts, int score, const float *bias, int n_groups,
+                    int top_groups, int group_best, int k, int renormalise, float scale, int *topk_idx, float *topk_w,
+                    hipStream_t s) {
+    const char *what = "moe_route";
+    if (n_experts <= 0 || n_experts > 1024 || k <= 0 || k > 16 || k > n_experts)
+        return set_error(kErrBadArg, "%s: need 1 <= k <= 16 and k <= n_experts <= 1024", what);
+    if (n_groups <= 0 || n_groups > 64 || n_experts % n_groups || top_groups <= 0 || top_groups > n_groups)
+        return set_error(kErrBadArg, "%s: need 1 <= top_groups <= n_groups <= 64, n_groups a divisor of n_experts", what);
+    if (score != 0 && score != 1) return set_error(kErrBadArg, "%s: score %d (0 softmax, 1 sigmoid)", what, score);
+    if (group_best != 1 && group_best != 2) return set_error(kErrBadArg, "%s: group_best %d (1, 2)", what, group_best);
+    if (n_tokens < 0 || (long long)n_tokens * k > 4194304)
+        return set_error(kErrBadArg, "%s: need 0 <= n_tokens * k <= 4194304", what);
+    if (n_tokens == 0) return kOk;
+    if (!logits || !topk_idx || !topk_w) return set_error(kErrBadArg, "%s: NULL pointer", what);
+    RouteArgs a = {};
+    a.z = logits;
+    a.n_tokens = n_tokens;
+    a.n_experts = n_experts;
+    a.sigmoid = score;
+    a.bias = bias;
+    a.n_groups = n_groups;
+    a.top_groups = top_groups;
+    a.best = group_best;
+    a.k = k;
+    a.renorm = renormalise;
+    a.scale = scale;
+    a.idx = topk_idx;
+    a.w = topk_w;
+    return launch_route(a, s);
+}
+
+static bool lora_sizes(int n_tokens, int n_in, int max_rank) {
+    return n_tokens >= 0 && n_tokens <= 524288 && n_in > 0 && n_in <= 1 << 20 && n_in % 8 == 0 && max_rank > 0 &&
+           max_rank <= 256 && max_rank % 8 == 0;
+}
+
+size_t mnemo_lora_workspace_bytes(int n_tokens, int n_in, int max_rank) {
+    return lora_sizes(n_tokens, n_in, max_rank) ? lora_workspace_bytes(n_tokens, n_in, max_rank) : 0;
+}
+
+int mnemo_lora_add(const float *x, const void *a_w, const void *b_w, int adapter_type, const int *adapter_ids,
+                   const int *ranks, const float *scales, const float *base, float *out, int n_tokens, int n_in,
+                   int n_out, int n_adapters, int max_rank, void *workspace, size_t workspace_bytes, hipStream_t s) {
+    const char *what = "lora_add";
+    if (!lora_sizes(n_tokens, n_in, max_rank))
+        return set_error(kErrBadArg, "%s: need 0 <= n_tokens <= 524288, n_in (to 2^20) and max_rank (to 256) multiples of 8",
+                         what);
+    if (n_out <= 0 || n_out > 1 << 24 || n_adapters <= 0 || n_adapters > 65536)
+        return set_error(kErrBadArg, "%s: need 1 <= n_out <= 2^24 and 1 <= n_adapters <= 65536", what);
+    if (adapter_type != 0 && adapter_type != 1)
+        return set_error(kErrBadArg, "%s: adapter_type %d (0 f16, 1 bf16)", what, adapter_type);
+    if (n_tokens == 0) return kOk;
+    if (!x || !a_w || !b_w || !adapter_ids || !ranks || !scales || !base || !out || !workspace)
+        return set_error(kErrBadArg, "%s: NULL pointer", what);
+    if (((uintptr_t)a_w | (uintptr_t)b_w) % 16) return set_error(kErrBadArg, "%s: a_w and b_w must be 16-byte aligned", what);
+    const size_t need = lora_workspace_bytes(n_tokens, n_in, max_rank);
+    if ((uintptr_t)workspace % 16 || workspace_bytes < need)
+        return set_error(kErrBadArg, "%s: workspace not 16-byte aligned, or %zu < %zu bytes", what, workspace_bytes, need);
+    LoraArgs a = {};
+    a.x = x;
+    a.base = base;
+    a.out = out;
+    a.a = a_w;
+    a.b = b_w;
+    a.bf16 = adapter_type;
+    a.ids = adapter_ids;
+    a.ranks = ranks;
+    a.scales = scales;
+    a.n_tokens = n_tokens;
+    a.K = n_in;
+    a.M = n_out;
+    a.n_adapters = n_adapters;
+    a.max_rank = max_rank;
+    a.ws = (float *)workspace;
+    return launch_lora(a, s);
+}
+
+static bool logprobs_sizes(int n_rows, int vocab, int n_top) {
+    return n_rows >= 0 && n_rows <= 65535 && vocab > 0 && vocab <= 1 << 30 && n_top >= 0 && n_top <= 64;
+}
+
+size_t mnemo_logprobs_workspace_bytes(int n_rows, int vocab, int n_top) {
+    return n_rows > 0 && logprobs_sizes(n_rows, vocab, n_top) ? logprobs_workspace_bytes(n_rows, vocab, n_top) : 0;
+}
+
+int mnemo_logprobs(const float *logits, const int *targets, int n_rows, int vocab, float *logprob, int *rank,
+                   float *entropy, int n_top, int *top_ids, float *top_logprobs, void *workspace,
+                   size_t workspace_bytes, hipStream_t s) {
+    const char *what = "logprobs";
+    if (!logprobs_sizes(n_rows, vocab, n_top))
+        return set_error(kErrBadArg, "%s: need 0 <= n_rows <= 65535, 1 <= vocab <= 2^30 and 0 <= n_top <= 64", what);
+    if (n_rows == 0) return kOk;
+    if (!logits || (targets && !logprob) || (n_top && (!top_ids || !top_logprobs)))
+        return set_error(kErrBadArg, "%s: logits, or a place for what is asked for, is NULL", what);
+    const size_t need = logprobs_workspace_bytes(n_rows, vocab, n_top);
+    if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need)
+        return set_error(kErrBadArg, "%s: workspace NULL, not 16-byte aligned, or %zu < %zu bytes", what, workspace_bytes,
+                         need);
+    LogprobsArgs a = {};
+    a.z = logits;
+    a.targets = targets;
+    a.n_rows = n_rows;
+    a.vocab = vocab;
+    a.k = n_top;
+    a.logp = logprob;
+    a.rank = targets ? rank : nullptr;
+    a.entropy = entropy;
+    a.ids = top_ids;
+    a.tops = top_logprobs;
+    a.ws = workspace;
+    return launch_logprobs(a, s);
+}
+
 }  // extern "C"

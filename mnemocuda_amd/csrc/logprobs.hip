@@ -1,0 +1,313 @@
+// logprobs.hip -- log probabilities of given tokens, their ranks, the entropy and the likeliest tokens of rows of
+// logits.
+//
+// With m = max z, S = sum exp(z - m), T = sum exp(z - m) (z - m):
+//   log p_t = z_t - m - log S,   entropy = -sum p log p = log S - T / S,
+//   rank = 1 + the tokens before t in the order (z falling, index rising).
+// One pass over the logits: a thread keeps m, S and T of what it has seen (S and T are rescaled when m rises)
+// and the count of tokens before t.  A wave keeps its likeliest tokens as 64 sorted keys, one a lane: the bits of
+// z as a whole number that orders as z does, over the complement of the index.  Few tokens get so far as to be
+// looked at: a thread compares the largest of its 16 logits with the workgroup's n-th best so far.  Lists are
+// merged as two halves of a bitonic sequence.
+// Rows are cut into parts where they are few; a second launch joins the parts.
+#include <float.h>
+#include <math.h>
+
+#include "mnemo_common.hpp"
+#include "mnemo_internal.hpp"
+
+namespace mnemo {
+
+typedef float lpf4 __attribute__((ext_vector_type(4)));
+
+constexpr int kLpThreads = 256, kLpWaves = kLpThreads / 64;
+constexpr int kLpWords = 4;                           // words of four logits per thread and step
+constexpr int kLpStep = 4 * kLpThreads * kLpWords;    // logits of a step
+constexpr float kLpLog2e = 1.44269504088896341f;
+
+struct LpSums {
+    float m, S, T;  // m is at least -FLT_MAX: a row without any number has S = 0
+    int before;     // tokens before the target
+};
+
+// what d = m - (larger m) turns S and T into
+__device__ __forceinline__ void lp_rescale(double &S, double &T, double d) {
+    const double f = exp(d);
+    T = f * (T + S * fmax(d, -1e30));
+    S = f * S;
+}
+
+__device__ __forceinline__ uint32_t order32(float v) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f);  // one zero
+    return b >> 31 ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float unorder32(uint32_t b) {
+    return __builtin_bit_cast(float, b >> 31 ? b & 0x7fffffffu : ~b);
+}
+__device__ __forceinline__ uint64_t lp_key(float z, int id) { return (uint64_t)order32(z) << 32 | (0xffffffffu - (uint32_t)id); }
+
+__device__ __forceinline__ uint64_t lane64(uint64_t v, int l) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, l), hi = __builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), l);
+    return (uint64_t)hi << 32 | lo;
+}
+__device__ __forceinline__ uint64_t xor64(uint64_t v, int o) { return __shfl_xor((unsigned long long)v, o); }
+
+// One step of a sorting network: lanes whose bit o is clear take the larger where `down` is set.
+__device__ __forceinline__ uint64_t lp_exchange(uint64_t v, int o, bool down) {
+    const uint64_t w = xor64(v, o);
+    const bool larger = ((lane_id() & o) == 0) == down;
+    return (v > w) == larger ? v : w;
+}
+// a bitonic sequence, sorted falling
+__device__ __forceinline__ uint64_t lp_merge(uint64_t v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = lp_exchange(v, o, true);
+    return v;
+}
+__device__ __forceinline__ uint64_t lp_sort(uint64_t v) {
+#pragma unroll
+    for (int n = 2; n <= 64; n <<= 1)
+#pragma unroll
+        for (int o = n >> 1; o > 0; o >>= 1) v = lp_exchange(v, o, (lane_id() & n) == 0 || n == 64);
+    return v;
+}
+// the 64 largest of two lists, sorted
+__device__ __forceinline__ uint64_t lp_join(uint64_t a, uint64_t b) {
+    const uint64_t r = __shfl((unsigned long long)b, 63 - lane_id());
+    return lp_merge(a > r ? a : r);
+}
+
+// What is known of a row goes out (wave 0): list is sorted.
+__device__ __forceinline__ void lp_finish(const LogprobsArgs &a, int r, double m, double S, double T, int before, float zt,
+                                          int t, uint64_t list) {
+    const int lane = lane_id();
+    const double logS = log(S);
+    const bool none = S == 0.0, bad = S != S;
+    if (lane == 0) {
+        if (a.targets) {
+            const bool in = (unsigned)t < (unsigned)a.vocab;
+            float lp = (float)((double)zt - m - logS);
+            if (none) lp = -INFINITY;
+            if (bad) lp = NAN;
+            a.logp[r] = in ? lp : 0.0f;
+            if (a.rank) a.rank[r] = in && !bad ? before + 1 : 0;
+        }
+        if (a.entropy) a.entropy[r] = bad ? NAN : none ? 0.0f : (float)(logS - T / S);
+    }
+    if (lane < a.k) {
+        const float z = unorder32((uint32_t)(list >> 32));
+        const bool is = list != 0 && z > -INFINITY && !bad;
+        a.ids[(size_t)r * a.k + lane] = is ? (int)(0xffffffffu - (uint32_t)list) : -1;
+        a.tops[(size_t)r * a.k + lane] = bad ? NAN : is ? (float)((double)z - m - logS) : -INFINITY;
+    }
+}
+
+// sums over the wave, in every lane
+__device__ __forceinline__ void lp_join_lanes(double &m, double &S, double &T, int &before) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const double m2 = __shfl_xor(m, o);
+        double S2 = __shfl_xor(S, o), T2 = __shfl_xor(T, o);
+        before += __shfl_xor(before, o);
+        const double mn = fmax(m, m2);
+        if (m < mn) lp_rescale(S, T, m - mn);
+        if (m2 < mn) lp_rescale(S2, T2, m2 - mn);
+        m = mn;
+        S += S2;
+        T += T2;
+    }
+}
+
+template <bool TOP>
+__global__ void __launch_bounds__(kLpThreads) logprobs_kernel(LogprobsArgs a, int per_part) {
+    __shared__ uint64_t lists[TOP ? kLpWaves : 1][64];
+    __shared__ LpSums sums[kLpWaves];
+    __shared__ uint32_t floor_;  // the best of the waves' n-th best so far (as order32)
+    const int r = blockIdx.y, part = blockIdx.x, tid = threadIdx.x, lane = lane_id(), wave = tid >> 6;
+    const float *z = a.z + (size_t)r * a.vocab;
+    const int from = part * per_part, to = min(a.vocab, from + per_part);
+    if (TOP && tid == 0) floor_ = 0;
+
+    const int t = a.targets ? a.targets[r] : -1;
+    const float zt = (unsigned)t < (unsigned)a.vocab ? z[t] : INFINITY;
+
+    lpf4 x[kLpWords];
+    auto load = [&](int at) {
+#pragma unroll
+        for (int g = 0; g < kLpWords; g++) {
+            const int i = at + 4 * (kLpThreads * g + tid);
+            if (i + 3 < to) __builtin_memcpy(&x[g], z + i, 16);
+            else
+                for (int j = 0; j < 4; j++) x[g][j] = i + j < to ? z[i + j] : -INFINITY;
+        }
+    };
+    load(from);
+    LpSums s = {-FLT_MAX, 0.0f, 0.0f, 0};
+    uint64_t list = 0;
+    float least = -INFINITY;  // the wave's n-th best so far
+    if (TOP) __syncthreads();
+    for (int at = from; at < to; at += kLpStep) {
+        lpf4 y[kLpWords];
+#pragma unroll
+        for (int g = 0; g < kLpWords; g++) y[g] = x[g];
+        if (at + kLpStep < to) load(at + kLpStep);
+        float top = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < kLpWords; g++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) top = fmaxf(top, y[g][j]);
+        if (top > s.m) {
+            const float d = s.m - top, f = __builtin_amdgcn_exp2f(d * kLpLog2e);
+            s.T = f * fmaf(s.S, fmaxf(d, -1e30f), s.T);
+            s.S *= f;
+            s.m = top;
+        }
+#pragma unroll
+        for (int g = 0; g < kLpWords; g++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float d = y[g][j] - s.m, e = __builtin_amdgcn_exp2f(d * kLpLog2e);
+                s.S += e;
+                s.T = fmaf(e, fmaxf(d, -1e30f), s.T);
+            }
+        const int first = at + 4 * tid;
+        if (a.rank) {
+            if (at + kLpStep <= t) {
+#pragma unroll
+                for (int g = 0; g < kLpWords; g++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) s.before += y[g][j] >= zt;
+            } else if (at > t) {
+#pragma unroll
+                for (int g = 0; g < kLpWords; g++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) s.before += y[g][j] > zt;
+            } else {
+#pragma unroll
+                for (int g = 0; g < kLpWords; g++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        s.before += y[g][j] > zt || (y[g][j] == zt && first + 4 * kLpThreads * g + j < t);
+            }
+        }
+        if (TOP) {
+            uint64_t own = 0;
+            if (at == from) {  // the lanes' best are a list to begin with
+#pragma unroll
+                for (int g = 0; g < kLpWords; g++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const uint64_t c = lp_key(y[g][j], first + 4 * kLpThreads * g + j);
+                        own = c > own ? c : own;
+                    }
+                list = lp_sort(own);
+                least = unorder32((uint32_t)(lane64(list, a.k - 1) >> 32));
+            }
+            const uint32_t known = *(volatile uint32_t *)&floor_;
+            if (known) least = fmaxf(least, unorder32(known));
+            if (__any(top >= least)) {
+                uint64_t last = lane64(list, a.k - 1);
+#pragma unroll
+                for (int g = 0; g < kLpWords; g++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const uint64_t c = lp_key(y[g][j], first + 4 * kLpThreads * g + j);
+                        uint64_t left = __ballot(y[g][j] >= least && c > last && c != own);
+                        while (left) {
+                            const uint64_t one = lane64(c, __ffsll((unsigned long long)left) - 1);
+                            left &= left - 1;
+                            if (one <= last) continue;
+                            const int place = __popcll(__ballot(list > one));
+                            const uint64_t up = __shfl_up((unsigned long long)list, 1);
+                            list = lane < place ? list : lane == place ? one : up;
+                            last = lane64(list, a.k - 1);
+                        }
+                    }
+                const uint32_t l = (uint32_t)(last >> 32);
+                least = fmaxf(least, unorder32(l));
+                if (lane == 0 && l > known) atomicMax(&floor_, l);
+            }
+        }
+    }
+    double m = s.m, S = s.S, T = s.T;
+    int before = s.before;
+    lp_join_lanes(m, S, T, before);
+    if (lane == 0) sums[wave] = {(float)m, (float)S, (float)T, before};
+    if (TOP) lists[wave][lane] = list;
+    __syncthreads();
+    if (wave != 0) return;
+    const LpSums p = sums[lane & (kLpWaves - 1)];
+    m = p.m;
+    S = lane < kLpWaves ? p.S : 0.0f;
+    T = lane < kLpWaves ? p.T : 0.0f;
+    before = lane < kLpWaves ? p.before : 0;
+    lp_join_lanes(m, S, T, before);
+    if (TOP)
+        for (int w = 1; w < kLpWaves; w++) list = lp_join(list, lists[w][lane]);
+    if (gridDim.x == 1) lp_finish(a, r, m, S, T, before, zt, t, list);
+    else {
+        const size_t at = (size_t)r * gridDim.x + part;
+        if (lane == 0) ((LpSums *)a.ws)[at] = {(float)m, (float)S, (float)T, before};
+        if (TOP && lane < a.k)
+            ((uint64_t *)((LpSums *)a.ws + (size_t)a.n_rows * gridDim.x))[at * a.k + lane] = list;
+    }
+}
+
+// Joins the parts (at most 64) of row blockIdx.x: wave w of 16 the lists of parts w, w + 16, ...
+template <bool TOP>
+__global__ void __launch_bounds__(TOP ? 1024 : 64) logprobs_join_kernel(LogprobsArgs a, int parts) {
+    __shared__ uint64_t lists[TOP ? 16 : 1][64];
+    const int r = blockIdx.x, lane = lane_id(), wave = threadIdx.x >> 6;
+    uint64_t list = 0;
+    if (TOP) {
+        const uint64_t *l = (const uint64_t *)((const LpSums *)a.ws + (size_t)a.n_rows * parts) + (size_t)r * parts * a.k;
+        for (int p = wave; p < parts; p += 16) {
+            const uint64_t one = lane < a.k ? l[(size_t)p * a.k + lane] : 0;
+            list = p == wave ? one : lp_join(list, one);
+        }
+        for (int half = 8; half > 0; half >>= 1) {
+            if (wave >= half) lists[wave][lane] = list;
+            __syncthreads();
+            if (wave < half && wave + half < parts) list = lp_join(list, lists[wave + half][lane]);
+        }
+    }
+    if (wave != 0) return;
+    const LpSums p = lane < parts ? ((const LpSums *)a.ws)[(size_t)r * parts + lane] : LpSums{-FLT_MAX, 0.0f, 0.0f, 0};
+    double m = p.m, S = p.S, T = p.T;
+    int before = p.before;
+    lp_join_lanes(m, S, T, before);
+    const int t = a.targets ? a.targets[r] : -1;
+    const float zt = (unsigned)t < (unsigned)a.vocab ? a.z[(size_t)r * a.vocab + t] : 0.0f;
+    lp_finish(a, r, m, S, T, before, zt, t, list);
+}
+
+// Parts of a row: enough for four workgroups a CU, each at least a step.
+static int lp_parts(int n_rows, int vocab, int *per_part) {
+    const long long steps = ((long long)vocab + kLpStep - 1) / kLpStep;
+    long long parts = steps < 64 ? steps : 64;
+    if (parts * n_rows > 1024) parts = 1024 / n_rows > 1 ? 1024 / n_rows : 1;
+    const long long per = (steps + parts - 1) / parts;
+    *per_part = (int)(per * kLpStep < vocab ? per * kLpStep : vocab);
+    return (int)((steps + per - 1) / per);
+}
+
+size_t logprobs_workspace_bytes(int n_rows, int vocab, int k) {
+    int per;
+    const int parts = lp_parts(n_rows, vocab, &per);
+    return parts == 1 ? 16 : (size_t)n_rows * parts * (sizeof(LpSums) + (size_t)k * 8);
+}
+
+int launch_logprobs(const LogprobsArgs &a, hipStream_t s) {
+    int per;
+    const int parts = lp_parts(a.n_rows, a.vocab, &per);
+    const dim3 grid(parts, a.n_rows), block(kLpThreads);
+    if (a.k) hipLaunchKernelGGL(logprobs_kernel<true>, grid, block, 0, s, a, per);
+    else hipLaunchKernelGGL(logprobs_kernel<false>, grid, block, 0, s, a, per);
+    if (int rc = check_launch("logprobs")) return rc;
+    if (parts == 1) return kOk;
+    if (a.k) hipLaunchKernelGGL(logprobs_join_kernel<true>, dim3(a.n_rows), dim3(1024), 0, s, a, parts);
+    else hipLaunchKernelGGL(logprobs_join_kernel<false>, dim3(a.n_rows), dim3(64), 0, s, a, parts);
+    return check_launch("logprobs");
+}
+
+}  // namespace mnemo

@@ -247,6 +247,49 @@ struct LogitsArgs {
 };
 int launch_logits_process(const LogitsArgs &a, hipStream_t s);
 
+// ---- batches that hold prompts (route.hip, lora.hip, logprobs.hip)
+struct RouteArgs {
+    const float *z;  // [n_tokens][n_experts]
+    int n_tokens, n_experts;
+    int sigmoid;        // else softmax
+    const float *bias;  // [n_experts], or NULL
+    int n_groups, top_groups, best;
+    int k, renorm;
+    float scale;
+    int *idx;  // [n_tokens][k]
+    float *w;
+    // filled by launch_route: experts of a group, log2 of the lanes that hold them, experts per lane, 16-byte loads
+    int per_group, lanes_log, per_lane, vec;
+};
+int launch_route(RouteArgs a, hipStream_t s);
+
+struct LoraArgs {
+    const float *x, *base;  // [n_tokens][K], [n_tokens][M]
+    float *out;
+    const void *a, *b;  // [n_adapters][max_rank][K], [n_adapters][M][max_rank]
+    int bf16;           // else f16
+    const int *ids, *ranks;
+    const float *scales;
+    int n_tokens, K, M, n_adapters, max_rank;
+    float *ws;
+};
+size_t lora_workspace_bytes(int n_tokens, int K, int max_rank);
+int launch_lora(const LoraArgs &a, hipStream_t s);
+
+struct LogprobsArgs {
+    const float *z;  // [n_rows][vocab]
+    const int *targets;
+    int n_rows, vocab, k;
+    float *logp;
+    int *rank;
+    float *entropy;
+    int *ids;  // [n_rows][k]
+    float *tops;
+    void *ws;
+};
+size_t logprobs_workspace_bytes(int n_rows, int vocab, int k);
+int launch_logprobs(const LogprobsArgs &a, hipStream_t s);
+
 // Records (and prints, as the reference's KERNEL_LAUNCH_CHECK does, kernels.cu:1062-1067)
 // the error of the last launch; returns a kErr code.
 int check_launch(const char *what);

@@ -6,6 +6,7 @@
 #include <limits.h>
 #include <math.h>
 
+#include "mfma_types.hpp"
 #include "mnemo_common.hpp"
 #include "mnemo_internal.hpp"
 
@@ -40,12 +41,6 @@ namespace mnemo {
 // the value's scale, relative to a power of two (wref) that follows the largest such product in the
 // same way, not the largest scale: a large scale of no weight leaves the others their bits.  The
 // reference of P is a whole power there, so that O and its unit are rescaled without rounding.
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef float f4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-
 constexpr int kPaRows = 16;
 constexpr float kSlack = 5.0f, kLift = 9.0f;  // powers of two: P <= 2^14 (int8: 2^5, P times scale below 2^15 wref)
 
@@ -159,18 +154,6 @@ __device__ __forceinline__ float sum_heads(float v) {
 // 1 / v of a power of two from 2^-126 to 2^126
 __device__ __forceinline__ float inverse2(float v) {
     return __builtin_bit_cast(float, 0x7f000000u - __builtin_bit_cast(uint32_t, v));
-}
-
-// 8 int8 as f16: 0x64uu is 1024 + uu, so with the sign bit flipped and 1152 taken off it is the number.
-__device__ __forceinline__ h4 cvt4(uint32_t w) {
-    const uint32_t u = w ^ 0x80808080u;
-    const uint32_t lo = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u), hi = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
-    const h2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
-    const h2 a = __builtin_bit_cast(h2, lo) - off, b = __builtin_bit_cast(h2, hi) - off;
-    return __builtin_shufflevector(a, b, 0, 1, 2, 3);
-}
-__device__ __forceinline__ h8 cvt8(uint32_t a, uint32_t b) {
-    return __builtin_shufflevector(cvt4(a), cvt4(b), 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 template <int KV, int HD, int STEP>

@@ -93,6 +93,12 @@ SIGNATURES: dict[str, tuple] = {
                                      stream_t]),
     "mnemo_kv_pages_copy": (i32, [ip, ip, i32, vp, vp, fp, fp, i32, i32, i32, i32, i32, i32, stream_t]),
     "mnemo_logits_process": (i32, [fp, fp, i32, i32, ip, ip, ip, i32, fp, fp, fp, ip, fp, i32, vp, stream_t]),
+    # batches that hold prompts
+    "mnemo_moe_route": (i32, [fp, i32, i32, i32, fp, i32, i32, i32, i32, i32, f32, ip, fp, stream_t]),
+    "mnemo_lora_workspace_bytes": (sz, [i32, i32, i32]),
+    "mnemo_lora_add": (i32, [fp, vp, vp, i32, ip, ip, fp, fp, fp, i32, i32, i32, i32, i32, vp, sz, stream_t]),
+    "mnemo_logprobs_workspace_bytes": (sz, [i32, i32, i32]),
+    "mnemo_logprobs": (i32, [fp, ip, i32, i32, fp, ip, fp, i32, ip, fp, vp, sz, stream_t]),
     # model directory (mnemo_model.h); structs travel as void*
     "mnemo_parse_config": (i32, [C.c_char_p, vp]),
     "mnemo_parse_resident_manifest": (i32, [C.c_char_p, vp, i32, vp]),

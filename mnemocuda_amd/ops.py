@@ -682,3 +682,66 @@ def logits_process(logits, out, history=None, history_lens=None, prompt_lens=Non
         _arg(logits, "logits", F32), _arg(out, "out", F32), n, vocab, *h, *b,
         _opt_arg(allowed, "allowed", I32, n * ((vocab + 31) // 32)), _stream())
     _check_rc(lib, rc, "mnemo_logits_process")
+
+
+# ---------------------------------------------------------------- batches that hold prompts
+def moe_route(logits, topk_idx, topk_w, sigmoid: bool = False, bias=None, n_groups: int = 1, top_groups: int = 1,
+              group_best: int = 1, renormalise: bool = True, scale: float = 1.0):
+    """topk_idx, topk_w [T, k]: the experts of each row of logits [T, n_experts] and their weights, best first, as
+    moe_prefill takes them.  Softmax or sigmoid scores; the choice goes by score + bias [n_experts], among the experts
+    of the top_groups groups with the largest sum of their group_best best."""
+    lib = load_library()
+    shape, to = logits.shape, topk_idx.shape
+    if len(shape) != 2 or len(to) != 2 or to[0] != shape[0] or topk_w.shape != to:
+        raise MnemoError("moe_route: logits must be [T, n_experts], topk_idx and topk_w [T, k]")
+    rc = lib.mnemo_moe_route(_arg(logits, "logits", F32), shape[0], shape[1], int(sigmoid),
+                             _opt_arg(bias, "bias", F32, shape[1]), int(n_groups), int(top_groups), int(group_best), to[1],
+                             int(renormalise), float(scale), _arg(topk_idx, "topk_idx", I32), _arg(topk_w, "topk_w", F32),
+                             _stream())
+    _check_rc(lib, rc, "mnemo_moe_route")
+
+
+def lora_workspace_bytes(n_tokens: int, n_in: int, max_rank: int) -> int:
+    return int(load_library().mnemo_lora_workspace_bytes(n_tokens, n_in, max_rank))
+
+
+def lora_add(x, a_w, b_w, adapter_ids, ranks, scales, base, out, ws):
+    """out[t] = base[t] + scales[a] * B_a (A_a x[t]) with a = adapter_ids[t] (none outside the table): x [T, n_in], base
+    and out [T, n_out] (out may be base), a_w [n_adapters, max_rank, n_in] and b_w [n_adapters, n_out, max_rank] float16 or
+    bfloat16, of which the first ranks[a] ranks count."""
+    lib = load_library()
+    if x.dim() != 2 or a_w.dim() != 3 or b_w.dim() != 3 or base.dim() != 2 or out.shape != base.shape:
+        raise MnemoError("lora_add: x, base and out must have 2 dimensions, a_w and b_w 3")
+    (T, K), (N, R, _), M = x.shape, a_w.shape, base.shape[1]
+    if a_w.shape[2] != K or b_w.shape != (N, M, R) or base.shape[0] != T:
+        raise MnemoError("lora_add: a_w must be [n_adapters, max_rank, n_in], b_w [n_adapters, n_out, max_rank], x [T, n_in], "
+                         "base and out [T, n_out]")
+    if a_w.dtype is not torch.float16 and a_w.dtype is not torch.bfloat16:
+        raise MnemoError(f"adapters must be float16 or bfloat16, got {a_w.dtype}")
+    rc = lib.mnemo_lora_add(_arg(x, "x", F32), _arg(a_w, "a_w"), _arg(b_w, "b_w", a_w.dtype),
+                            int(a_w.dtype is torch.bfloat16), _arg(adapter_ids, "adapter_ids", I32, T),
+                            _arg(ranks, "ranks", I32, N), _arg(scales, "scales", F32, N), _arg(base, "base", F32),
+                            _arg(out, "out", F32), T, K, M, N, R, _arg(ws, "ws"), ws.numel() * ws.element_size(), _stream())
+    _check_rc(lib, rc, "mnemo_lora_add")
+
+
+def logprobs_workspace_bytes(n_rows: int, vocab: int, n_top: int) -> int:
+    return int(load_library().mnemo_logprobs_workspace_bytes(n_rows, vocab, n_top))
+
+
+def logprobs(logits, targets, logprob, rank, entropy, top_ids, top_logprobs, ws):
+    """Of each row of logits [n, vocab]: the log probability and rank of targets[n], the entropy, and the ids and log
+    probabilities [n, n_top] of the likeliest tokens.  Any of the three may be left out (targets with logprob and rank,
+    entropy, top_ids with top_logprobs: None)."""
+    lib = load_library()
+    if logits.dim() != 2 or (top_ids is not None and (top_logprobs is None or top_ids.dim() != 2 or
+                                                      top_ids.shape[0] != logits.shape[0] or
+                                                      top_logprobs.shape != top_ids.shape)):
+        raise MnemoError("logprobs: logits must be [n, vocab], top_ids and top_logprobs [n, n_top]")
+    n, vocab = logits.shape
+    rc = lib.mnemo_logprobs(_arg(logits, "logits", F32), _opt_arg(targets, "targets", I32, n), n, vocab,
+                            _opt_arg(logprob, "logprob", F32, n), _opt_arg(rank, "rank", I32, n),
+                            _opt_arg(entropy, "entropy", F32, n), 0 if top_ids is None else top_ids.shape[1],
+                            _opt_arg(top_ids, "top_ids", I32), _opt_arg(top_logprobs, "top_logprobs", F32),
+                            _arg(ws, "ws"), ws.numel() * ws.element_size(), _stream())
+    _check_rc(lib, rc, "mnemo_logprobs")

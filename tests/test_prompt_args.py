@@ -1,0 +1,94 @@
+"""Refusals of the entry points for batches that hold prompts: every call below is rejected on the host, before any
+launch (no GPU)."""
+import pytest
+
+from mnemocuda_amd import lib as mlib
+
+A = 4096  # a non-null, aligned address that no call below reaches
+
+
+@pytest.fixture(scope="module")
+def L():
+    return mlib.load_library()
+
+
+def refused(L, rc, what, capfd):
+    assert rc == 1
+    assert what in capfd.readouterr().err
+    assert L.mnemo_last_error() == 1
+
+
+def route(L, *, z=A, T=4, E=64, score=0, bias=A, groups=4, top=2, best=2, k=6, idx=A, w=A):
+    return L.mnemo_moe_route(z, T, E, score, bias, groups, top, best, k, 1, 1.0, idx, w, None)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(z=None), dict(idx=None), dict(w=None), dict(T=-1), dict(T=4194304, k=2), dict(E=0), dict(E=1025, groups=1, top=1), dict(E=4, k=6),
+    dict(k=0), dict(k=17), dict(groups=0), dict(groups=3), dict(groups=128, E=128), dict(top=0), dict(top=5), dict(best=0),
+    dict(best=3), dict(score=2), dict(score=-1)])
+def test_route_refuses(L, bad, capfd):
+    refused(L, route(L, **bad), "moe_route", capfd)
+
+
+def lora(L, *, x=A, a=A, b=A, typ=0, ids=A, ranks=A, scales=A, base=A, out=A, T=4, K=64, M=32, N=2, R=16, ws=A, wsb=1 << 30):
+    return L.mnemo_lora_add(x, a, b, typ, ids, ranks, scales, base, out, T, K, M, N, R, ws, wsb, None)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(x=None), dict(a=None), dict(b=None), dict(ids=None), dict(ranks=None), dict(scales=None), dict(base=None),
+    dict(out=None), dict(ws=None), dict(ws=A + 4), dict(wsb=16), dict(a=A + 8), dict(b=A + 2), dict(typ=2), dict(typ=-1),
+    dict(T=-1), dict(T=524289), dict(K=0), dict(K=60), dict(K=(1 << 20) + 8), dict(M=0), dict(M=(1 << 24) + 1), dict(N=0),
+    dict(N=65537), dict(R=0), dict(R=12), dict(R=264)])
+def test_lora_refuses(L, bad, capfd):
+    refused(L, lora(L, **bad), "lora_add", capfd)
+
+
+def logprobs(L, *, z=A, t=A, n=2, V=100, lp=A, rank=A, ent=A, k=4, ids=A, tops=A, ws=A, wsb=1 << 30):
+    return L.mnemo_logprobs(z, t, n, V, lp, rank, ent, k, ids, tops, ws, wsb, None)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(z=None), dict(lp=None), dict(ids=None), dict(tops=None), dict(n=-1), dict(n=65536), dict(V=0), dict(V=(1 << 30) + 1),
+    dict(k=-1), dict(k=65), dict(ws=None), dict(ws=A + 8), dict(V=100000, wsb=16)])
+def test_logprobs_refuses(L, bad, capfd):
+    refused(L, logprobs(L, **bad), "logprobs", capfd)
+
+
+def test_nothing_of_no_rows(L):
+    assert route(L, T=0, z=None, idx=None, w=None) == 0
+    assert lora(L, T=0, x=None, out=None, ws=None) == 0
+    assert logprobs(L, n=0, z=None, ws=None) == 0
+
+
+def test_workspaces(L):
+    assert L.mnemo_lora_workspace_bytes(100, 4096, 16) == 4 * 100 * 16 * 4
+    assert L.mnemo_lora_workspace_bytes(524288, 1 << 20, 256) == 8 * 524288 * 256 * 4  # past 32 bits
+    assert L.mnemo_lora_workspace_bytes(10, 60, 16) == L.mnemo_lora_workspace_bytes(10, 64, 260) == 0
+    assert L.mnemo_logprobs_workspace_bytes(1, 151936, 20) > 0
+    assert L.mnemo_logprobs_workspace_bytes(0, 100, 4) == L.mnemo_logprobs_workspace_bytes(1, 100, 65) == 0
+
+
+def test_wrappers_refuse_host_tensors_and_shapes(L):
+    """The Python wrappers check tensors before anything is launched (CPU tensors reach no kernel)."""
+    import torch
+
+    from mnemocuda_amd import MnemoError, ops
+    z = lambda *s, t=torch.float32: torch.zeros(s, dtype=t)  # noqa: E731
+    i = lambda *s: z(*s, t=torch.int32)  # noqa: E731
+    h = lambda *s: z(*s, t=torch.float16)  # noqa: E731
+    with pytest.raises(MnemoError, match="moe_route: logits must be"):
+        ops.moe_route(z(4, 8), i(3, 2), z(3, 2))
+    with pytest.raises(MnemoError, match="GPU tensor"):
+        ops.moe_route(z(4, 8), i(4, 2), z(4, 2))
+    with pytest.raises(MnemoError, match="a_w must be"):
+        ops.lora_add(z(4, 64), h(2, 8, 64), h(2, 8, 32), i(4), i(2), z(2), z(4, 32), z(4, 32), z(64))
+    with pytest.raises(MnemoError, match="2 dimensions"):
+        ops.lora_add(z(4, 64), h(2, 8, 64), h(2, 32, 8), i(4), i(2), z(2), z(4, 32), z(4, 33), z(64))
+    with pytest.raises(MnemoError, match="float16 or bfloat16"):
+        ops.lora_add(z(4, 64), z(2, 8, 64), z(2, 32, 8), i(4), i(2), z(2), z(4, 32), z(4, 32), z(64))
+    with pytest.raises(MnemoError, match="GPU tensor"):
+        ops.lora_add(z(4, 64), h(2, 8, 64), h(2, 32, 8), i(4), i(2), z(2), z(4, 32), z(4, 32), z(64))
+    with pytest.raises(MnemoError, match="logprobs: logits must be"):
+        ops.logprobs(z(4, 64), i(4), z(4), i(4), z(4), i(4, 3), z(4, 2), z(64))
+    with pytest.raises(MnemoError, match="GPU tensor"):
+        ops.logprobs(z(4, 64), i(4), z(4), i(4), z(4), None, None, z(64))
