@@ -465,7 +465,28 @@ int mnemo_logits_process(const float *logits, float *out, int n_rows, int vocab,
 /* ---- Prompts of several requests (no reference counterpart: it takes a prompt token by token,
  * src/forward.c:1783-1830) ------------------------------------------------------------------
  *
- * Routing of n_tokens tokens from their router logits [n_tokens][n_experts], for mnemo_moe_prefill:
+ * Attention of several new tokens per sequence over the paged cache, which holds them already
+ * (mnemo_paged_attn_prep): prompts, chunks of prompts, drafted tokens, single ones, in one call.
+ * Sequence s has the rows starts[s] .. starts[s+1]-1 of q and out [n_tokens][n_heads][head_dim]
+ * (starts [n_seqs + 1], rising, in device memory), n of them, of which token i is position
+ * p = seq_lens[s] - n + i:
+ *   out[i][h] = softmax_j(scale q[i][h] . k_j) v_j over the positions j <= p
+ * A token before position 0 gets zeros; rows of no sequence are left as they are; the positions of a
+ * page id outside 0..n_pages-1 are absent.  What a token does not see does not reach it, whatever it
+ * holds.  n_heads = gqa * n_kv_heads with gqa <= 16; sizes as for mnemo_paged_attention_decode;
+ * n_tokens <= 4,194,304, and (n_tokens * gqa / 32 + n_seqs) * n_kv_heads * max_pages * page_size < 2^36.
+ * out must not overlap q.  workspace: mnemo_paged_attention_prompt_workspace_bytes(...) bytes (68 MB at
+ * most), 16-byte aligned, no initialisation; calls sharing it must not overlap. */
+size_t mnemo_paged_attention_prompt_workspace_bytes(int n_heads, int n_kv_heads, int head_dim);
+int mnemo_paged_attention_prompt(const float *q, const void *k_pages, const void *v_pages,
+                                 const float *k_scales, const float *v_scales, int kv_type,
+                                 float *out, int n_tokens, int n_heads, int head_dim,
+                                 int n_kv_heads, int n_pages, int page_size, const int *block_table,
+                                 int n_seqs, int max_pages, const int *starts, const int *seq_lens,
+                                 float scale, void *workspace, size_t workspace_bytes,
+                                 hipStream_t stream);
+
+/* Routing of n_tokens tokens from their router logits [n_tokens][n_experts], for mnemo_moe_prefill:
  *   s_e = 1 / (1 + exp(-z_e)) (score 1) or exp(z_e) / sum_f exp(z_f) (score 0);  c_e = s_e + bias[e]
  *   The experts are n_groups runs of n_experts / n_groups.  A group scores the sum of its group_best
  *   (1 or 2) largest c; the top_groups best groups are kept (ties to the lower index).

@@ -23,7 +23,7 @@ GRAPH_CALLER = PKG / "attn_graph"  # tests/c_caller/attn_graph.c, linked against
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 
 HIP_SOURCES = ["abi.hip", "gemv_launch.hip", "router.hip", "gemm.hip", "gemm_grouped.hip", "moe.hip", "sample.hip", "attn.hip", "attn_decode.hip", "embed.hip",
-               "paged_attn.hip", "kv_pages.hip", "logits.hip", "route.hip", "lora.hip", "logprobs.hip"]
+               "paged_attn.hip", "paged_prompt.hip", "kv_pages.hip", "logits.hip", "route.hip", "lora.hip", "logprobs.hip"]
 C_SOURCES = ["host/mnemo_host.c", "host/mnemo_model.c"]
 
 HIPCC_FLAGS = [

@@ -806,6 +806,55 @@ int mnemo_logits_process(const float *logits, float *out, int n_rows, int vocab,
 }
 
 // ------------------------------------------------------------------ batches that hold prompts
+size_t mnemo_paged_attention_prompt_workspace_bytes(int n_heads, int n_kv_heads, int head_dim) {
+    return n_heads > 0 && n_kv_heads > 0 && (head_dim == 64 || head_dim == 128 || head_dim == 256)
+               ? paged_prompt_workspace_bytes(head_dim)
+               : 0;
+}
+
+int mnemo_paged_attention_prompt(const float *q, const void *k_pages, const void *v_pages, const float *k_scales,
+                                 const float *v_scales, int kv_type, float *out, int n_tokens, int n_heads, int head_dim,
+                                 int n_kv_heads, int n_pages, int page_size, const int *block_table, int n_seqs,
+                                 int max_pages, const int *starts, const int *seq_lens, float scale, void *workspace,
+                                 size_t workspace_bytes, hipStream_t s) {
+    const char *what = "paged_attention_prompt";
+    PagedPromptArgs a = {};
+    a.c = {(void *)k_pages, (void *)v_pages, (float *)k_scales, (float *)v_scales, kv_type, n_pages, page_size,
+           n_kv_heads, head_dim};
+    if (int rc = check_cache(what, a.c)) return rc;
+    if (n_heads <= 0 || n_heads % n_kv_heads || n_heads / n_kv_heads > 16)
+        return set_error(kErrBadArg, "%s: n_heads must be 1 to 16 times n_kv_heads", what);
+    if (n_seqs <= 0 || n_seqs > kMaxSeqs || max_pages <= 0 || (long long)max_pages * page_size > 1 << 30 ||
+        (long long)n_seqs * max_pages > 1 << 30)
+        return set_error(kErrBadArg, "%s: need 1 <= n_seqs <= %d, 1 <= max_pages * page_size <= 2^30 and n_seqs * max_pages <= 2^30",
+                         what, kMaxSeqs);
+    if (n_tokens < 0 || n_tokens > 1 << 22) return set_error(kErrBadArg, "%s: n_tokens must be in 0..%d", what, 1 << 22);
+    const int gqa = n_heads / n_kv_heads;
+    // the steps are counted in an int; a tile has more than 32 / gqa tokens, but for each sequence's last
+    if ((__int128)((long long)n_tokens * gqa / 32 + n_seqs) * n_kv_heads * max_pages * page_size >= (__int128)1 << 36)
+        return set_error(kErrBadArg, "%s: (n_tokens * gqa / 32 + n_seqs) * n_kv_heads * max_pages * page_size must be below 2^36",
+                         what);
+    if (n_tokens == 0) return kOk;
+    if (!q || !out || !block_table || !starts || !seq_lens || !workspace)
+        return set_error(kErrBadArg, "%s: NULL pointer", what);
+    const size_t need = paged_prompt_workspace_bytes(head_dim);
+    if ((uintptr_t)workspace % 16 || workspace_bytes < need)
+        return set_error(kErrBadArg, "%s: workspace not 16-byte aligned, or %zu < %zu bytes", what, workspace_bytes, need);
+    a.q = q;
+    a.out = out;
+    a.table = block_table;
+    a.starts = starts;
+    a.lens = seq_lens;
+    a.n_tokens = n_tokens;
+    a.n_seqs = n_seqs;
+    a.max_pages = max_pages;
+    a.nh = n_heads;
+    a.gqa = gqa;
+    a.scale = scale;
+    a.ws = (float *)workspace;
+    return launch_paged_prompt(a, s);
+}
+
 int mnemo_moe_route(const float *logits, int n_tokens, int n_experts, int score, const float *bias, int n_groups,
                     int top_groups, int group_best, int k, int renormalise, float scale, int *topk_idx, float *topk_w,
                     hipStream_t s) {

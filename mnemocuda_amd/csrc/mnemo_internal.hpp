@@ -247,7 +247,21 @@ struct LogitsArgs {
 };
 int launch_logits_process(const LogitsArgs &a, hipStream_t s);
 
-// ---- batches that hold prompts (route.hip, lora.hip, logprobs.hip)
+// ---- batches that hold prompts (paged_prompt.hip, route.hip, lora.hip, logprobs.hip)
+struct PagedPromptArgs {
+    const float *q;
+    float *out;
+    PagedCache c;
+    const int *table, *starts, *lens;  // starts [n_seqs + 1]: first row of q of each sequence
+    int n_tokens, n_seqs, max_pages, nh, gqa;
+    float scale;
+    float *ws;
+    int tl;  // log2 of the tokens of a tile (launch_paged_prompt)
+};
+size_t paged_prompt_workspace_bytes(int hd);
+int paged_prompt_tile_log(int hd, int gqa);
+int launch_paged_prompt(PagedPromptArgs a, hipStream_t s);
+
 struct RouteArgs {
     const float *z;  // [n_tokens][n_experts]
     int n_tokens, n_experts;

@@ -94,6 +94,9 @@ SIGNATURES: dict[str, tuple] = {
     "mnemo_kv_pages_copy": (i32, [ip, ip, i32, vp, vp, fp, fp, i32, i32, i32, i32, i32, i32, stream_t]),
     "mnemo_logits_process": (i32, [fp, fp, i32, i32, ip, ip, ip, i32, fp, fp, fp, ip, fp, i32, vp, stream_t]),
     # batches that hold prompts
+    "mnemo_paged_attention_prompt_workspace_bytes": (sz, [i32, i32, i32]),
+    "mnemo_paged_attention_prompt": (i32, [fp, vp, vp, fp, fp, i32, fp, i32, i32, i32, i32, i32, i32, ip, i32, i32, ip,
+                                           ip, f32, vp, sz, stream_t]),
     "mnemo_moe_route": (i32, [fp, i32, i32, i32, fp, i32, i32, i32, i32, i32, f32, ip, fp, stream_t]),
     "mnemo_lora_workspace_bytes": (sz, [i32, i32, i32]),
     "mnemo_lora_add": (i32, [fp, vp, vp, i32, ip, ip, fp, fp, fp, i32, i32, i32, i32, i32, vp, sz, stream_t]),

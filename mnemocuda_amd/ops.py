@@ -685,6 +685,26 @@ def logits_process(logits, out, history=None, history_lens=None, prompt_lens=Non
 
 
 # ---------------------------------------------------------------- batches that hold prompts
+def paged_attention_prompt_workspace_bytes(n_heads: int, n_kv_heads: int, head_dim: int) -> int:
+    return int(load_library().mnemo_paged_attention_prompt_workspace_bytes(n_heads, n_kv_heads, head_dim))
+
+
+def paged_attention_prompt(q, k_pages, v_pages, block_table, starts, seq_lens, out, scale: float, ws, ks=None, vs=None):
+    """Causal attention of the rows starts[s] .. starts[s+1]-1 of q [T, n_heads, head_dim], the last new tokens of
+    sequence s (the cache holds them already: the last of them is position seq_lens[s] - 1), into out."""
+    lib = load_library()
+    ptrs, (_, n_pages, nkv, ps, hd) = _pages(k_pages, v_pages, ks, vs, False)
+    table, n_seqs, max_pages = _rows(block_table)
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != hd or out.shape != shape:
+        raise MnemoError("paged_attention_prompt: q and out must be [T, n_heads, head_dim]")
+    rc = lib.mnemo_paged_attention_prompt(
+        _arg(q, "q", F32), *ptrs, _arg(out, "out", F32), shape[0], shape[1], hd, nkv, n_pages, ps, table, n_seqs, max_pages,
+        _arg(starts, "starts", I32, n_seqs + 1), _arg(seq_lens, "seq_lens", I32, n_seqs), float(scale), _arg(ws, "ws"),
+        ws.numel() * ws.element_size(), _stream())
+    _check_rc(lib, rc, "mnemo_paged_attention_prompt")
+
+
 def moe_route(logits, topk_idx, topk_w, sigmoid: bool = False, bias=None, n_groups: int = 1, top_groups: int = 1,
               group_best: int = 1, renormalise: bool = True, scale: float = 1.0):
     """topk_idx, topk_w [T, k]: the experts of each row of logits [T, n_experts] and their weights, best first, as

@@ -18,6 +18,22 @@ def refused(L, rc, what, capfd):
     assert L.mnemo_last_error() == 1
 
 
+def prompt(L, *, q=A, kp=A, vp=A, ks=None, vs=None, kv_type=0, out=A, T=20, nh=8, hd=128, nkv=2, n_pages=8, ps=64, table=A, n_seqs=4,
+           max_pages=4, starts=A, lens=A, ws=A, wsb=1 << 30):
+    return L.mnemo_paged_attention_prompt(q, kp, vp, ks, vs, kv_type, out, T, nh, hd, nkv, n_pages, ps, table, n_seqs, max_pages,
+                                          starts, lens, 0.1, ws, wsb, None)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(kp=None), dict(vp=None), dict(kp=A + 8), dict(kv_type=2), dict(kv_type=1), dict(kv_type=1, ks=A, vs=A + 4), dict(hd=96),
+    dict(ps=48), dict(nkv=0), dict(n_pages=0), dict(n_pages=(1 << 30) + 1), dict(q=None), dict(out=None), dict(table=None),
+    dict(starts=None), dict(lens=None), dict(ws=None), dict(ws=A + 4), dict(wsb=8), dict(wsb=1 << 20), dict(nh=7), dict(nh=34),
+    dict(nh=0), dict(n_seqs=0), dict(n_seqs=4097), dict(max_pages=0), dict(max_pages=1 << 25), dict(T=-1), dict(T=(1 << 22) + 1),
+    dict(n_seqs=4096, max_pages=1 << 19, ps=16), dict(T=1 << 22, max_pages=1 << 14, nh=32), dict(T=1 << 20, max_pages=1 << 20)])
+def test_prompt_attention_refuses(L, bad, capfd):
+    refused(L, prompt(L, **bad), "paged_attention_prompt", capfd)
+
+
 def route(L, *, z=A, T=4, E=64, score=0, bias=A, groups=4, top=2, best=2, k=6, idx=A, w=A):
     return L.mnemo_moe_route(z, T, E, score, bias, groups, top, best, k, 1, 1.0, idx, w, None)
 
@@ -55,6 +71,7 @@ def test_logprobs_refuses(L, bad, capfd):
 
 
 def test_nothing_of_no_rows(L):
+    assert prompt(L, T=0, q=None, out=None, ws=None) == 0
     assert route(L, T=0, z=None, idx=None, w=None) == 0
     assert lora(L, T=0, x=None, out=None, ws=None) == 0
     assert logprobs(L, n=0, z=None, ws=None) == 0
@@ -76,6 +93,11 @@ def test_wrappers_refuse_host_tensors_and_shapes(L):
     z = lambda *s, t=torch.float32: torch.zeros(s, dtype=t)  # noqa: E731
     i = lambda *s: z(*s, t=torch.int32)  # noqa: E731
     h = lambda *s: z(*s, t=torch.float16)  # noqa: E731
+    k, v = h(8, 2, 16, 64), h(8, 2, 64, 16)
+    with pytest.raises(MnemoError, match="do not fit"):  # v laid out as k is
+        ops.paged_attention_prompt(z(5, 4, 64), k, h(8, 2, 16, 64), i(2, 3), i(3), i(2), z(5, 4, 64), 0.1, z(64))
+    with pytest.raises(MnemoError, match="GPU tensor"):
+        ops.paged_attention_prompt(z(5, 4, 64), k, v, i(2, 3), i(3), i(2), z(5, 4, 64), 0.1, z(64))
     with pytest.raises(MnemoError, match="moe_route: logits must be"):
         ops.moe_route(z(4, 8), i(3, 2), z(3, 2))
     with pytest.raises(MnemoError, match="GPU tensor"):
