@@ -259,7 +259,6 @@ struct PagedPromptArgs {
     int tl;  // log2 of the tokens of a tile (launch_paged_prompt)
 };
 size_t paged_prompt_workspace_bytes(int hd);
-int paged_prompt_tile_log(int hd, int gqa);
 int launch_paged_prompt(PagedPromptArgs a, hipStream_t s);
 
 struct RouteArgs {

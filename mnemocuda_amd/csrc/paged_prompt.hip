@@ -22,6 +22,9 @@
 #include <limits.h>
 #include <math.h>
 
+#include <float.h>
+
+#include "gemm_ops.hpp"
 #include "mfma_types.hpp"
 #include "mnemo_common.hpp"
 #include "mnemo_internal.hpp"
@@ -32,29 +35,29 @@ namespace {
 
 constexpr float kSlack = 5.0f, kLift = 9.0f;  // powers of two
 constexpr int kStep = 64;                     // positions
-constexpr int kWaves = 4, kThreads = 64 * kWaves;
-constexpr int kGroups = 512;                  // workgroups, two per CU
 
+// 128 rows, by 4 waves of 32 or, at head_dim 256, 8 of 16: two waves per SIMD either way.
+constexpr int kRows = 128;
 template <int HD>
 struct Shape {
     static constexpr int RT = HD == 256 ? 1 : 2;  // tiles of 16 rows per wave
-    static constexpr int kRows = 16 * RT * kWaves;
+    static constexpr int kThreads = 64 * kRows / (16 * RT);
     static constexpr int kKs = HD / 32, kNd = HD / 16;  // dim steps of S, dim tiles of O
 };
+__host__ __device__ constexpr int groups_of(int hd) { return hd == 256 ? 256 : 512; }  // workgroups that fill the chip
 
 // Workspace: two partials per workgroup (max [rows], sum [rows], O [rows][hd]), and what they are: begun[g] describes the
 // tile that begins in workgroup g's share and goes on behind it (its second partial), taken[g] is the first step of the
 // tile that it goes on with from the workgroup before (its first), -1 for none.
-__host__ __device__ constexpr int rows_of(int hd) { return hd == 256 ? 64 : 128; }
-__host__ __device__ constexpr int part_floats(int hd) { return rows_of(hd) * (hd + 2); }
+__host__ __device__ constexpr int part_floats(int hd) { return kRows * (hd + 2); }
 struct Begun {
     int first;  // first step, -1 for none
     int row0, n_rows, kvh;  // first token (row of q), rows in use, KV head
 };
 __device__ __forceinline__ Begun *begun_of(const PagedPromptArgs &a) {
-    return (Begun *)(a.ws + (size_t)2 * kGroups * part_floats(a.c.hd));
+    return (Begun *)(a.ws + (size_t)2 * groups_of(a.c.hd) * part_floats(a.c.hd));
 }
-__device__ __forceinline__ int *taken_of(const PagedPromptArgs &a) { return (int *)(begun_of(a) + kGroups); }
+__device__ __forceinline__ int *taken_of(const PagedPromptArgs &a) { return (int *)(begun_of(a) + groups_of(a.c.hd)); }
 
 // ------------------------------------------------------------------ the row of steps
 struct Seq {
@@ -102,7 +105,7 @@ struct Plan {
     int per;         // sequences per lane of the sums
     int before;      // lane: steps before its sequences
 };
-__device__ __forceinline__ Plan make_plan(const PagedPromptArgs &a) {
+__device__ __forceinline__ Plan make_plan(const PagedPromptArgs &a, int groups) {
     Plan p;
     p.per = (a.n_seqs + 63) / 64;
     p.short_ = false;
@@ -118,13 +121,18 @@ __device__ __forceinline__ Plan make_plan(const PagedPromptArgs &a) {
     const int incl = wave_scan(sum);
     p.total = __builtin_amdgcn_readlane(incl, 63);
     p.before = incl - sum;
-    p.groups = max(min(kGroups, p.total), 1);
+    p.groups = max(min(groups, p.total), 1);
     p.base = p.total / p.groups;
     p.more = p.total - p.base * p.groups;
     return p;
 }
 __device__ __forceinline__ int first_of(const Plan &p, int g) {
     return g >= p.groups ? p.total : g * p.base + min(g, p.more);
+}
+
+// of tile j: the positions that its last token sees
+__device__ __forceinline__ int tile_steps(const Seq &s, int tl, int j) {
+    return (s.len - s.n + min((j + 1) << tl, s.n) + kStep - 1) / kStep;
 }
 
 struct Where {
@@ -160,9 +168,21 @@ __device__ __forceinline__ Where find(const PagedPromptArgs &a, const Plan &p, i
     }
     w.tile = lo;
     w.step = at - steps_before(w.s, a.tl, lo);
-    const int end = w.s.len - w.s.n + min((lo + 1) << a.tl, w.s.n);  // positions that the tile's last token sees
-    w.steps = (end + kStep - 1) / kStep;
+    w.steps = tile_steps(w.s, a.tl, lo);
     return w;
+}
+// The tile after w, from its first step on (there is one).
+__device__ __forceinline__ void advance(const PagedPromptArgs &a, Where &w) {
+    if (++w.tile == tiles_of(w.s, a.tl)) {
+        if (++w.kvh == a.c.nkv) {
+            w.kvh = 0;
+            do w.s = seq_of(a, ++w.seq);
+            while (w.s.n == 0 || w.s.len == 0);
+        }
+        w.tile = max(w.s.n - w.s.len, 0) >> a.tl;  // the first one with a position
+    }
+    w.step = 0;
+    w.steps = tile_steps(w.s, a.tl, w.tile);
 }
 
 // max over the four lanes that share a row (lane % 16), in all of them
@@ -184,88 +204,173 @@ __device__ __forceinline__ int k_word(int p, int c) {
 }
 __device__ __forceinline__ int v_word(int d, int c) { return d * (kStep / 8) + (c ^ ((d >> 1) & 7)); }
 
-// 8 int8 as bf16, exact
-__device__ __forceinline__ u4 int8_bf16(uint32_t a, uint32_t b) {
-    u4 w;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t x = i < 2 ? a : b;
-        const float lo = (float)(int8_t)(x >> (16 * (i & 1))), hi = (float)(int8_t)(x >> (16 * (i & 1) + 8));
-        w[i] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo), 0x07060302u);
-    }
-    return w;
+// Steps that some row of a tile does not see all of hold its tokens' positions, 128 at most, and the rest of the
+// words that the first and the last of them lie in.
+constexpr int kOddWords = (kRows + 2 * kStep) / 32;
+
+// Two f16 parts of each of two values: together 22 bits or more.
+struct h2x2 {
+    h2 hi, lo;
+};
+__device__ __forceinline__ h2x2 two_parts(float a, float b) {
+    asm("" : "+v"(a), "+v"(b));  // one value for both parts: a product folded into a conversion would round differently
+    h2x2 x;
+    x.hi = h2{(_Float16)a, (_Float16)b};
+    x.lo = h2{(_Float16)fmaf((float)x.hi[0], -1.0f, a), (_Float16)fmaf((float)x.hi[1], -1.0f, b)};
+    return x;
 }
 
 template <int KV, int HD>
-__global__ void __launch_bounds__(kThreads, 2) paged_prompt_kernel(PagedPromptArgs a) {
+__global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(PagedPromptArgs a) {
     using S = Shape<HD>;
-    constexpr int RT = S::RT, KS = S::kKs, ND = S::kNd;
+    constexpr int RT = S::RT, KS = S::kKs, ND = S::kNd, kThreads = S::kThreads, kGroups = groups_of(HD);
     constexpr int EB = KV == kKvF16 ? 2 : 1;
-    constexpr int NL = kStep * HD * EB / 16 / kThreads;  // 16-byte loads per thread of K, and of V
-    __shared__ u4 kt[kStep * HD / 8], vt[kStep * HD / 8];
-    __shared__ __align__(16) float ksc[KV == kKvInt8 ? kStep : 4], vsc[KV == kKvInt8 ? kStep : 4];
-    __shared__ uint32_t odd[2][2];  // by the step's parity: positions with values that are none
+    constexpr bool kEarly = KV == kKvF16 || HD == 64;  // V's operands wait in registers for the weights
+    constexpr int kWords = kStep * HD / 8;  // 16-byte words of K, and of V, of a step in LDS
+    // f16: a step's words are copied straight into one buffer while the other is worked on.  int8: they are copied as
+    // they are, and converted by the waves that copied them.
+    constexpr int kBufs = KV == kKvF16 ? 2 : 1, kRaw = KV == kKvInt8 ? kStep * HD / 16 : 1;
+    __shared__ __align__(1024) u4 kt[kBufs][kWords], vt[kBufs][kWords];  // (words are picked by bits of their addresses)
+    __shared__ u4 k_raw[kRaw], v_raw[kRaw];
+    // int8: scales of K and V, and log2 of the latter's size
+    constexpr int kScales = KV == kKvInt8 ? kStep : 4;
+    __shared__ __align__(16) float ksc[kScales], vsc[kScales], vlg[kScales], sc_raw[2][kScales];
+    // f16: positions of the tile, from its first token's last step on, whose values are no numbers
+    __shared__ uint32_t odd[kOddWords];
     const int lane = lane_id(), r = lane & 15, kg = lane >> 4, tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int ps = a.c.ps, psl = 31 - __builtin_clz(ps);
     // neighbouring shares, which read the same pages, on one XCD
     const int g = (blockIdx.x & 7) * (kGroups / 8) + (blockIdx.x >> 3);
+    // of the lane's words of K (row 16 (r/4) + r%4, word kg) and V (dim r, word 2 kg)
+    const uint32_t ka0 = lds_addr(&kt[0][0]) + 16 * k_word<HD>(16 * (r >> 2) + (r & 3), kg);
+    const uint32_t va0 = lds_addr(&vt[0][0]) + 16 * v_word(r, 2 * kg);
+    // ---- a wave's loads: K rows i * kKRows + wave * kKWave + k_l, V dims i * kVRows + wave * kVWave + v_l, 16 bytes a lane,
+    // from uniform addresses and these offsets of the lane
+    constexpr int KW = HD * EB / 16, VW = kStep * EB / 16, kKWave = 64 / KW, kVWave = 64 / VW;
+    constexpr int kKRows = kThreads / KW, kVRows = kThreads / VW, NL = kStep / kKRows;
+    static_assert(NL * kVRows == HD && kKWave <= 16, "whole rows, of one page");
+    const int k_l = lane / KW, v_l = lane / VW;
+    uint32_t k_off = k_l * (HD * EB), v_off = v_l * ps * EB;
+    int v_pos;  // first position of the lane's word of V
+    if (KV == kKvF16) {  // the words lie in LDS in the order that k_word and v_word give them
+        k_off += 16 * (lane % KW ^ (HD == 64 ? (k_l & 3) >> 1 : k_l & 3));
+        v_pos = 8 * (lane % VW ^ ((wave * kVWave + v_l) >> 1 & 7));
+    } else {
+        k_off += 16 * (lane % KW);
+        v_pos = 16 * (lane % VW);
+    }
+    v_off += (v_pos & (ps - 1)) * EB;
 
-    const Plan plan = make_plan(a);
+    const Plan plan = make_plan(a, kGroups);
     int at = first_of(plan, g);
     const int end = first_of(plan, g + 1);
     if (tid == 0) {
         begun_of(a)[g].first = -1;
         taken_of(a)[g] = -1;
     }
-    if (tid < 4) odd[tid >> 1][tid & 1] = 0;
-    int parity = 0;
-    __syncthreads();
+    // of the lane's rows: the token within a tile and its head
+    int tok_of[RT], head_of[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const int row = (wave * RT + rt) * 16 + r;
+        tok_of[rt] = row / a.gqa;
+        head_of[rt] = row - tok_of[rt] * a.gqa;
+    }
+    // the wave's first and last token
+    const int tok_first = __builtin_amdgcn_readfirstlane(tok_of[0]), tok_last = __builtin_amdgcn_readlane(tok_of[RT - 1], 15);
 
+    Where w;
+    if (at < end) w = find(a, plan, at);
     while (at < end) {
-        const Where w = find(a, plan, at);
-        const Seq sq = w.s;
         const int n = min(end - at, w.steps - w.step);
-        const int tok0 = w.tile << a.tl, toks = min(1 << a.tl, sq.n - tok0);
+        const int tok0 = w.tile << a.tl, toks = min(1 << a.tl, w.s.n - tok0);
         const int *table = a.table + (size_t)w.seq * a.max_pages;
-        const int pos0 = sq.len - sq.n + tok0;  // of the tile's first token
-        const uint8_t *kc = (const uint8_t *)a.c.k, *vc = (const uint8_t *)a.c.v;
+        const int pos0 = w.s.len - w.s.n + tok0;  // of the tile's first token
+        const int last = (w.s.len - 1) >> psl;
+        const int odd0 = max(pos0, 0) & ~(kStep - 1);  // what odd begins with
+
+        // ---- a step's pages: the entry of position p0 + lane
+        auto entry = [&](int p0) { return table[min((p0 + lane) >> psl, last)]; };
+        auto valid = [&](int e) { return (unsigned)e < (unsigned)a.c.n_pages ? e : 0; };
+        // copies K and V of the step at p0, into buffer b
+        auto load = [&](int p0, int ent, int b) {
+            const size_t page_bytes = (size_t)ps * HD * EB;  // of a KV head
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                const int row0 = i * kKRows + wave * kKWave;  // (a wave's rows lie in one page)
+                const uint8_t *k = (const uint8_t *)a.c.k + ((size_t)valid(__builtin_amdgcn_readlane(ent, row0)) * a.c.nkv + w.kvh) * page_bytes +
+                                   ((p0 + row0) & (ps - 1)) * (HD * EB);
+                if (KV == kKvF16) {
+                    const int m = ((row0 >> 4) & 3) * 4 + (row0 & 3);
+                    lds_copy16(k, k_off ^ (16 * (HD == 64 ? m >> 1 : m)), lds_addr(&kt[0][0]) + 16 * (b * kWords + i * kThreads + 64 * wave));
+                } else lds_copy16(k, k_off, lds_addr(k_raw) + 16 * (i * kThreads + 64 * wave));
+            }
+            if (ps >= kStep) {
+                const uint8_t *v = (const uint8_t *)a.c.v + ((size_t)valid(__builtin_amdgcn_readfirstlane(ent)) * a.c.nkv + w.kvh) * page_bytes +
+                                   (wave * kVWave * ps + (p0 & (ps - 1))) * EB;
+#pragma unroll
+                for (int i = 0; i < NL; i++, v += kVRows * ps * EB)
+                    if (KV == kKvF16) lds_copy16(v, v_off, lds_addr(&vt[0][0]) + 16 * (b * kWords + i * kThreads + 64 * wave));
+                    else lds_copy16(v, v_off, lds_addr(v_raw) + 16 * (i * kThreads + 64 * wave));
+            } else {
+                const uint8_t *v = (const uint8_t *)a.c.v + ((size_t)valid(__shfl(ent, v_pos)) * a.c.nkv + w.kvh) * page_bytes + v_off +
+                                   wave * kVWave * ps * EB;
+#pragma unroll
+                for (int i = 0; i < NL; i++, v += kVRows * ps * EB)
+                    if (KV == kKvF16) lds_copy16(v, lds_addr(&vt[0][0]) + 16 * (b * kWords + i * kThreads + 64 * wave));
+                    else lds_copy16(v, lds_addr(v_raw) + 16 * (i * kThreads + 64 * wave));
+            }
+            if (KV == kKvInt8 && wave < 2)  // the first waves' copies of the scales
+                lds_copy4((wave ? a.c.vsc : a.c.ksc) + ((size_t)valid(ent) * a.c.nkv + w.kvh) * ps + ((p0 + lane) & (ps - 1)),
+                          lds_addr(&sc_raw[0][0]) + 4 * kStep * wave);
+        };
+        // int8: what the wave has copied, as f16
+        auto convert = [&] {
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                const int row = i * kKRows + wave * kKWave + k_l, d = i * kVRows + wave * kVWave + v_l, kw = lane % KW, vw = lane % VW;
+                const u4 x = k_raw[i * kThreads + tid], y = v_raw[i * kThreads + tid];
+                kt[0][k_word<HD>(row, 2 * kw)] = __builtin_bit_cast(u4, cvt8(x[0], x[1]));
+                kt[0][k_word<HD>(row, 2 * kw + 1)] = __builtin_bit_cast(u4, cvt8(x[2], x[3]));
+                vt[0][v_word(d, 2 * vw)] = __builtin_bit_cast(u4, cvt8(y[0], y[1]));
+                vt[0][v_word(d, 2 * vw + 1)] = __builtin_bit_cast(u4, cvt8(y[2], y[3]));
+            }
+            if (wave < 2) {
+                const float x = sc_raw[wave][lane];
+                (wave ? vsc : ksc)[lane] = x;
+                if (wave) vlg[lane] = __builtin_amdgcn_logf(fabsf(x));
+            }
+        };
+
+        int p0 = w.step * kStep, b = 0;
+        const int p_end = p0 + n * kStep;
+        int ent = entry(p0), ent_next = entry(p0 + kStep);
+        lds_barrier();  // the buffers are free
+        if (KV == kKvF16 && tid < kOddWords) odd[tid] = 0;
+        load(p0, ent, 0);
 
         // ---- the lane's rows
-        int lim[RT];  // last position that the row sees
-        size_t io[RT];  // of its query and output
-        bool used[RT];
+        int lim[RT];  // last position that the row sees; what the rows of no token (INT_MAX) give is dropped
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
-            const int row = (wave * RT + rt) * 16 + r, tok = row / a.gqa, head = row - tok * a.gqa;
-            used[rt] = tok < toks;
-            lim[rt] = used[rt] ? pos0 + tok : INT_MAX;  // what other rows give is dropped
-            io[rt] = ((size_t)(sq.start + tok0 + (used[rt] ? tok : 0)) * a.nh + w.kvh * a.gqa + (used[rt] ? head : 0)) * HD;
-        }
-        int lim_max = -1, lim_min = INT_MAX;
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
-            lim_max = max(lim_max, used[rt] ? lim[rt] : -1);
-            lim_min = min(lim_min, lim[rt]);
-        }
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) {
-            lim_max = max(lim_max, __shfl_xor(lim_max, o));
-            lim_min = min(lim_min, __shfl_xor(lim_min, o));
-        }
-        lim_max = __builtin_amdgcn_readfirstlane(lim_max);
-        lim_min = __builtin_amdgcn_readfirstlane(lim_min);
+        for (int rt = 0; rt < RT; rt++) lim[rt] = tok_of[rt] < toks ? pos0 + tok_of[rt] : INT_MAX;
+        auto io = [&](int rt) {  // of the row's query and output, the tile's first for the rows of no token
+            const bool used = tok_of[rt] < toks;
+            return ((size_t)(w.s.start + tok0 + (used ? tok_of[rt] : 0)) * a.nh + w.kvh * a.gqa + (used ? head_of[rt] : 0)) * HD;
+        };
+        const int lim_min = pos0 + tok_first, lim_max = tok_first < toks ? pos0 + min(tok_last, toks - 1) : -1;
 
         // ---- Q
         h8 qhi[RT][KS], qlo[RT][KS];
         float c[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
+            const float *qp = a.q + io(rt) + 8 * kg;
             float q[KS][8], qm = 0.0f;
 #pragma unroll
             for (int st = 0; st < KS; st++) {
-                __builtin_memcpy(&q[st][0], a.q + io[rt] + 32 * st + 8 * kg, 16);
-                __builtin_memcpy(&q[st][4], a.q + io[rt] + 32 * st + 8 * kg + 4, 16);
+                __builtin_memcpy(&q[st][0], qp + 32 * st, 16);
+                __builtin_memcpy(&q[st][4], qp + 32 * st + 4, 16);
             }
 #pragma unroll
             for (int st = 0; st < KS; st++)
@@ -273,51 +378,21 @@ __global__ void __launch_bounds__(kThreads, 2) paged_prompt_kernel(PagedPromptAr
                 for (int j = 0; j < 8; j++) qm = fmaxf(qm, fabsf(q[st][j]));
             qm = max_row(qm);
             const int qe = (int)((__builtin_bit_cast(uint32_t, qm) >> 23) & 255) - 127;  // exponent of the largest
-            const float qs = ldexpf(1.0f, -qe);
-            c[rt] = ldexpf(a.scale * 1.44269504088896341f, qe);
+            const float qs = copysignf(ldexpf(1.0f, -qe), a.scale);
+            // more than 0, so that the largest product has the largest score and what is masked stays below
+            c[rt] = ldexpf(fabsf(a.scale) * 1.44269504088896341f, qe);
+            c[rt] = c[rt] < FLT_MIN ? FLT_MIN : c[rt];
 #pragma unroll
             for (int st = 0; st < KS; st++)
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    float x = q[st][j] * qs;
-                    asm("" : "+v"(x));  // one value for both parts
-                    qhi[rt][st][j] = (_Float16)x;
-                    qlo[rt][st][j] = (_Float16)(x - (float)qhi[rt][st][j]);
+                for (int j = 0; j < 8; j += 2) {
+                    const h2x2 x = two_parts(q[st][j] * qs, q[st][j + 1] * qs);
+                    qhi[rt][st][j] = x.hi[0];
+                    qhi[rt][st][j + 1] = x.hi[1];
+                    qlo[rt][st][j] = x.lo[0];
+                    qlo[rt][st][j + 1] = x.lo[1];
                 }
         }
-
-        // ---- a step's pages: the entry of position p0 + lane
-        const int last = (sq.len - 1) >> psl;
-        auto entry = [&](int p0) { return table[min((p0 + lane) >> psl, last)]; };
-        auto page_of = [&](int ent, int p) {  // of position p of the step
-            const int e = ps >= kStep ? __builtin_amdgcn_readfirstlane(ent) : __shfl(ent, p);
-            return (unsigned)e < (unsigned)a.c.n_pages ? e : 0;
-        };
-        u4 kr[NL], vr[NL];
-        float sc = 0.0f;
-        auto load = [&](int p0, int ent) {
-#pragma unroll
-            for (int i = 0; i < NL; i++) {
-                constexpr int KW = HD * EB / 16, VW = kStep * EB / 16;  // words of a row
-                const int nn = i * kThreads + tid;
-                const int row = nn / KW, kw = nn % KW;
-                const int kp = page_of(ent, row);
-                const uint8_t *k = kc + ((((size_t)kp * a.c.nkv + w.kvh) * ps + ((p0 + row) & (ps - 1))) * HD) * EB + 16 * kw;
-                __builtin_memcpy(&kr[i], k, 16);
-                const int d = nn / VW, vp0 = nn % VW * (16 / EB);
-                const int vp = page_of(ent, vp0);
-                const uint8_t *v = vc + ((((size_t)vp * a.c.nkv + w.kvh) * HD + d) * ps + ((p0 + vp0) & (ps - 1))) * EB;
-                __builtin_memcpy(&vr[i], v, 16);
-            }
-            if (KV == kKvInt8 && tid < 2 * kStep) {
-                const int e = (unsigned)ent < (unsigned)a.c.n_pages ? ent : 0;
-                sc = (tid < kStep ? a.c.ksc : a.c.vsc)[((size_t)e * a.c.nkv + w.kvh) * ps + ((p0 + lane) & (ps - 1))];
-            }
-        };
-        // positions of a step that are there
-        auto present = [&](int p0, int ent) {
-            return (uint64_t)__ballot((unsigned)ent < (unsigned)a.c.n_pages && p0 + lane < sq.len);
-        };
 
         float m[RT], l[RT];  // reference (log2) of the lane's row, sum over the lane's positions
         f4 o[RT][ND] = {};
@@ -326,207 +401,211 @@ __global__ void __launch_bounds__(kThreads, 2) paged_prompt_kernel(PagedPromptAr
             m[rt] = -INFINITY;
             l[rt] = 0.0f;
         }
-        int p0 = w.step * kStep;
-        const int p_end = p0 + n * kStep;
-        int ent = entry(p0);
-        load(p0, ent);
-        int ent_next = entry(p0 + kStep);
-        for (; p0 < p_end; p0 += kStep) {
-            const uint64_t there = present(p0, ent);
-            const bool edge = there != ~0ull || p0 + kStep - 1 > pos0;  // some row does not see all of the step
+        for (; p0 < p_end; p0 += kStep, b ^= KV == kKvF16) {
+            // positions that are there; whether there is something that some row does not see
+            const uint64_t there = __ballot((unsigned)ent < (unsigned)a.c.n_pages && p0 + lane < w.s.len);
+            wait_vm<0>();  // the wave's own copies
             lds_barrier();
-            // ---- K and V into LDS
-#pragma unroll
-            for (int i = 0; i < NL; i++) {
-                constexpr int KW = HD * EB / 16, VW = kStep * EB / 16;
-                const int nn = i * kThreads + tid;
-                const int row = nn / KW, kw = nn % KW, d = nn / VW, vw = nn % VW;
-                if (KV == kKvF16) {
-                    kt[k_word<HD>(row, kw)] = kr[i];
-                    u4 v = vr[i];
-                    if (edge) {
-                        // what lies past the end, or ahead of a row, may be no number, which a weight of 0 does not hide
-                        const uint32_t in = (uint32_t)(there >> (8 * vw)) & 255u;
-                        uint32_t none = 0;
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            if (!(in >> (2 * j) & 1)) v[j] &= 0xffff0000u;
-                            if (!(in >> (2 * j + 1) & 1)) v[j] &= 0xffffu;
-                            if ((v[j] & 0x7c00u) == 0x7c00u) {
-                                none |= 1u << (2 * j);
-                                v[j] &= 0xffff0000u;
-                            }
-                            if ((v[j] & 0x7c000000u) == 0x7c000000u) {
-                                none |= 2u << (2 * j);
-                                v[j] &= 0xffffu;
-                            }
-                        }
-                        if (none) atomicOr(&odd[parity][vw >> 2], none << (8 * (vw & 3)));
-                    }
-                    vt[v_word(d, vw)] = v;
-                } else {
-                    kt[k_word<HD>(row, 2 * kw)] = __builtin_bit_cast(u4, cvt8(kr[i][0], kr[i][1]));
-                    kt[k_word<HD>(row, 2 * kw + 1)] = __builtin_bit_cast(u4, cvt8(kr[i][2], kr[i][3]));
-                    vt[v_word(d, 2 * vw)] = int8_bf16(vr[i][0], vr[i][1]);
-                    vt[v_word(d, 2 * vw + 1)] = int8_bf16(vr[i][2], vr[i][3]);
-                }
+            if (KV == kKvInt8) {
+                convert();
+                lds_barrier();
             }
-            if (KV == kKvInt8 && tid < 2 * kStep) (tid < kStep ? ksc : vsc)[lane] = sc;
-            lds_barrier();
-            const int ent_now = ent;
-            if (p0 + kStep < p_end) {
-                ent = ent_next;
-                load(p0 + kStep, ent);
-                ent_next = entry(p0 + 2 * kStep);
-            }
-            uint64_t none = 0;
-            if (KV == kKvF16 && edge) none = (uint64_t)odd[parity][1] << 32 | odd[parity][0];
-            parity ^= 1;
-            if (tid < 2) odd[parity][tid] = 0;  // (last read before the step's first barrier)
-            if (p0 > lim_max) continue;  // no row of the wave sees the step
-            // ---- S^T: lane: row r, positions p0 + 16 kg + 4t + i
-            f4 s[RT][4] = {};
+            if (KV == kKvF16 && (there != ~0ull || p0 + kStep - 1 > pos0)) {
+                // V past the end, or ahead of a row, may be no number, which a weight of 0 does not hide: it becomes 0.
+                // What is there and no number is noted, for the rows that do see it.
+                const int p = v_pos, in = (int)((there >> p) & 255);
+                const bool ahead = p0 >= odd0;  // else all rows see what is there
+                uint32_t sum = 0;  // bit 15 of a half: an exponent of all ones is among them
 #pragma unroll
-            for (int st = 0; st < KS; st++)
+                for (int i = 0; i < NL; i++) {
+                    const u4 v = vt[b][i * kThreads + tid];
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const h8 kf = __builtin_bit_cast(h8, kt[k_word<HD>(16 * (r >> 2) + 4 * t + (r & 3), 4 * st + kg)]);
-#pragma unroll
-                    for (int rt = 0; rt < RT; rt++) {
-                        s[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qhi[rt][st], s[rt][t], 0, 0, 0);
-                        s[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qlo[rt][st], s[rt][t], 0, 0, 0);
-                    }
+                    for (int j = 0; j < 4; j++) sum |= (v[j] & 0x7fff7fffu) + 0x04000400u;
                 }
-            // ---- weights
-            const bool full = there == ~0ull && p0 + kStep - 1 <= lim_min;  // uniform
-            const uint32_t mine = (uint32_t)(there >> (16 * kg)) & 0xffffu;
-            h8 phi[RT][2], plo[RT][2];
-            b8 pb[RT][2][3];
-#pragma unroll
-            for (int rt = 0; rt < RT; rt++) {
-                float smax = -INFINITY;
-#pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    f4 ks;
-                    if (KV == kKvInt8) ks = *(const f4 *)&ksc[16 * kg + 4 * t];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        float x = s[rt][t][i] * c[rt];
-                        if (KV == kKvInt8) x *= ks[i];
-                        if (!full) x = (mine >> (4 * t + i) & 1) && p0 + 16 * kg + 4 * t + i <= lim[rt] ? x : -INFINITY;
-                        s[rt][t][i] = x;
-                        smax = fmaxf(smax, x);
-                    }
-                }
-                if (__any(smax > m[rt] + kSlack)) {  // uniform
-                    const float mn = fmaxf(m[rt], max_row(smax));
-                    const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - mn);
-                    l[rt] *= al;
-                    m[rt] = mn;
-#pragma unroll
-                    for (int i = 0; i < ND; i++) o[rt][i] *= al;
-                }
-                const float ref = m[rt] == -INFINITY ? 0.0f : KV == kKvF16 ? m[rt] - kLift : m[rt];
-                if (KV == kKvF16) {
-#pragma unroll
-                    for (int t = 0; t < 4; t++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            float p = __builtin_amdgcn_exp2f(s[rt][t][i] - ref);
-                            l[rt] += p;
-                            asm("" : "+v"(p));
-                            const _Float16 hi = (_Float16)p;
-                            phi[rt][t / 2][4 * (t & 1) + i] = hi;
-                            plo[rt][t / 2][4 * (t & 1) + i] = (_Float16)(p - (float)hi);
-                        }
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        float p[8];
+                if (in != 255 || (ahead && (sum & 0x80008000u))) {
+                    uint32_t bad = 0;
+                    for (int i = 0; i < NL; i++) {
+                        u4 v = vt[b][i * kThreads + tid];
 #pragma unroll
                         for (int j = 0; j < 8; j++) {
-                            const int t = 2 * k + j / 4, i = j & 3;
-                            const float x = __builtin_amdgcn_exp2f(s[rt][t][i] - ref);
-                            l[rt] += x;
-                            p[j] = x * vsc[16 * kg + 4 * t + i];
-                            // the scale of a masked position may be no number
-                            if (!full) p[j] = s[rt][t][i] == -INFINITY ? 0.0f : p[j];
+                            const uint32_t inf = 0x7c00u << (16 * (j & 1));
+                            const bool none = ahead && (v[j / 2] & inf) == inf;
+                            if (none || !(in >> j & 1)) v[j / 2] &= ~(0xffffu << (16 * (j & 1)));
+                            if (none && (in >> j & 1)) bad |= 1u << j;
                         }
-                        bf16_parts(p, pb[rt][k]);
+                        vt[b][i * kThreads + tid] = v;
                     }
+                    if (bad) atomicOr(&odd[(p0 - odd0 + p) >> 5], bad << (p & 31));
                 }
+                lds_barrier();
             }
-            // ---- O^T
+            if (p0 + kStep < p_end) {
+                ent = ent_next;
+                ent_next = entry(p0 + 2 * kStep);
+                load(p0 + kStep, ent, b ^ 1);
+            }
+            if (p0 > lim_max) continue;  // no row of the wave sees the step
+            const bool full = there == ~0ull && p0 + kStep - 1 <= lim_min;  // uniform
+            // ---- in halves: of a lane's 16 positions the first 8, then the others.  Operands are read from LDS a phase
+            // ahead: K for the products before, V for the weights before
+            const uint32_t kb = ka0 + b * (16 * kWords), vb = va0 + b * (16 * kWords);
+            u4 w8[ND > 2 * KS ? ND : 2 * KS];
+            auto read_k = [&](int k) {
 #pragma unroll
-            for (int i = 0; i < ND; i++)
+                for (int st = 0; st < KS; st++)
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const u4 vw = vt[v_word(16 * i + r, 2 * kg + k)];
+                    for (int t = 0; t < 2; t++) w8[2 * st + t] = lds_get<u4>(kb ^ (64 * st), (8 * k + 4 * t) * (HD * 2));
+            };
+            read_k(0);
 #pragma unroll
-                    for (int rt = 0; rt < RT; rt++) {
-                        if (KV == kKvF16) {
-                            o[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, vw), phi[rt][k], o[rt][i], 0, 0, 0);
-                            o[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, vw), plo[rt][k], o[rt][i], 0, 0, 0);
-                        } else {
+            for (int k = 0; k < 2; k++) {
+                // S^T: lane: row r, positions p0 + first + 4t + i
+                const int first = 16 * kg + 8 * k;
+                f4 s[RT][2] = {};
 #pragma unroll
-                            for (int j = 2; j >= 0; j--)
-                                o[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, vw), pb[rt][k][j], o[rt][i], 0, 0, 0);
-                        }
-                    }
+                for (int st = 0; st < KS; st++) {
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+#pragma unroll
+                        for (int rt = 0; rt < RT; rt++) s[rt][t] = mfma(__builtin_bit_cast(h8, w8[2 * st + t]), qhi[rt][st], s[rt][t]);
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+#pragma unroll
+                        for (int rt = 0; rt < RT; rt++) s[rt][t] = mfma(__builtin_bit_cast(h8, w8[2 * st + t]), qlo[rt][st], s[rt][t]);
                 }
-            // ---- values that are no numbers, for the rows that see them
-            while (KV == kKvF16 && none) {
-                const int j = __ffsll((unsigned long long)none) - 1;
-                none &= none - 1;
-                const int page = __builtin_amdgcn_readlane(ent_now, j);
+                auto read_v = [&] {
+#pragma unroll
+                    for (int i = 0; i < ND; i++) w8[i] = lds_get<u4>(vb ^ (16 * k), i * (16 * kStep * 2));
+                };
+                if (kEarly) {
+                    read_v();
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                // weights
+                h8 phi[RT], plo[RT];
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++) {
-                    float p = 0.0f;
+                    uint32_t seen = 255;
+                    if (!full) {
+                        const int live = min(max(lim[rt] - (p0 + first), -1), 7) + 1;
+                        seen = (uint32_t)(there >> first) & ((1u << live) - 1);
+                    }
+                    float top = -INFINITY;  // of the lane's scores
+                    f4 f[2], vs[2];
+                    if (KV == kKvF16) {
+                        if (!full) {
 #pragma unroll
-                    for (int x = 0; x < 16; x++)
-                        if (x == (j & 15)) p = (float)phi[rt][x >> 3][x & 7] + (float)plo[rt][x >> 3][x & 7];
-                    p = __shfl(p, (j & ~15) + r);
+                            for (int j = 0; j < 8; j++) s[rt][j / 4][j & 3] = seen >> j & 1 ? s[rt][j / 4][j & 3] : -INFINITY;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 8; j++) top = fmaxf(top, s[rt][j / 4][j & 3]);
+                        top *= c[rt];
+                    } else {
+#pragma unroll
+                        for (int t = 0; t < 2; t++) {
+                            f[t] = *(const f4 *)&ksc[first + 4 * t] * c[rt];
+                            vs[t] = *(const f4 *)&vsc[first + 4 * t];
+                            const f4 lg = *(const f4 *)&vlg[first + 4 * t];
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                const float y = fmaf(s[rt][t][i], f[t][i], lg[i]);
+                                top = fmaxf(top, full || (seen >> (4 * t + i) & 1) ? y : -INFINITY);
+                            }
+                        }
+                    }
+                    if (__any(top > m[rt] + kSlack)) {  // uniform
+                        top = max_row(top);
+                        const float mn = top > m[rt] + kSlack ? top : m[rt];  // a row's own doing
+                        const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - mn);
+                        l[rt] *= al;
+                        m[rt] = mn;
+#pragma unroll
+                        for (int i = 0; i < ND; i++) o[rt][i] *= al;
+                    }
+                    const float ref = m[rt] == -INFINITY ? 0.0f : m[rt] - kLift;
+                    float p[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        float x = fmaf(s[rt][j / 4][j & 3], KV == kKvF16 ? c[rt] : f[j / 4][j & 3], -ref);
+                        if (KV == kKvInt8 && !full) x = seen >> j & 1 ? x : -INFINITY;
+                        x = __builtin_amdgcn_exp2f(x);
+                        l[rt] += x;
+                        // (the scale of a position that is not seen may be no number)
+                        if (KV == kKvInt8) x = full || (seen >> j & 1) ? x * vs[j / 4][j & 3] : 0.0f;
+                        p[j] = x;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; j += 2) {
+                        const h2x2 x = two_parts(p[j], p[j + 1]);
+                        phi[rt][j] = x.hi[0];
+                        phi[rt][j + 1] = x.hi[1];
+                        plo[rt][j] = x.lo[0];
+                        plo[rt][j + 1] = x.lo[1];
+                    }
+                }
+                if (!kEarly) read_v();
+                // O^T
+#pragma unroll
+                for (int i = 0; i < ND; i++)
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++) o[rt][i] = mfma(__builtin_bit_cast(h8, w8[i]), phi[rt], o[rt][i]);
+#pragma unroll
+                for (int i = 0; i < ND; i++)
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++) o[rt][i] = mfma(__builtin_bit_cast(h8, w8[i]), plo[rt], o[rt][i]);
+                if (k == 0) read_k(1);
+            }
+        }
+        if (KV == kKvF16) {
+            // values that are no numbers: nor is, then, their dim of the rows that see them.  (The last barrier has passed
+            // since they were noted.)
+            for (int i = 0; i < kOddWords; i++)
+                for (uint32_t left = odd[i]; left; left &= left - 1) {
+                    const int p = odd0 + 32 * i + __ffs((int)left) - 1;
+                    const int page = valid(table[min(p >> psl, last)]);
+                    const uint16_t *v = (const uint16_t *)a.c.v + (((size_t)page * a.c.nkv + w.kvh) * HD + 4 * kg) * ps + (p & (ps - 1));
 #pragma unroll
                     for (int i = 0; i < ND; i++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int d = 16 * i + 4 * kg + e;
-                            const float v = h2f(((const uint16_t *)vc)[(((size_t)page * a.c.nkv + w.kvh) * HD + d) * ps + ((p0 + j) & (ps - 1))]);
-                            if (!(fabsf(v) <= 65504.0f) && p0 + j <= lim[rt]) o[rt][i][e] += p * v;
+                        for (int e = 0; e < 4; e++, v += e < 4 ? ps : 13 * ps) {
+                            const bool none = (*v & 0x7c00) == 0x7c00;
+#pragma unroll
+                            for (int rt = 0; rt < RT; rt++)
+                                if (none && p <= lim[rt]) o[rt][i][e] = NAN;
                         }
                 }
-            }
         }
         const bool begins = w.step == 0, finishes = w.step + n == w.steps;
-        const int piece = 2 * g + begins;
-        float *part = a.ws + (size_t)piece * part_floats(HD);
+        float *part = a.ws + (size_t)(2 * g + begins) * part_floats(HD);
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
             const float sum = sum_row(l[rt]);
-            if (!used[rt]) continue;
+            if (lim[rt] == INT_MAX) continue;
             if (begins && finishes) {
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                float *out = a.out + io(rt) + 4 * kg;
 #pragma unroll
                 for (int i = 0; i < ND; i++) {
                     const f4 x = o[rt][i] * inv;
-                    __builtin_memcpy(a.out + io[rt] + 16 * i + 4 * kg, &x, 16);
+                    __builtin_memcpy(out + 16 * i, &x, 16);
                 }
             } else {
                 const int row = (wave * RT + rt) * 16 + r;
                 if (kg == 0) {
                     part[row] = m[rt];
-                    part[S::kRows + row] = sum;
+                    part[kRows + row] = sum;
                 }
 #pragma unroll
                 for (int i = 0; i < ND; i++)
-                    __builtin_memcpy(part + 2 * S::kRows + (size_t)row * HD + 16 * i + 4 * kg, &o[rt][i], 16);
+                    __builtin_memcpy(part + 2 * kRows + (size_t)row * HD + 16 * i + 4 * kg, &o[rt][i], 16);
             }
         }
         if (tid == 0) {
             if (!begins) taken_of(a)[g] = at - w.step;
-            else if (!finishes) begun_of(a)[g] = {at, sq.start + tok0, toks * a.gqa, w.kvh};
+            else if (!finishes) begun_of(a)[g] = {at, w.s.start + tok0, toks * a.gqa, w.kvh};
         }
         at += n;
+        if (at < end) advance(a, w);
     }
 
     if (__any(plan.short_))  // tokens before position 0: zeros
@@ -539,14 +618,18 @@ __global__ void __launch_bounds__(kThreads, 2) paged_prompt_kernel(PagedPromptAr
         }
 }
 
-// Merges the partials of the tile that begins in workgroup blockIdx.x's share and goes on behind it; blockIdx.y: 16 of
-// its rows.
+// Merges the partials of the tile that begins in workgroup blockIdx.x's share and goes on behind it.  256 threads are
+// HD / 4 lanes of four dims, times 4 rows (blockIdx.y: which), times threads that divide the partials among them.
 template <int HD>
 __global__ void __launch_bounds__(256) paged_prompt_merge_kernel(PagedPromptArgs a) {
+    constexpr int kGroups = groups_of(HD), D4 = HD / 4, ROWS = 4, CHAIN = 256 / (D4 * ROWS) > 0 ? 256 / (D4 * ROWS) : 1;
+    constexpr int ROW_PASS = 256 / (D4 * CHAIN);  // rows at once
+    __shared__ __align__(16) float so[CHAIN][ROW_PASS][HD];
+    __shared__ float sm[CHAIN][ROW_PASS], sl[CHAIN][ROW_PASS];
     const Begun b = begun_of(a)[blockIdx.x];
-    if (b.first < 0 || 16 * (int)blockIdx.y >= b.n_rows) return;
+    if (b.first < 0 || ROWS * (int)blockIdx.y >= b.n_rows) return;
     const int *taken = taken_of(a);
-    int n = 0;
+    int n = 1;
     for (int g0 = blockIdx.x + 1; g0 < kGroups; g0 += 64) {  // workgroups that go on with it, one after another
         const int g = g0 + lane_id();
         const uint64_t on = __ballot(g < kGroups && taken[min(g, kGroups - 1)] == b.first);
@@ -554,55 +637,94 @@ __global__ void __launch_bounds__(256) paged_prompt_merge_kernel(PagedPromptArgs
         n += more;
         if (more < 64) break;
     }
-    constexpr int R = rows_of(HD);
-    const float *first = a.ws + (size_t)(2 * blockIdx.x + 1) * part_floats(HD);
-    const float *rest = a.ws + (size_t)(2 * blockIdx.x + 2) * part_floats(HD);  // every second one from here
-    for (int e = threadIdx.x; e < 16 * (HD / 4); e += 256) {
-        const int row = 16 * blockIdx.y + e / (HD / 4), d = 4 * (e % (HD / 4));
-        if (row >= b.n_rows) break;
-        float mm = first[row];
-#pragma unroll 4
-        for (int i = 0; i < n; i++) mm = fmaxf(mm, rest[(size_t)2 * i * part_floats(HD) + row]);
+    // partial i: the second of workgroup blockIdx.x, then the first of each that follows
+    auto part = [&](int i) { return a.ws + (size_t)(2 * (blockIdx.x + i) + (i == 0)) * part_floats(HD); };
+    const int d = 4 * (threadIdx.x % D4), c = threadIdx.x / D4 % CHAIN, rr = threadIdx.x / (D4 * CHAIN);
+    for (int r0 = 0; r0 < ROWS; r0 += ROW_PASS) {
+        const int row = ROWS * blockIdx.y + r0 + rr;
+        const int in = min(row, b.n_rows - 1);
+        float m = -INFINITY, l = 0.0f;
         f4 x = {};
-        float sum = 0.0f;
-#pragma unroll 4
-        for (int i = -1; i < n; i++) {
-            const float *p = i < 0 ? first : rest + (size_t)2 * i * part_floats(HD);
-            const float f = mm == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(p[row] - mm);
-            f4 y;
-            __builtin_memcpy(&y, p + 2 * R + (size_t)row * HD + d, 16);
-            x += y * f;
-            sum = fmaf(p[R + row], f, sum);
+        for (int i0 = c; i0 < n; i0 += 4 * CHAIN) {  // four loads in flight
+            float pm[4], pl[4];
+            f4 y[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const float *p = part(min(i0 + u * CHAIN, n - 1));
+                pm[u] = p[in];
+                pl[u] = p[kRows + in];
+                __builtin_memcpy(&y[u], p + 2 * kRows + (size_t)in * HD + d, 16);
+                if (i0 + u * CHAIN >= n) {
+                    pm[u] = -INFINITY;
+                    pl[u] = 0.0f;
+                    y[u] = f4{0.f, 0.f, 0.f, 0.f};
+                }
+            }
+            float mn = m;
+#pragma unroll
+            for (int u = 0; u < 4; u++) mn = fmaxf(mn, pm[u]);
+            const float f0 = mn == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+            x *= f0;
+            l *= f0;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const float f = mn == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm[u] - mn);
+                x += y[u] * f;  // (partials of a query that is no number are none, and stay it)
+                l = fmaf(pl[u], f, l);
+            }
+            m = mn;
         }
-        x *= sum == 0.0f ? 0.0f : 1.0f / sum;
-        const int tok = row / a.gqa, head = row - tok * a.gqa;
-        __builtin_memcpy(a.out + ((size_t)(b.row0 + tok) * a.nh + b.kvh * a.gqa + head) * HD + d, &x, 16);
+        if (CHAIN > 1) {
+            __syncthreads();
+            __builtin_memcpy(&so[c][rr][d], &x, 16);
+            if (d == 0) {
+                sm[c][rr] = m;
+                sl[c][rr] = l;
+            }
+            __syncthreads();
+            if (c == 0) {
+                float mn = m;
+#pragma unroll
+                for (int i = 1; i < CHAIN; i++) mn = fmaxf(mn, sm[i][rr]);
+                f4 sum = {};
+                l = 0.0f;
+#pragma unroll
+                for (int i = 0; i < CHAIN; i++) {
+                    const float f = mn == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[i][rr] - mn);
+                    f4 y;
+                    __builtin_memcpy(&y, &so[i][rr][d], 16);
+                    sum += y * f;
+                    l = fmaf(sl[i][rr], f, l);
+                }
+                x = sum;
+            }
+        }
+        if (c == 0 && row < b.n_rows) {
+            x *= l == 0.0f ? 0.0f : 1.0f / l;
+            const int tok = row / a.gqa, head = row - tok * a.gqa;
+            __builtin_memcpy(a.out + ((size_t)(b.row0 + tok) * a.nh + b.kvh * a.gqa + head) * HD + d, &x, 16);
+        }
     }
 }
 
 template <int KV, int HD>
 int launch_shape(const PagedPromptArgs &a, hipStream_t s) {
-    hipLaunchKernelGGL((paged_prompt_kernel<KV, HD>), dim3(kGroups), dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL((paged_prompt_kernel<KV, HD>), dim3(groups_of(HD)), dim3(Shape<HD>::kThreads), 0, s, a);
     if (int rc = check_launch("paged_attention_prompt")) return rc;
-    hipLaunchKernelGGL(paged_prompt_merge_kernel<HD>, dim3(kGroups, rows_of(HD) / 16), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(paged_prompt_merge_kernel<HD>, dim3(groups_of(HD), kRows / 4), dim3(256), 0, s, a);
     return check_launch("paged_attention_prompt");
 }
 
 }  // namespace
 
 size_t paged_prompt_workspace_bytes(int hd) {
-    return (size_t)2 * kGroups * part_floats(hd) * sizeof(float) + kGroups * (sizeof(Begun) + sizeof(int));
-}
-
-// Tokens of a tile: a power of two, whose rows fill the tile as far as they can.
-int paged_prompt_tile_log(int hd, int gqa) {
-    int tl = 0;
-    while ((2 << tl) * gqa <= rows_of(hd)) tl++;
-    return tl;
+    return (size_t)groups_of(hd) * (2 * part_floats(hd) * sizeof(float) + sizeof(Begun) + sizeof(int));
 }
 
 int launch_paged_prompt(PagedPromptArgs a, hipStream_t s) {
-    a.tl = paged_prompt_tile_log(a.c.hd, a.gqa);
+    // tokens of a tile: a power of two, whose rows fill the tile as far as they can
+    a.tl = 0;
+    while ((2 << a.tl) * a.gqa <= kRows) a.tl++;
     if (a.c.kv_type == kKvF16)
         return a.c.hd == 64 ? launch_shape<kKvF16, 64>(a, s) : a.c.hd == 128 ? launch_shape<kKvF16, 128>(a, s)
                                                                               : launch_shape<kKvF16, 256>(a, s);
