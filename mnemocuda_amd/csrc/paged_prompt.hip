@@ -208,14 +208,13 @@ __device__ __forceinline__ int v_word(int d, int c) { return d * (kStep / 8) + (
 // words that the first and the last of them lie in.
 constexpr int kOddWords = (kRows + 2 * kStep) / 32;
 
-// Two f16 parts of each of two values: together 22 bits or more.
+// Two f16 parts of each of two values, the first cut off, the second rounded: together 22 bits or more.
 struct h2x2 {
     h2 hi, lo;
 };
 __device__ __forceinline__ h2x2 two_parts(float a, float b) {
-    asm("" : "+v"(a), "+v"(b));  // one value for both parts: a product folded into a conversion would round differently
     h2x2 x;
-    x.hi = h2{(_Float16)a, (_Float16)b};
+    x.hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(a, b));
     x.lo = h2{(_Float16)fmaf((float)x.hi[0], -1.0f, a), (_Float16)fmaf((float)x.hi[1], -1.0f, b)};
     return x;
 }
@@ -225,7 +224,6 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
     using S = Shape<HD>;
     constexpr int RT = S::RT, KS = S::kKs, ND = S::kNd, kThreads = S::kThreads, kGroups = groups_of(HD);
     constexpr int EB = KV == kKvF16 ? 2 : 1;
-    constexpr bool kEarly = KV == kKvF16 || HD == 64;  // V's operands wait in registers for the weights
     constexpr int kWords = kStep * HD / 8;  // 16-byte words of K, and of V, of a step in LDS
     // f16: a step's words are copied straight into one buffer while the other is worked on.  int8: they are copied as
     // they are, and converted by the waves that copied them.
@@ -446,41 +444,45 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
             }
             if (p0 > lim_max) continue;  // no row of the wave sees the step
             const bool full = there == ~0ull && p0 + kStep - 1 <= lim_min;  // uniform
-            // ---- in halves: of a lane's 16 positions the first 8, then the others.  Operands are read from LDS a phase
-            // ahead: K for the products before, V for the weights before
+            // ---- in halves: of a lane's 16 positions the first 8, then the others.  Operands are read from LDS four at a
+            // time, four ahead of the products: K for the products before, V for the weights before.
             const uint32_t kb = ka0 + b * (16 * kWords), vb = va0 + b * (16 * kWords);
-            u4 w8[ND > 2 * KS ? ND : 2 * KS];
-            auto read_k = [&](int k) {
+            constexpr int CK = KS / 2, CV = ND / 4;  // fours of K and of V
+            u4 w4[2][4];
+            auto read_k = [&](int k, int n, int to) {
 #pragma unroll
-                for (int st = 0; st < KS; st++)
-#pragma unroll
-                    for (int t = 0; t < 2; t++) w8[2 * st + t] = lds_get<u4>(kb ^ (64 * st), (8 * k + 4 * t) * (HD * 2));
+                for (int i = 0; i < 4; i++) w4[to][i] = lds_get<u4>(kb ^ (64 * (2 * n + i / 2)), (8 * k + 4 * (i & 1)) * (HD * 2));
+                __builtin_amdgcn_sched_barrier(0x7f);  // (LDS reads stay where they are)
             };
-            read_k(0);
+            auto read_v = [&](int k, int n, int to) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) w4[to][i] = lds_get<u4>(vb ^ (16 * k), (4 * n + i) * (16 * kStep * 2));
+                __builtin_amdgcn_sched_barrier(0x7f);
+            };
+            read_k(0, 0, 0);
 #pragma unroll
             for (int k = 0; k < 2; k++) {
+                constexpr int per_half = CK + CV;
                 // S^T: lane: row r, positions p0 + first + 4t + i
                 const int first = 16 * kg + 8 * k;
                 f4 s[RT][2] = {};
 #pragma unroll
-                for (int st = 0; st < KS; st++) {
+                for (int n = 0; n < CK; n++) {
+                    const int at = (k * per_half + n) & 1;
+                    if (n + 1 < CK) read_k(k, n + 1, at ^ 1);
 #pragma unroll
-                    for (int t = 0; t < 2; t++)
+                    for (int st = 0; st < 2; st++) {
 #pragma unroll
-                        for (int rt = 0; rt < RT; rt++) s[rt][t] = mfma(__builtin_bit_cast(h8, w8[2 * st + t]), qhi[rt][st], s[rt][t]);
+                        for (int t = 0; t < 2; t++)
 #pragma unroll
-                    for (int t = 0; t < 2; t++)
+                            for (int rt = 0; rt < RT; rt++) s[rt][t] = mfma(__builtin_bit_cast(h8, w4[at][2 * st + t]), qhi[rt][2 * n + st], s[rt][t]);
 #pragma unroll
-                        for (int rt = 0; rt < RT; rt++) s[rt][t] = mfma(__builtin_bit_cast(h8, w8[2 * st + t]), qlo[rt][st], s[rt][t]);
+                        for (int t = 0; t < 2; t++)
+#pragma unroll
+                            for (int rt = 0; rt < RT; rt++) s[rt][t] = mfma(__builtin_bit_cast(h8, w4[at][2 * st + t]), qlo[rt][2 * n + st], s[rt][t]);
+                    }
                 }
-                auto read_v = [&] {
-#pragma unroll
-                    for (int i = 0; i < ND; i++) w8[i] = lds_get<u4>(vb ^ (16 * k), i * (16 * kStep * 2));
-                };
-                if (kEarly) {
-                    read_v();
-                    __builtin_amdgcn_sched_barrier(0);
-                }
+                read_v(k, 0, (k * per_half + CK) & 1);
                 // weights
                 h8 phi[RT], plo[RT];
 #pragma unroll
@@ -543,17 +545,21 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
                         plo[rt][j + 1] = x.lo[1];
                     }
                 }
-                if (!kEarly) read_v();
                 // O^T
 #pragma unroll
-                for (int i = 0; i < ND; i++)
+                for (int n = 0; n < CV; n++) {
+                    const int at = (k * per_half + CK + n) & 1;
+                    if (n + 1 < CV) read_v(k, n + 1, at ^ 1);
+                    else if (k == 0) read_k(1, 0, at ^ 1);
 #pragma unroll
-                    for (int rt = 0; rt < RT; rt++) o[rt][i] = mfma(__builtin_bit_cast(h8, w8[i]), phi[rt], o[rt][i]);
+                    for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int i = 0; i < ND; i++)
+                        for (int rt = 0; rt < RT; rt++) o[rt][4 * n + i] = mfma(__builtin_bit_cast(h8, w4[at][i]), phi[rt], o[rt][4 * n + i]);
 #pragma unroll
-                    for (int rt = 0; rt < RT; rt++) o[rt][i] = mfma(__builtin_bit_cast(h8, w8[i]), plo[rt], o[rt][i]);
-                if (k == 0) read_k(1);
+                    for (int i = 0; i < 4; i++)
+#pragma unroll
+                        for (int rt = 0; rt < RT; rt++) o[rt][4 * n + i] = mfma(__builtin_bit_cast(h8, w4[at][i]), plo[rt], o[rt][4 * n + i]);
+                }
             }
         }
         if (KV == kKvF16) {
