@@ -474,7 +474,7 @@ int mnemo_logits_process(const float *logits, float *out, int n_rows, int vocab,
  * A token before position 0 gets zeros; rows of no sequence are left as they are; the positions of a
  * page id outside 0..n_pages-1 are absent.  What a token does not see does not reach it, whatever it
  * holds.  n_heads = gqa * n_kv_heads with gqa <= 16; sizes as for mnemo_paged_attention_decode;
- * n_tokens <= 4,194,304, and (n_tokens * gqa / 32 + n_seqs) * n_kv_heads * max_pages * page_size < 2^36.
+ * n_tokens <= 4,194,304, and (n_tokens * gqa / 32 + n_seqs) * n_kv_heads * max_pages * page_size < 2^35.
  * out must not overlap q.  workspace: mnemo_paged_attention_prompt_workspace_bytes(...) bytes (68 MB at
  * most), 16-byte aligned, no initialisation; calls sharing it must not overlap. */
 size_t mnemo_paged_attention_prompt_workspace_bytes(int n_heads, int n_kv_heads, int head_dim);

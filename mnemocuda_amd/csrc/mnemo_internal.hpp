@@ -256,7 +256,7 @@ struct PagedPromptArgs {
     int n_tokens, n_seqs, max_pages, nh, gqa;
     float scale;
     float *ws;
-    int tl;  // log2 of the tokens of a tile (launch_paged_prompt)
+    int tl, cost;  // log2 of the tokens of a tile, what one takes beside its steps (launch_paged_prompt)
 };
 size_t paged_prompt_workspace_bytes(int hd);
 int launch_paged_prompt(PagedPromptArgs a, hipStream_t s);

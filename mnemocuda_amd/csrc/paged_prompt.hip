@@ -35,6 +35,9 @@ namespace {
 
 constexpr float kSlack = 5.0f, kLift = 9.0f;  // powers of two
 constexpr int kStep = 64;                     // positions
+// The shares are counted in units: a step is one, and what a tile takes beside its steps (its queries, its output) are
+// a few, `cost`.  A share has kLeast or more, as far as there are any.
+constexpr int kLeast = 3;
 
 // 128 rows, by 4 waves of 32 or, at head_dim 256, 8 of 16: two waves per SIMD either way.
 constexpr int kRows = 128;
@@ -47,11 +50,11 @@ struct Shape {
 __host__ __device__ constexpr int groups_of(int hd) { return hd == 256 ? 256 : 512; }  // workgroups that fill the chip
 
 // Workspace: two partials per workgroup (max [rows], sum [rows], O [rows][hd]), and what they are: begun[g] describes the
-// tile that begins in workgroup g's share and goes on behind it (its second partial), taken[g] is the first step of the
+// tile that begins in workgroup g's share and goes on behind it (its second partial), taken[g] is the first unit of the
 // tile that it goes on with from the workgroup before (its first), -1 for none.
 __host__ __device__ constexpr int part_floats(int hd) { return kRows * (hd + 2); }
 struct Begun {
-    int first;  // first step, -1 for none
+    int first;  // first unit, -1 for none
     int row0, n_rows, kvh;  // first token (row of q), rows in use, KV head
 };
 __device__ __forceinline__ Begun *begun_of(const PagedPromptArgs &a) {
@@ -74,9 +77,9 @@ __device__ __forceinline__ Seq seq_of(const PagedPromptArgs &a, int s) {
 // x (x + 1) / 2 modulo 2^32
 __device__ __forceinline__ uint32_t triangle(uint32_t x) { return x & 1 ? x * ((x + 1) / 2) : (x / 2) * (x + 1); }
 
-// The steps of the first j tiles of 2^tl tokens, none of them the sequence's last: the sum over i = 1 .. j of
-// ceil(max(b + i 2^tl, 0) / 64), b = len - n.
-__device__ __forceinline__ int steps_before(const Seq &s, int tl, int j) {
+// The units of the first j tiles of 2^tl tokens, none of them the sequence's last: with b = len - n, the sum over
+// i = 1 .. j of ceil(max(b + i 2^tl, 0) / 64) steps, and `cost` for each tile that has one.
+__device__ __forceinline__ int units_before(const Seq &s, int tl, int cost, int j) {
     int b = s.len - s.n;
     if (b < 0) {  // tiles of tokens before position 0 have no steps
         const int none = min(-b >> tl, j);
@@ -84,26 +87,26 @@ __device__ __forceinline__ int steps_before(const Seq &s, int tl, int j) {
         b += none << tl;
         if (b <= -(1 << tl)) return 0;
     }
-    if (tl > 6) return j * (j + 1) * (1 << (tl - 7)) + j * ((b + 63) >> 6);
+    if (tl > 6) return j * (j + 1) * (1 << (tl - 7)) + j * (((b + 63) >> 6) + cost);
     const int gl = 6 - tl;
     const uint32_t c = (uint32_t)(b + (1 << tl) - 1) >> tl, d = c + (uint32_t)j;  // ceil(u / 2^gl) from u = c + 1 to d
     auto sum = [&](uint32_t x) { return (triangle(x >> gl) << gl) + (x & ((1u << gl) - 1)) * ((x >> gl) + 1); };
-    return (int)(sum(d) - sum(c));
+    return (int)(sum(d) - sum(c)) + j * cost;
 }
 __device__ __forceinline__ int tiles_of(const Seq &s, int tl) { return (s.n + (1 << tl) - 1) >> tl; }
 // of one KV head
-__device__ __forceinline__ int steps_of(const Seq &s, int tl) {
+__device__ __forceinline__ int units_of(const Seq &s, int tl, int cost) {
     if (s.n == 0 || s.len == 0) return 0;
-    return steps_before(s, tl, tiles_of(s, tl) - 1) + (s.len + kStep - 1) / kStep;
+    return units_before(s, tl, cost, tiles_of(s, tl) - 1) + (s.len + kStep - 1) / kStep + cost;
 }
 
 struct Plan {
-    int total;       // steps
+    int total;       // units
     int groups;      // workgroups that have some
-    int base, more;  // steps of a workgroup; the first `more` of them have one more
+    int base, more;  // units of a workgroup; the first `more` of them have one more
     bool short_;     // lane: a sequence of its has tokens before position 0
     int per;         // sequences per lane of the sums
-    int before;      // lane: steps before its sequences
+    int before;      // lane: units before its sequences
 };
 __device__ __forceinline__ Plan make_plan(const PagedPromptArgs &a, int groups) {
     Plan p;
@@ -115,13 +118,13 @@ __device__ __forceinline__ Plan make_plan(const PagedPromptArgs &a, int groups) 
         if (s0 + i < a.n_seqs) {
             const Seq s = seq_of(a, s0 + i);
             p.short_ |= s.n > s.len;
-            sum += steps_of(s, a.tl);
+            sum += units_of(s, a.tl, a.cost);
         }
     sum *= a.c.nkv;
     const int incl = wave_scan(sum);
     p.total = __builtin_amdgcn_readlane(incl, 63);
     p.before = incl - sum;
-    p.groups = max(min(groups, p.total), 1);
+    p.groups = max(min(groups, p.total / kLeast), 1);
     p.base = p.total / p.groups;
     p.more = p.total - p.base * p.groups;
     return p;
@@ -137,9 +140,9 @@ __device__ __forceinline__ int tile_steps(const Seq &s, int tl, int j) {
 
 struct Where {
     Seq s;
-    int seq, kvh, tile, step, steps;
+    int seq, kvh, tile, unit, steps;
 };
-// The tile of step u, and the step within it.
+// The tile of unit u, and the unit within it.
 __device__ __forceinline__ Where find(const PagedPromptArgs &a, const Plan &p, int u) {
     // the last lane that begins at or before u holds it (lanes without steps share their successor's beginning)
     const int lane = lane_id(), L = __popcll(__ballot(p.before <= u)) - 1;
@@ -149,7 +152,7 @@ __device__ __forceinline__ Where find(const PagedPromptArgs &a, const Plan &p, i
     if (p.per > 1) {
         const int s = L * p.per + lane;
         const bool in = lane < p.per && s < a.n_seqs;
-        const int n = in ? steps_of(seq_of(a, s), a.tl) * a.c.nkv : 0;
+        const int n = in ? units_of(seq_of(a, s), a.tl, a.cost) * a.c.nkv : 0;
         const int before = wave_scan(n) - n;
         const int j = __popcll(__ballot(lane < p.per && before <= at)) - 1;
         w.seq = L * p.per + j;
@@ -157,21 +160,21 @@ __device__ __forceinline__ Where find(const PagedPromptArgs &a, const Plan &p, i
     }
     w.seq = __builtin_amdgcn_readfirstlane(w.seq);
     w.s = seq_of(a, w.seq);
-    const int each = steps_of(w.s, a.tl);
+    const int each = units_of(w.s, a.tl, a.cost);
     w.kvh = at / each;
     at -= w.kvh * each;
-    int lo = 0, hi = tiles_of(w.s, a.tl) - 1;  // the last tile that begins at or before the step
+    int lo = 0, hi = tiles_of(w.s, a.tl) - 1;  // the last tile that begins at or before the unit
     while (lo < hi) {
         const int mid = (lo + hi + 1) / 2;
-        if (steps_before(w.s, a.tl, mid) <= at) lo = mid;
+        if (units_before(w.s, a.tl, a.cost, mid) <= at) lo = mid;
         else hi = mid - 1;
     }
     w.tile = lo;
-    w.step = at - steps_before(w.s, a.tl, lo);
+    w.unit = at - units_before(w.s, a.tl, a.cost, lo);
     w.steps = tile_steps(w.s, a.tl, lo);
     return w;
 }
-// The tile after w, from its first step on (there is one).
+// The tile after w, from its first unit on (there is one).
 __device__ __forceinline__ void advance(const PagedPromptArgs &a, Where &w) {
     if (++w.tile == tiles_of(w.s, a.tl)) {
         if (++w.kvh == a.c.nkv) {
@@ -181,7 +184,7 @@ __device__ __forceinline__ void advance(const PagedPromptArgs &a, Where &w) {
         }
         w.tile = max(w.s.n - w.s.len, 0) >> a.tl;  // the first one with a position
     }
-    w.step = 0;
+    w.unit = 0;
     w.steps = tile_steps(w.s, a.tl, w.tile);
 }
 
@@ -238,8 +241,6 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
     const int lane = lane_id(), r = lane & 15, kg = lane >> 4, tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int ps = a.c.ps, psl = 31 - __builtin_clz(ps);
-    // neighbouring shares, which read the same pages, on one XCD
-    const int g = (blockIdx.x & 7) * (kGroups / 8) + (blockIdx.x >> 3);
     // of the lane's words of K (row 16 (r/4) + r%4, word kg) and V (dim r, word 2 kg)
     const uint32_t ka0 = lds_addr(&kt[0][0]) + 16 * k_word<HD>(16 * (r >> 2) + (r & 3), kg);
     const uint32_t va0 = lds_addr(&vt[0][0]) + 16 * v_word(r, 2 * kg);
@@ -261,6 +262,9 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
     v_off += (v_pos & (ps - 1)) * EB;
 
     const Plan plan = make_plan(a, kGroups);
+    // neighbouring shares, which read the same pages, on one XCD; workgroups that go without one behind them
+    const int per_xcd = (plan.groups + 7) / 8;
+    const int g = (int)(blockIdx.x >> 3) < per_xcd ? (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3) : blockIdx.x;
     int at = first_of(plan, g);
     const int end = first_of(plan, g + 1);
     if (tid == 0) {
@@ -281,7 +285,13 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
     Where w;
     if (at < end) w = find(a, plan, at);
     while (at < end) {
-        const int n = min(end - at, w.steps - w.step);
+        const int units = min(end - at, w.steps + a.cost - w.unit);
+        const int step = max(w.unit - a.cost, 0), n = max(w.unit + units - a.cost, 0) - step;
+        if (n == 0) {  // none of its steps: the next workgroup begins it
+            at += units;
+            if (at < end) advance(a, w);
+            continue;
+        }
         const int tok0 = w.tile << a.tl, toks = min(1 << a.tl, w.s.n - tok0);
         const int *table = a.table + (size_t)w.seq * a.max_pages;
         const int pos0 = w.s.len - w.s.n + tok0;  // of the tile's first token
@@ -341,7 +351,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
             }
         };
 
-        int p0 = w.step * kStep, b = 0;
+        int p0 = step * kStep, b = 0;
         const int p_end = p0 + n * kStep;
         int ent = entry(p0), ent_next = entry(p0 + kStep);
         lds_barrier();  // the buffers are free
@@ -412,28 +422,32 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
                 // V past the end, or ahead of a row, may be no number, which a weight of 0 does not hide: it becomes 0.
                 // What is there and no number is noted, for the rows that do see it.
                 const int p = v_pos, in = (int)((there >> p) & 255);
-                const bool ahead = p0 >= odd0;  // else all rows see what is there
+                u4 keep;
+#pragma unroll
+                for (int j = 0; j < 4; j++) keep[j] = (in >> (2 * j) & 1 ? 0xffffu : 0u) | (in >> (2 * j + 1) & 1 ? 0xffff0000u : 0u);
                 uint32_t sum = 0;  // bit 15 of a half: an exponent of all ones is among them
 #pragma unroll
                 for (int i = 0; i < NL; i++) {
-                    const u4 v = vt[b][i * kThreads + tid];
+                    const u4 v = vt[b][i * kThreads + tid] & keep;
+                    if (in != 255) vt[b][i * kThreads + tid] = v;
 #pragma unroll
                     for (int j = 0; j < 4; j++) sum |= (v[j] & 0x7fff7fffu) + 0x04000400u;
                 }
-                if (in != 255 || (ahead && (sum & 0x80008000u))) {
+                if (p0 >= odd0 && (sum & 0x80008000u)) {  // (before odd0 all rows see what is there)
                     uint32_t bad = 0;
                     for (int i = 0; i < NL; i++) {
                         u4 v = vt[b][i * kThreads + tid];
 #pragma unroll
                         for (int j = 0; j < 8; j++) {
                             const uint32_t inf = 0x7c00u << (16 * (j & 1));
-                            const bool none = ahead && (v[j / 2] & inf) == inf;
-                            if (none || !(in >> j & 1)) v[j / 2] &= ~(0xffffu << (16 * (j & 1)));
-                            if (none && (in >> j & 1)) bad |= 1u << j;
+                            if ((v[j / 2] & inf) == inf) {
+                                v[j / 2] &= ~(0xffffu << (16 * (j & 1)));
+                                bad |= 1u << j;
+                            }
                         }
                         vt[b][i * kThreads + tid] = v;
                     }
-                    if (bad) atomicOr(&odd[(p0 - odd0 + p) >> 5], bad << (p & 31));
+                    atomicOr(&odd[(p0 - odd0 + p) >> 5], bad << (p & 31));
                 }
                 lds_barrier();
             }
@@ -464,6 +478,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
             for (int k = 0; k < 2; k++) {
                 constexpr int per_half = CK + CV;
                 // S^T: lane: row r, positions p0 + first + 4t + i
+                __builtin_amdgcn_s_setprio(1);  // the SIMD's other wave forms its weights meanwhile
                 const int first = 16 * kg + 8 * k;
                 f4 s[RT][2] = {};
 #pragma unroll
@@ -483,6 +498,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
                     }
                 }
                 read_v(k, 0, (k * per_half + CK) & 1);
+                __builtin_amdgcn_s_setprio(0);
                 // weights
                 h8 phi[RT], plo[RT];
 #pragma unroll
@@ -545,6 +561,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
                         plo[rt][j + 1] = x.lo[1];
                     }
                 }
+                __builtin_amdgcn_s_setprio(1);
                 // O^T
 #pragma unroll
                 for (int n = 0; n < CV; n++) {
@@ -581,7 +598,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
                         }
                 }
         }
-        const bool begins = w.step == 0, finishes = w.step + n == w.steps;
+        const bool begins = step == 0, finishes = step + n == w.steps;
         float *part = a.ws + (size_t)(2 * g + begins) * part_floats(HD);
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
@@ -607,10 +624,10 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
             }
         }
         if (tid == 0) {
-            if (!begins) taken_of(a)[g] = at - w.step;
-            else if (!finishes) begun_of(a)[g] = {at, w.s.start + tok0, toks * a.gqa, w.kvh};
+            if (!begins) taken_of(a)[g] = at - w.unit;
+            else if (!finishes) begun_of(a)[g] = {at - w.unit, w.s.start + tok0, toks * a.gqa, w.kvh};
         }
-        at += n;
+        at += units;
         if (at < end) advance(a, w);
     }
 
@@ -625,15 +642,15 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
 }
 
 // Merges the partials of the tile that begins in workgroup blockIdx.x's share and goes on behind it.  256 threads are
-// HD / 4 lanes of four dims, times 4 rows (blockIdx.y: which), times threads that divide the partials among them.
+// HD / 4 lanes of four dims, times threads that divide the partials among them where there are many, times rows;
+// blockIdx.y: which 4 rows.
 template <int HD>
 __global__ void __launch_bounds__(256) paged_prompt_merge_kernel(PagedPromptArgs a) {
-    constexpr int kGroups = groups_of(HD), D4 = HD / 4, ROWS = 4, CHAIN = 256 / (D4 * ROWS) > 0 ? 256 / (D4 * ROWS) : 1;
-    constexpr int ROW_PASS = 256 / (D4 * CHAIN);  // rows at once
-    __shared__ __align__(16) float so[CHAIN][ROW_PASS][HD];
-    __shared__ float sm[CHAIN][ROW_PASS], sl[CHAIN][ROW_PASS];
+    constexpr int kGroups = groups_of(HD), D4 = HD / 4, PARTS = 256 / D4;
+    __shared__ __align__(16) float so[PARTS][HD];
+    __shared__ float sm[PARTS], sl[PARTS];
     const Begun b = begun_of(a)[blockIdx.x];
-    if (b.first < 0 || ROWS * (int)blockIdx.y >= b.n_rows) return;
+    if (b.first < 0 || 4 * (int)blockIdx.y >= b.n_rows) return;
     const int *taken = taken_of(a);
     int n = 1;
     for (int g0 = blockIdx.x + 1; g0 < kGroups; g0 += 64) {  // workgroups that go on with it, one after another
@@ -645,22 +662,26 @@ __global__ void __launch_bounds__(256) paged_prompt_merge_kernel(PagedPromptArgs
     }
     // partial i: the second of workgroup blockIdx.x, then the first of each that follows
     auto part = [&](int i) { return a.ws + (size_t)(2 * (blockIdx.x + i) + (i == 0)) * part_floats(HD); };
-    const int d = 4 * (threadIdx.x % D4), c = threadIdx.x / D4 % CHAIN, rr = threadIdx.x / (D4 * CHAIN);
-    for (int r0 = 0; r0 < ROWS; r0 += ROW_PASS) {
-        const int row = ROWS * blockIdx.y + r0 + rr;
-        const int in = min(row, b.n_rows - 1);
+    // few partials: 16 rows by every fourth workgroup; many: 4 rows, by threads that divide the partials
+    const bool few = n <= 4;
+    if (few && blockIdx.y & 3) return;
+    const int chain = few ? 1 : PARTS < 4 ? 1 : PARTS / 4, per_pass = PARTS / chain;  // threads per word, rows at once
+    const int d = 4 * (threadIdx.x % D4), slot = threadIdx.x / D4, c = slot % chain, rr = slot / chain;
+    const int rows = min(few ? 16 : 4, b.n_rows - 4 * (int)blockIdx.y);
+    for (int r0 = 0; r0 < rows; r0 += per_pass) {
+        const int row = 4 * blockIdx.y + min(r0 + rr, rows - 1);
         float m = -INFINITY, l = 0.0f;
         f4 x = {};
-        for (int i0 = c; i0 < n; i0 += 4 * CHAIN) {  // four loads in flight
+        for (int i0 = c; i0 < n; i0 += 4 * chain) {  // four loads in flight
             float pm[4], pl[4];
             f4 y[4];
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                const float *p = part(min(i0 + u * CHAIN, n - 1));
-                pm[u] = p[in];
-                pl[u] = p[kRows + in];
-                __builtin_memcpy(&y[u], p + 2 * kRows + (size_t)in * HD + d, 16);
-                if (i0 + u * CHAIN >= n) {
+                const float *p = part(min(i0 + u * chain, n - 1));
+                pm[u] = p[row];
+                pl[u] = p[kRows + row];
+                __builtin_memcpy(&y[u], p + 2 * kRows + (size_t)row * HD + d, 16);
+                if (i0 + u * chain >= n) {
                     pm[u] = -INFINITY;
                     pl[u] = 0.0f;
                     y[u] = f4{0.f, 0.f, 0.f, 0.f};
@@ -680,32 +701,27 @@ __global__ void __launch_bounds__(256) paged_prompt_merge_kernel(PagedPromptArgs
             }
             m = mn;
         }
-        if (CHAIN > 1) {
-            __syncthreads();
-            __builtin_memcpy(&so[c][rr][d], &x, 16);
+        if (chain > 1) {  // (one pass)
+            __builtin_memcpy(&so[slot][d], &x, 16);
             if (d == 0) {
-                sm[c][rr] = m;
-                sl[c][rr] = l;
+                sm[slot] = m;
+                sl[slot] = l;
             }
             __syncthreads();
-            if (c == 0) {
-                float mn = m;
-#pragma unroll
-                for (int i = 1; i < CHAIN; i++) mn = fmaxf(mn, sm[i][rr]);
-                f4 sum = {};
-                l = 0.0f;
-#pragma unroll
-                for (int i = 0; i < CHAIN; i++) {
-                    const float f = mn == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[i][rr] - mn);
-                    f4 y;
-                    __builtin_memcpy(&y, &so[i][rr][d], 16);
-                    sum += y * f;
-                    l = fmaf(sl[i][rr], f, l);
-                }
-                x = sum;
+            if (c > 0) continue;
+            float mn = m;
+            for (int i = 1; i < chain; i++) mn = fmaxf(mn, sm[slot + i]);
+            x = f4{0.f, 0.f, 0.f, 0.f};
+            l = 0.0f;
+            for (int i = 0; i < chain; i++) {
+                const float f = mn == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[slot + i] - mn);
+                f4 y;
+                __builtin_memcpy(&y, &so[slot + i][d], 16);
+                x += y * f;
+                l = fmaf(sl[slot + i], f, l);
             }
         }
-        if (c == 0 && row < b.n_rows) {
+        if (r0 + rr < rows) {
             x *= l == 0.0f ? 0.0f : 1.0f / l;
             const int tok = row / a.gqa, head = row - tok * a.gqa;
             __builtin_memcpy(a.out + ((size_t)(b.row0 + tok) * a.nh + b.kvh * a.gqa + head) * HD + d, &x, 16);
@@ -731,6 +747,9 @@ int launch_paged_prompt(PagedPromptArgs a, hipStream_t s) {
     // tokens of a tile: a power of two, whose rows fill the tile as far as they can
     a.tl = 0;
     while ((2 << a.tl) * a.gqa <= kRows) a.tl++;
+    // 4096 tokens of 32 heads of 256 take 527 us at 2, 492 at 3; of 64 heads of 128, int8, 631 and 639, of 12 of 64, mixed, 33.4
+    // and 34.1 (2000 of 64 heads of 128: 239 with none)
+    a.cost = a.c.hd == 256 ? 3 : 2;
     if (a.c.kv_type == kKvF16)
         return a.c.hd == 64 ? launch_shape<kKvF16, 64>(a, s) : a.c.hd == 128 ? launch_shape<kKvF16, 128>(a, s)
                                                                               : launch_shape<kKvF16, 256>(a, s);
