@@ -9,7 +9,7 @@
 // z as a whole number that orders as z does, over the complement of the index.  Few tokens get so far as to be
 // looked at: a thread compares the largest of its 16 logits with the workgroup's n-th best so far.  Lists are
 // merged as two halves of a bitonic sequence.
-// Rows are cut into parts where they are few; a second launch joins the parts.
+// Rows are cut into parts where they do not fill the chip; a second launch joins the parts.
 #include <float.h>
 #include <math.h>
 
@@ -25,17 +25,19 @@ constexpr int kLpWords = 4;                           // words of four logits pe
 constexpr int kLpStep = 4 * kLpThreads * kLpWords;    // logits of a step
 constexpr float kLpLog2e = 1.44269504088896341f;
 
+// Rows 0 .. whole-1 are done by a workgroup each, the others in parts of per_part logits, which a second launch joins.
+struct LpPlan {
+    int whole, parts, per_part;
+};
 struct LpSums {
     float m, S, T;  // m is at least -FLT_MAX: a row without any number has S = 0
     int before;     // tokens before the target
 };
 
-// what d = m - (larger m) turns S and T into
-__device__ __forceinline__ void lp_rescale(double &S, double &T, double d) {
-    const double f = exp(d);
-    T = f * (T + S * fmax(d, -1e30));
-    S = f * S;
-}
+template <int O>
+struct Lane {
+    static constexpr int value = O;
+};
 
 __device__ __forceinline__ uint32_t order32(float v) {
     const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f);  // one zero
@@ -50,35 +52,55 @@ __device__ __forceinline__ uint64_t lane64(uint64_t v, int l) {
     const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, l), hi = __builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), l);
     return (uint64_t)hi << 32 | lo;
 }
-__device__ __forceinline__ uint64_t xor64(uint64_t v, int o) { return __shfl_xor((unsigned long long)v, o); }
+// v of lane ^ O
+template <int O>
+__device__ __forceinline__ uint32_t xor_lanes(uint32_t v) {
+    if (O == 32 || O == 16) {
+        // the swap leaves the lower (even) rows' values everywhere in one register, the upper ones' in the other
+        const auto p = O == 32 ? __builtin_amdgcn_permlane32_swap(v, v, false, false) : __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return lane_id() & O ? p[0] : p[1];
+    }
+    if (O == 8) return __builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xF, 0xF, false);  // row_ror:8
+    if (O == 4) {  // ^7, then ^3
+        const int h = __builtin_amdgcn_update_dpp(0, (int)v, kDppRowHalfMirror, 0xF, 0xF, false);
+        return __builtin_amdgcn_update_dpp(0, h, 0x1B, 0xF, 0xF, false);
+    }
+    return __builtin_amdgcn_update_dpp(0, (int)v, O == 2 ? kDppXor2 : kDppXor1, 0xF, 0xF, false);
+}
+template <int O>
+__device__ __forceinline__ uint64_t xor64(uint64_t v) {
+    return (uint64_t)xor_lanes<O>((uint32_t)(v >> 32)) << 32 | xor_lanes<O>((uint32_t)v);
+}
+template <int O>
+__device__ __forceinline__ double xor_double(double v) { return __builtin_bit_cast(double, xor64<O>(__builtin_bit_cast(uint64_t, v))); }
 
-// One step of a sorting network: lanes whose bit o is clear take the larger where `down` is set.
-__device__ __forceinline__ uint64_t lp_exchange(uint64_t v, int o, bool down) {
-    const uint64_t w = xor64(v, o);
-    const bool larger = ((lane_id() & o) == 0) == down;
+// One step of a sorting network: lanes whose bit O is clear take the larger where `down` is set.
+template <int O>
+__device__ __forceinline__ uint64_t lp_exchange(uint64_t v, bool down) {
+    const uint64_t w = xor64<O>(v);
+    const bool larger = ((lane_id() & O) == 0) == down;
     return (v > w) == larger ? v : w;
 }
-// a bitonic sequence, sorted falling
-__device__ __forceinline__ uint64_t lp_merge(uint64_t v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = lp_exchange(v, o, true);
+// a bitonic sequence of 2 O lanes, sorted
+template <int O>
+__device__ __forceinline__ uint64_t lp_merge(uint64_t v, bool down) {
+    v = lp_exchange<O>(v, down);
+    if constexpr (O > 1) v = lp_merge<O / 2>(v, down);
     return v;
 }
-__device__ __forceinline__ uint64_t lp_sort(uint64_t v) {
-#pragma unroll
-    for (int n = 2; n <= 64; n <<= 1)
-#pragma unroll
-        for (int o = n >> 1; o > 0; o >>= 1) v = lp_exchange(v, o, (lane_id() & n) == 0 || n == 64);
-    return v;
+template <int N>
+__device__ __forceinline__ uint64_t lp_sort(uint64_t v) {  // runs of N lanes, falling and rising in turn
+    if constexpr (N > 2) v = lp_sort<N / 2>(v);
+    return lp_merge<N / 2>(v, N == 64 || (lane_id() & N) == 0);
 }
 // the 64 largest of two lists, sorted
 __device__ __forceinline__ uint64_t lp_join(uint64_t a, uint64_t b) {
     const uint64_t r = __shfl((unsigned long long)b, 63 - lane_id());
-    return lp_merge(a > r ? a : r);
+    return lp_merge<32>(a > r ? a : r, true);
 }
 
 // What is known of a row goes out (wave 0): list is sorted.
-__device__ __forceinline__ void lp_finish(const LogprobsArgs &a, int r, double m, double S, double T, int before, float zt,
+__device__ __forceinline__ void lp_finish(const LogprobsArgs &a, int r, float m, double S, double T, int before, float zt,
                                           int t, uint64_t list) {
     const int lane = lane_id();
     const double logS = log(S);
@@ -86,7 +108,7 @@ __device__ __forceinline__ void lp_finish(const LogprobsArgs &a, int r, double m
     if (lane == 0) {
         if (a.targets) {
             const bool in = (unsigned)t < (unsigned)a.vocab;
-            float lp = (float)((double)zt - m - logS);
+            float lp = (float)((double)zt - (double)m - logS);
             if (none) lp = -INFINITY;
             if (bad) lp = NAN;
             a.logp[r] = in ? lp : 0.0f;
@@ -98,34 +120,44 @@ __device__ __forceinline__ void lp_finish(const LogprobsArgs &a, int r, double m
         const float z = unorder32((uint32_t)(list >> 32));
         const bool is = list != 0 && z > -INFINITY && !bad;
         a.ids[(size_t)r * a.k + lane] = is ? (int)(0xffffffffu - (uint32_t)list) : -1;
-        a.tops[(size_t)r * a.k + lane] = bad ? NAN : is ? (float)((double)z - m - logS) : -INFINITY;
+        a.tops[(size_t)r * a.k + lane] = bad ? NAN : is ? (float)((double)z - (double)m - logS) : -INFINITY;
     }
 }
 
-// sums over the wave, in every lane
-__device__ __forceinline__ void lp_join_lanes(double &m, double &S, double &T, int &before) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const double m2 = __shfl_xor(m, o);
-        double S2 = __shfl_xor(S, o), T2 = __shfl_xor(T, o);
-        before += __shfl_xor(before, o);
-        const double mn = fmax(m, m2);
-        if (m < mn) lp_rescale(S, T, m - mn);
-        if (m2 < mn) lp_rescale(S2, T2, m2 - mn);
-        m = mn;
-        S += S2;
-        T += T2;
+// The lanes' sums joined, in every lane: all relative to the largest m, then added.
+__device__ __forceinline__ void lp_join_lanes(float &m, double &S, double &T, int &before) {
+    float M = max16(m);
+    M = fmaxf(M, __builtin_bit_cast(float, xor_lanes<16>(__builtin_bit_cast(uint32_t, M))));
+    M = fmaxf(M, __builtin_bit_cast(float, xor_lanes<32>(__builtin_bit_cast(uint32_t, M))));
+    if (m < M) {
+        const double d = (double)m - (double)M, f = exp(d);
+        T = f * (T + S * fmax(d, -1e30));
+        S *= f;
     }
+    m = M;
+    auto add = [&](auto o) {
+        constexpr int O = decltype(o)::value;
+        S += xor_double<O>(S);
+        T += xor_double<O>(T);
+        before += (int)xor_lanes<O>((uint32_t)before);
+    };
+    add(Lane<1>{});
+    add(Lane<2>{});
+    add(Lane<4>{});
+    add(Lane<8>{});
+    add(Lane<16>{});
+    add(Lane<32>{});
 }
 
 template <bool TOP>
-__global__ void __launch_bounds__(kLpThreads) logprobs_kernel(LogprobsArgs a, int per_part) {
+__global__ void __launch_bounds__(kLpThreads) logprobs_kernel(LogprobsArgs a, LpPlan p) {
     __shared__ uint64_t lists[TOP ? kLpWaves : 1][64];
     __shared__ LpSums sums[kLpWaves];
     __shared__ uint32_t floor_;  // the best of the waves' n-th best so far (as order32)
-    const int r = blockIdx.y, part = blockIdx.x, tid = threadIdx.x, lane = lane_id(), wave = tid >> 6;
+    const int cut = (int)blockIdx.x - p.whole;  // of the rows that are cut: row and part
+    const int r = cut < 0 ? (int)blockIdx.x : p.whole + cut / p.parts, part = cut < 0 ? 0 : cut % p.parts, tid = threadIdx.x, lane = lane_id(), wave = tid >> 6;
     const float *z = a.z + (size_t)r * a.vocab;
-    const int from = part * per_part, to = min(a.vocab, from + per_part);
+    const int from = part * p.per_part, to = cut < 0 ? a.vocab : min(a.vocab, from + p.per_part);
     if (TOP && tid == 0) floor_ = 0;
 
     const int t = a.targets ? a.targets[r] : -1;
@@ -200,7 +232,7 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(LogprobsArgs a, in
                         const uint64_t c = lp_key(y[g][j], first + 4 * kLpThreads * g + j);
                         own = c > own ? c : own;
                     }
-                list = lp_sort(own);
+                list = lp_sort<64>(own);
                 least = unorder32((uint32_t)(lane64(list, a.k - 1) >> 32));
             }
             const uint32_t known = *(volatile uint32_t *)&floor_;
@@ -229,41 +261,40 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(LogprobsArgs a, in
             }
         }
     }
-    double m = s.m, S = s.S, T = s.T;
+    float m = s.m;
+    double S = s.S, T = s.T;
     int before = s.before;
     lp_join_lanes(m, S, T, before);
-    if (lane == 0) sums[wave] = {(float)m, (float)S, (float)T, before};
+    if (lane == 0) sums[wave] = {m, (float)S, (float)T, before};
     if (TOP) lists[wave][lane] = list;
     __syncthreads();
     if (wave != 0) return;
-    const LpSums p = sums[lane & (kLpWaves - 1)];
-    m = p.m;
-    S = lane < kLpWaves ? p.S : 0.0f;
-    T = lane < kLpWaves ? p.T : 0.0f;
-    before = lane < kLpWaves ? p.before : 0;
+    const LpSums q = sums[lane & (kLpWaves - 1)];
+    m = q.m;
+    S = lane < kLpWaves ? q.S : 0.0f;
+    T = lane < kLpWaves ? q.T : 0.0f;
+    before = lane < kLpWaves ? q.before : 0;
     lp_join_lanes(m, S, T, before);
     if (TOP)
         for (int w = 1; w < kLpWaves; w++) list = lp_join(list, lists[w][lane]);
-    if (gridDim.x == 1) lp_finish(a, r, m, S, T, before, zt, t, list);
+    if (cut < 0) lp_finish(a, r, m, S, T, before, zt, t, list);
     else {
-        const size_t at = (size_t)r * gridDim.x + part;
-        if (lane == 0) ((LpSums *)a.ws)[at] = {(float)m, (float)S, (float)T, before};
-        if (TOP && lane < a.k)
-            ((uint64_t *)((LpSums *)a.ws + (size_t)a.n_rows * gridDim.x))[at * a.k + lane] = list;
+        if (lane == 0) ((LpSums *)a.ws)[cut] = {m, (float)S, (float)T, before};
+        if (TOP && lane < a.k) ((uint64_t *)((LpSums *)a.ws + (size_t)(a.n_rows - p.whole) * p.parts))[(size_t)cut * a.k + lane] = list;
     }
 }
 
-// Joins the parts (at most 64) of row blockIdx.x: wave w of 16 the lists of parts w, w + 16, ...
+// Joins the parts (at most 64) of the cut row blockIdx.x: wave w of 16 the lists of parts w, w + 16, ...
 template <bool TOP>
-__global__ void __launch_bounds__(TOP ? 1024 : 64) logprobs_join_kernel(LogprobsArgs a, int parts) {
+__global__ void __launch_bounds__(TOP ? 1024 : 64) logprobs_join_kernel(LogprobsArgs a, LpPlan p) {
     __shared__ uint64_t lists[TOP ? 16 : 1][64];
-    const int r = blockIdx.x, lane = lane_id(), wave = threadIdx.x >> 6;
+    const int cut = blockIdx.x, r = p.whole + cut, parts = p.parts, lane = lane_id(), wave = threadIdx.x >> 6;
     uint64_t list = 0;
     if (TOP) {
-        const uint64_t *l = (const uint64_t *)((const LpSums *)a.ws + (size_t)a.n_rows * parts) + (size_t)r * parts * a.k;
-        for (int p = wave; p < parts; p += 16) {
-            const uint64_t one = lane < a.k ? l[(size_t)p * a.k + lane] : 0;
-            list = p == wave ? one : lp_join(list, one);
+        const uint64_t *l = (const uint64_t *)((const LpSums *)a.ws + (size_t)(a.n_rows - p.whole) * parts) + (size_t)cut * parts * a.k;
+        for (int i = wave; i < parts; i += 16) {
+            const uint64_t one = lane < a.k ? l[(size_t)i * a.k + lane] : 0;
+            list = i == wave ? one : lp_join(list, one);
         }
         for (int half = 8; half > 0; half >>= 1) {
             if (wave >= half) lists[wave][lane] = list;
@@ -272,41 +303,48 @@ __global__ void __launch_bounds__(TOP ? 1024 : 64) logprobs_join_kernel(Logprobs
         }
     }
     if (wave != 0) return;
-    const LpSums p = lane < parts ? ((const LpSums *)a.ws)[(size_t)r * parts + lane] : LpSums{-FLT_MAX, 0.0f, 0.0f, 0};
-    double m = p.m, S = p.S, T = p.T;
-    int before = p.before;
+    const LpSums q = lane < parts ? ((const LpSums *)a.ws)[(size_t)cut * parts + lane] : LpSums{-FLT_MAX, 0.0f, 0.0f, 0};
+    float m = q.m;
+    double S = q.S, T = q.T;
+    int before = q.before;
     lp_join_lanes(m, S, T, before);
     const int t = a.targets ? a.targets[r] : -1;
     const float zt = (unsigned)t < (unsigned)a.vocab ? a.z[(size_t)r * a.vocab + t] : 0.0f;
     lp_finish(a, r, m, S, T, before, zt, t, list);
 }
 
-// Parts of a row: enough for four workgroups a CU, each at least a step.
-static int lp_parts(int n_rows, int vocab, int *per_part) {
+// 1024 workgroups, four a CU, are at work at once: as many rows as fill them once or more are done whole, the others
+// (all, where there are fewer) are cut into parts of at least a step, so that they fill them too.
+static LpPlan lp_plan(int n_rows, int vocab) {
+    LpPlan p;
+    p.whole = n_rows / 1024 * 1024;
+    const int rest = n_rows - p.whole;
     const long long steps = ((long long)vocab + kLpStep - 1) / kLpStep;
-    long long parts = steps < 64 ? steps : 64;
-    if (parts * n_rows > 1024) parts = 1024 / n_rows > 1 ? 1024 / n_rows : 1;
+    long long parts = rest ? 1024 / rest : 1;
+    if (parts > 64) parts = 64;
+    if (parts > steps) parts = steps;
     const long long per = (steps + parts - 1) / parts;
-    *per_part = (int)(per * kLpStep < vocab ? per * kLpStep : vocab);
-    return (int)((steps + per - 1) / per);
+    p.parts = (int)((steps + per - 1) / per);
+    p.per_part = (int)(per * kLpStep < vocab ? per * kLpStep : vocab);
+    if (p.parts == 1) p.whole = n_rows;
+    return p;
 }
 
 size_t logprobs_workspace_bytes(int n_rows, int vocab, int k) {
-    int per;
-    const int parts = lp_parts(n_rows, vocab, &per);
-    return parts == 1 ? 16 : (size_t)n_rows * parts * (sizeof(LpSums) + (size_t)k * 8);
+    const LpPlan p = lp_plan(n_rows, vocab);
+    return p.whole == n_rows ? 16 : (size_t)(n_rows - p.whole) * p.parts * (sizeof(LpSums) + (size_t)k * 8);
 }
 
 int launch_logprobs(const LogprobsArgs &a, hipStream_t s) {
-    int per;
-    const int parts = lp_parts(a.n_rows, a.vocab, &per);
-    const dim3 grid(parts, a.n_rows), block(kLpThreads);
-    if (a.k) hipLaunchKernelGGL(logprobs_kernel<true>, grid, block, 0, s, a, per);
-    else hipLaunchKernelGGL(logprobs_kernel<false>, grid, block, 0, s, a, per);
+    const LpPlan p = lp_plan(a.n_rows, a.vocab);
+    const int rest = a.n_rows - p.whole;
+    const dim3 grid(p.whole + rest * p.parts), block(kLpThreads);
+    if (a.k) hipLaunchKernelGGL(logprobs_kernel<true>, grid, block, 0, s, a, p);
+    else hipLaunchKernelGGL(logprobs_kernel<false>, grid, block, 0, s, a, p);
     if (int rc = check_launch("logprobs")) return rc;
-    if (parts == 1) return kOk;
-    if (a.k) hipLaunchKernelGGL(logprobs_join_kernel<true>, dim3(a.n_rows), dim3(1024), 0, s, a, parts);
-    else hipLaunchKernelGGL(logprobs_join_kernel<false>, dim3(a.n_rows), dim3(64), 0, s, a, parts);
+    if (rest == 0) return kOk;
+    if (a.k) hipLaunchKernelGGL(logprobs_join_kernel<true>, dim3(rest), dim3(1024), 0, s, a, p);
+    else hipLaunchKernelGGL(logprobs_join_kernel<false>, dim3(rest), dim3(64), 0, s, a, p);
     return check_launch("logprobs");
 }
 
