@@ -19,6 +19,7 @@
 namespace mnemo {
 
 typedef float lpf4 __attribute__((ext_vector_type(4)));
+typedef lpf4 lpf4u __attribute__((aligned(4)));
 
 constexpr int kLpThreads = 256, kLpWaves = kLpThreads / 64;
 constexpr int kLpWords = 4;                           // words of four logits per thread and step
@@ -168,7 +169,7 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(LogprobsArgs a, Lp
 #pragma unroll
         for (int g = 0; g < kLpWords; g++) {
             const int i = at + 4 * (kLpThreads * g + tid);
-            if (i + 3 < to) __builtin_memcpy(&x[g], z + i, 16);
+            if (i + 3 < to) x[g] = __builtin_nontemporal_load((const lpf4u *)(z + i));
             else
                 for (int j = 0; j < 4; j++) x[g][j] = i + j < to ? z[i + j] : -INFINITY;
         }

@@ -21,9 +21,9 @@
 namespace mnemo {
 
 constexpr int kLoTile = 16;     // tokens
-constexpr int kLoWaves = 4, kLoThreads = 64 * kLoWaves;
-constexpr int kLoChunk = 256;   // of K, per wave and pass
-constexpr int kLoStep = kLoChunk * kLoWaves;
+constexpr int kLoShrinkWaves = 8, kLoExpandWaves = 4;
+constexpr int kLoChunk = 128, kLoSteps = kLoChunk / 32;  // of K, per wave and pass
+constexpr int kLoStep = kLoChunk * kLoShrinkWaves;
 constexpr int kLoMaxParts = 8;
 
 // The values of a token's operand (lane: token lane % 16), and what a matrix instruction makes of them.
@@ -85,9 +85,10 @@ __device__ __forceinline__ int lo_ids(const LoraArgs &a, int t0, uint32_t &first
 
 // parts[kb][t][r] = sum over part kb of K of A_a[r][k] x_t[k].  NR: tiles of 16 ranks.
 template <bool BF, int NR>
-__global__ void __launch_bounds__(kLoThreads) lora_shrink_kernel(LoraArgs a, int per_part) {
-    __shared__ __align__(16) float red[kLoWaves][kLoTile][16 * NR + 4];
-    const int lane = lane_id(), c = lane & 15, kg = lane >> 4, wave = threadIdx.x >> 6;
+__global__ void __launch_bounds__(64 * kLoShrinkWaves, NR <= 4 ? 4 : 2) lora_shrink_kernel(LoraArgs a, int per_part) {
+    constexpr int kThreads = 64 * kLoShrinkWaves;
+    __shared__ __align__(16) float red[kLoShrinkWaves][kLoTile][16 * NR + 4];
+    const int lane = lane_id(), c = lane & 15, kg = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int t0 = blockIdx.y * kLoTile, kb = blockIdx.x;
     const int k_from = kb * per_part, k_to = min(a.K, k_from + per_part);
     uint32_t firsts;
@@ -103,33 +104,30 @@ __global__ void __launch_bounds__(kLoThreads) lora_shrink_kernel(LoraArgs a, int
         f4 acc[NR] = {};
         int e = -127;
         for (int k0 = k_from + wave * kLoChunk; k0 < k_to; k0 += kLoStep) {
-            float v[8][8];
+            float v[kLoSteps][8];
             float largest = 0.0f;
 #pragma unroll
-            for (int st = 0; st < 8; st++) {
-                const int k = k0 + 32 * st + 8 * kg;
-                if (k < k_to) {  // K is a multiple of 8
+            for (int st = 0; st < kLoSteps; st++) {
+                const int k = k0 + 32 * st + 8 * kg;  // K is a multiple of 8
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[st][j] = 0.0f;
+                if (id == ad && k < k_to) {
                     __builtin_memcpy(&v[st][0], x + k, 16);
                     __builtin_memcpy(&v[st][4], x + k + 4, 16);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) v[st][j] = 0.0f;
                 }
             }
-            u4 w[8];
+            u4 w[2][kLoSteps];  // of a tile of ranks and of the next
             auto load = [&](int t) {
-                const int r = 16 * t + c;
+                // (no branches: rows behind the rank, whose sums are dropped, and words behind K, which meet zeros in x, are others')
+                const uint16_t *row = A + (size_t)min(16 * t + c, rank - 1) * a.K;
 #pragma unroll
-                for (int st = 0; st < 8; st++) {
-                    const int k = k0 + 32 * st + 8 * kg;
-                    w[st] = u4{0, 0, 0, 0};
-                    if (r < rank && k < k_to) __builtin_memcpy(&w[st], A + (size_t)r * a.K + k, 16);
-                }
+                for (int st = 0; st < kLoSteps; st++) __builtin_memcpy(&w[t & 1][st], row + min(k0 + 32 * st + 8 * kg, a.K - 8), 16);
             };
             load(0);
+            if (NR > 1) load(1);
             if (!BF) {
 #pragma unroll
-                for (int st = 0; st < 8; st++)
+                for (int st = 0; st < kLoSteps; st++)
 #pragma unroll
                     for (int j = 0; j < 8; j++) largest = fmaxf(largest, fabsf(v[st][j]));
                 const int en = max(e, lo_exponent(largest));
@@ -141,15 +139,16 @@ __global__ void __launch_bounds__(kLoThreads) lora_shrink_kernel(LoraArgs a, int
                     e = en;
                 }
             }
-            LoOperand<BF> o[8];
+            LoOperand<BF> o[kLoSteps];
 #pragma unroll
-            for (int st = 0; st < 8; st++) o[st].set(v[st], e);
+            for (int st = 0; st < kLoSteps; st++) o[st].set(v[st], e);
 #pragma unroll
             for (int t = 0; t < NR; t++) {
-                if (16 * t >= rank) break;
-                if (t > 0) load(t);
+                if (16 * t < rank) {
 #pragma unroll
-                for (int st = 0; st < 8; st++) acc[t] = o[st].mul(w[st], acc[t]);
+                    for (int st = 0; st < kLoSteps; st++) acc[t] = o[st].mul(w[t & 1][st], acc[t]);
+                    if (t + 2 < NR) load(t + 2);
+                }
             }
         }
         // the waves' sums are added
@@ -163,28 +162,38 @@ __global__ void __launch_bounds__(kLoThreads) lora_shrink_kernel(LoraArgs a, int
             __builtin_memcpy(&red[wave][c][16 * t + 4 * kg], &y, 16);
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < kLoTile * rank; i += kLoThreads) {
+        for (int i = threadIdx.x; i < kLoTile * rank; i += kThreads) {
             const int t = i / rank, r = i - t * rank;
             // (t is no lane's own token here)
-            if (t0 + t < a.n_tokens && a.ids[t0 + t] == ad)
-                a.ws[((size_t)kb * a.n_tokens + t0 + t) * a.max_rank + r] =
-                    (red[0][t][r] + red[1][t][r]) + (red[2][t][r] + red[3][t][r]);
+            if (t0 + t < a.n_tokens && a.ids[t0 + t] == ad) {
+                float y[kLoShrinkWaves];
+#pragma unroll
+                for (int w = 0; w < kLoShrinkWaves; w++) y[w] = red[w][t][r];
+#pragma unroll
+                for (int n = kLoShrinkWaves / 2; n > 0; n /= 2)
+#pragma unroll
+                    for (int w = 0; w < n; w++) y[w] += y[w + n];
+                a.ws[((size_t)kb * a.n_tokens + t0 + t) * a.max_rank + r] = y[0];
+            }
         }
     }
 }
 
 // out_t[m] = base_t[m] + scale sum_r B_a[m][r] v_t[r].  NS: steps of 32 ranks.  A wave has per_wave outputs.
 template <bool BF, int NS>
-__global__ void __launch_bounds__(kLoThreads) lora_expand_kernel(LoraArgs a, int parts, int per_wave) {
+__global__ void __launch_bounds__(64 * kLoExpandWaves, NS <= 4 ? 4 : 2) lora_expand_kernel(LoraArgs a, int parts, int per_wave) {
+    __shared__ __align__(16) float vs[kLoTile][32 * NS + 4];
+    __shared__ int ids[kLoTile];
     constexpr int U = NS <= 2 ? 4 : 1;  // tiles of 16 outputs at once
-    const int lane = lane_id(), c = lane & 15, kg = lane >> 4, wave = threadIdx.x >> 6;
+    const int lane = lane_id(), c = lane & 15, kg = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int t0 = blockIdx.y * kLoTile;
-    const int m_from = (blockIdx.x * kLoWaves + wave) * per_wave, m_to = min(a.M, m_from + per_wave);
+    const int m_from = (blockIdx.x * kLoExpandWaves + wave) * per_wave, m_to = min(a.M, m_from + per_wave);
     uint32_t firsts;
     const int id = lo_ids(a, t0, firsts);
     const size_t row = (size_t)min(t0 + c, a.n_tokens - 1);
     const float *base = a.base + row * a.M;
     float *out = a.out + row * a.M;
+    if (wave == 0 && kg == 0) ids[c] = id;
     int d = 0;
     for (; firsts; firsts &= firsts - 1, d++) {
         if (d % gridDim.z != blockIdx.z) continue;
@@ -205,101 +214,119 @@ __global__ void __launch_bounds__(kLoThreads) lora_expand_kernel(LoraArgs a, int
         const int rank = min(a.ranks[ad], a.max_rank);
         const float scale = a.scales[ad];
         const uint16_t *B = (const uint16_t *)a.b + (size_t)ad * a.M * a.max_rank;
+        const uint16_t *Bw = B + (size_t)m_from * a.max_rank;  // the wave's rows
+        // of the step that the rank ends in: what lies behind it may be no number
+        u4 keep;
+        {
+            const int r = (rank & ~31) + 8 * kg, live = rank - (r < rank ? r : 0);
+#pragma unroll
+            for (int j = 0; j < 4; j++) keep[j] = live > 2 * j + 1 ? ~0u : live > 2 * j ? 0xffffu : 0u;
+        }
         LoOperand<BF> o[NS];
         int e = -127;
-        {
-            float v[NS][8], largest = 0.0f;
-#pragma unroll
-            for (int st = 0; st < NS; st++) {
-                const int r = 32 * st + 8 * kg;
-#pragma unroll
-                for (int j = 0; j < 8; j++) v[st][j] = 0.0f;
-                if (mine && r < rank)
-                    for (int p = 0; p < parts; p++) {
-                        float y[8];
-                        __builtin_memcpy(y, a.ws + ((size_t)p * a.n_tokens + row) * a.max_rank + r, 32);
-#pragma unroll
-                        for (int j = 0; j < 8; j++) v[st][j] += r + j < rank ? y[j] : 0.0f;
-                    }
-#pragma unroll
-                for (int j = 0; j < 8; j++) largest = fmaxf(largest, fabsf(v[st][j]));
+        // v: the parts are added by all threads, for all waves
+        lds_barrier();
+        for (int i = threadIdx.x; i < kLoTile * 8 * NS; i += 64 * kLoExpandWaves) {
+            const int t = i / (8 * NS), r = i % (8 * NS) * 4;
+            f4 x = {};
+            if (ids[t] == ad && r < rank) {
+                const float *part = a.ws + ((size_t)t0 + t) * a.max_rank + r;
+#pragma unroll 2
+                for (int p = 0; p < parts; p++, part += (size_t)a.n_tokens * a.max_rank) {
+                    f4 one;
+                    __builtin_memcpy(&one, part, 16);
+                    x += one;
+                }
             }
-            if (!BF) e = lo_exponent(largest);
 #pragma unroll
-            for (int st = 0; st < NS; st++) o[st].set(v[st], e);
+            for (int j = 0; j < 4; j++) x[j] = r + j < rank ? x[j] : 0.0f;
+            __builtin_memcpy(&vs[t][r], &x, 16);
         }
+        lds_barrier();
+        float v[NS][8], largest = 0.0f;
+#pragma unroll
+        for (int st = 0; st < NS; st++) {
+            __builtin_memcpy(v[st], &vs[c][32 * st + 8 * kg], 32);
+#pragma unroll
+            for (int j = 0; j < 8; j++) largest = fmaxf(largest, fabsf(v[st][j]));
+        }
+        if (!BF) e = lo_exponent(largest);
+#pragma unroll
+        for (int st = 0; st < NS; st++) o[st].set(v[st], e);
         for (int m0 = m_from; m0 < m_to; m0 += 16 * U) {
             u4 w[U][NS];
             f4 y[U];
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const int m = m0 + 16 * u + c, mo = m0 + 16 * u + 4 * kg;
+                // (rows behind the last, and words behind the rank, which meet zeros in v, are others')
+                const uint32_t m = min(m0 + 16 * u + c, m_to - 1) - m_from;
 #pragma unroll
                 for (int st = 0; st < NS; st++) {
                     const int r = 32 * st + 8 * kg;
-                    w[u][st] = u4{0, 0, 0, 0};
-                    if (m < m_to && r < rank) __builtin_memcpy(&w[u][st], B + (size_t)m * a.max_rank + r, 16);
+                    __builtin_memcpy(&w[u][st], Bw + (m * a.max_rank + (r < rank ? r : 0)), 16);
                 }
-                y[u] = f4{0.f, 0.f, 0.f, 0.f};
-                if (mine) {
-                    if (mo + 3 < m_to) __builtin_memcpy(&y[u], base + mo, 16);
-                    else
-                        for (int i = 0; i < 4; i++)
-                            if (mo + i < m_to) y[u][i] = base[mo + i];
-                }
+                if (mine && m0 + 16 * u + 4 * kg + 3 < m_to) __builtin_memcpy(&y[u], base + m0 + 16 * u + 4 * kg, 16);
             }
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const int mo = m0 + 16 * u + 4 * kg;
-                f4 acc = {};
+                f4 z = {};
 #pragma unroll
                 for (int st = 0; st < NS; st++) {
-                    if (32 * st >= rank) break;
-                    if (32 * st + 32 > rank) {  // what lies behind the rank may be no number
-                        const int live = rank - 32 * st - 8 * kg;
-#pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            w[u][st][j] = live > 2 * j + 1 ? w[u][st][j] : live > 2 * j ? w[u][st][j] & 0xffffu : 0;
+                    if (32 * st < rank) {
+                        if (st == rank / 32) w[u][st] &= keep;
+                        z = o[st].mul(w[u][st], z);
                     }
-                    acc = o[st].mul(w[u][st], acc);
                 }
-                f4 z;
+                if (!BF)
 #pragma unroll
-                for (int i = 0; i < 4; i++) z[i] = fmaf(scale, BF ? acc[i] : ldexpf(acc[i], e - 13), y[u][i]);
-                if (mine) {
-                    if (mo + 3 < m_to) __builtin_memcpy(out + mo, &z, 16);
-                    else
-                        for (int i = 0; i < 4; i++)
-                            if (mo + i < m_to) out[mo + i] = z[i];
-                }
+                    for (int i = 0; i < 4; i++) z[i] = ldexpf(z[i], e - 13);
+                const int mo = m0 + 16 * u + 4 * kg;
+                if (!mine) continue;
+                if (mo + 3 < m_to) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) z[i] = fmaf(scale, z[i], y[u][i]);
+                    __builtin_memcpy(out + mo, &z, 16);
+                } else
+#pragma unroll
+                    for (int i = 0; i < 3; i++)
+                        if (mo + i < m_to) out[mo + i] = fmaf(scale, z[i], base[mo + i]);
             }
         }
     }
 }
 
-// Parts of K: as many as there are steps, but few enough that adding them stays cheap.
-static int lo_parts(int K, int *per_part) {
-    const int steps = (K + kLoStep - 1) / kLoStep;
-    const int per = (steps + kLoMaxParts - 1) / kLoMaxParts;
+// Parts of K: as many as there are steps, but no more than it takes to fill the chip, since the second launch reads them all.
+static int lo_parts(int n_tokens, int K, int *per_part) {
+    const int tiles = (n_tokens + kLoTile - 1) / kLoTile, steps = (K + kLoStep - 1) / kLoStep;
+    int parts = tiles >= 1024 ? 1 : (1024 + tiles - 1) / tiles;
+    if (parts > kLoMaxParts) parts = kLoMaxParts;
+    if (parts > steps) parts = steps;
+    if (parts < 1) parts = 1;
+    const int per = (steps + parts - 1) / parts;
     *per_part = per * kLoStep;
     return (steps + per - 1) / per;
 }
 
 size_t lora_workspace_bytes(int n_tokens, int K, int max_rank) {
     int per;
-    return (size_t)lo_parts(K, &per) * n_tokens * max_rank * sizeof(float);
+    return (size_t)lo_parts(n_tokens > 0 ? n_tokens : 1, K, &per) * n_tokens * max_rank * sizeof(float);
 }
 
 template <bool BF>
 static int launch_typed(const LoraArgs &a, hipStream_t s) {
     int per_part;
-    const int parts = lo_parts(a.K, &per_part), tiles = (a.n_tokens + kLoTile - 1) / kLoTile;
-    // a tile's adapters by workgroups of their own, where tiles alone do not fill the chip
-    int z = tiles >= 64 ? 1 : kLoTile;
-    z = z < a.n_tokens ? z : a.n_tokens;
-    z = z < a.n_adapters + 1 ? z : a.n_adapters + 1;
-    const dim3 block(kLoThreads);
-    const dim3 g1(parts, tiles, z);
+    const int parts = lo_parts(a.n_tokens, a.K, &per_part), tiles = (a.n_tokens + kLoTile - 1) / kLoTile;
+    // a tile's adapters by workgroups of their own, as far as the chip has room for them
+    const int per_wave = tiles < 64 ? 64 : a.max_rank <= 64 ? 128 : 256, m_blocks = (a.M + kLoExpandWaves * per_wave - 1) / (kLoExpandWaves * per_wave);
+    auto apart = [&](long long groups, long long room) {
+        long long z = room / groups;
+        z = z < kLoTile ? z : kLoTile;
+        z = z < a.n_tokens ? z : a.n_tokens;
+        z = z < a.n_adapters + 1 ? z : a.n_adapters + 1;
+        return (int)(z > 1 ? z : 1);
+    };
+    const dim3 block(64 * kLoShrinkWaves), block2(64 * kLoExpandWaves);
+    const dim3 g1(parts, tiles, apart((long long)parts * tiles, 1024));
     const int ranks = (a.max_rank + 15) / 16;
 #define MNEMO_SHRINK(N) hipLaunchKernelGGL((lora_shrink_kernel<BF, N>), g1, block, 0, s, a, per_part)
     if (ranks <= 1) MNEMO_SHRINK(1);
@@ -309,9 +336,8 @@ static int launch_typed(const LoraArgs &a, hipStream_t s) {
     else MNEMO_SHRINK(16);
 #undef MNEMO_SHRINK
     if (int rc = check_launch("lora_add")) return rc;
-    const int per_wave = 256;
-    const dim3 g2((a.M + kLoWaves * per_wave - 1) / (kLoWaves * per_wave), tiles, z);
-#define MNEMO_EXPAND(N) hipLaunchKernelGGL((lora_expand_kernel<BF, N>), g2, block, 0, s, a, parts, per_wave)
+    const dim3 g2(m_blocks, tiles, apart((long long)m_blocks * tiles, 2048));
+#define MNEMO_EXPAND(N) hipLaunchKernelGGL((lora_expand_kernel<BF, N>), g2, block2, 0, s, a, parts, per_wave)
     if (ranks <= 2) MNEMO_EXPAND(1);
     else if (ranks <= 4) MNEMO_EXPAND(2);
     else if (ranks <= 8) MNEMO_EXPAND(4);

@@ -79,7 +79,8 @@ def test_nothing_of_no_rows(L):
 
 def test_workspaces(L):
     assert L.mnemo_lora_workspace_bytes(100, 4096, 16) == 4 * 100 * 16 * 4
-    assert L.mnemo_lora_workspace_bytes(524288, 1 << 20, 256) == 8 * 524288 * 256 * 4  # past 32 bits
+    assert L.mnemo_lora_workspace_bytes(1000, 1 << 20, 256) == 8 * 1000 * 256 * 4
+    assert L.mnemo_lora_workspace_bytes(524288, 8192, 256) == 524288 * 256 * 4  # past 32 bits: nothing is cut off
     assert L.mnemo_lora_workspace_bytes(10, 60, 16) == L.mnemo_lora_workspace_bytes(10, 64, 260) == 0
     assert L.mnemo_logprobs_workspace_bytes(1, 151936, 20) > 0
     assert L.mnemo_logprobs_workspace_bytes(0, 100, 4) == L.mnemo_logprobs_workspace_bytes(1, 100, 65) == 0
