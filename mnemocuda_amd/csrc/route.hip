@@ -8,9 +8,9 @@
 // Without a bias, and with groups that score one expert, c grows with z: the choice is made among the logits.
 //
 // L lanes (16 or 64) look after a token and hold its experts in registers, a group's in adjacent lanes.
-// An expert's place in the order is one 64-bit key: the bits of c as a whole number that orders as c does, its
-// lowest ten replaced by 1023 - e.  Scores are formed in 64 bits, so that two that differ are told apart
-// (2^-42 of either is what the ten bits cost); k rounds take the largest key out.
+// An expert's place in the order is one number, its key: c with the lowest ten bits giving way to the index.  Scores
+// are formed in 64 bits, so that two that differ are told apart (2^-42 of either is what the ten bits cost); k
+// rounds take the largest key out.
 #include <math.h>
 
 #include "mnemo_common.hpp"
@@ -18,28 +18,35 @@
 
 namespace mnemo {
 
-// a whole number that orders as v does
-__device__ __forceinline__ uint64_t order_bits(double v) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    return b >> 63 ? ~b : b | 1ull << 63;
+// An expert's key: c with its lowest ten bits replaced by what orders its index, smaller before larger.  Keys are
+// compared as numbers.  kNone is below all of them.
+constexpr double kNone = -0x1.fffffffffffffp1023;
+__device__ __forceinline__ double make_key(double c, int e) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, fmin(c, -kNone));  // (an infinity has no bits to spare)
+    return __builtin_bit_cast(double, (b & ~1023ull) | (uint64_t)(b >> 63 ? e : 1023 - e));
 }
-__device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
+__device__ __forceinline__ int key_expert(double key) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, key);
+    return (int)(b >> 63 ? b & 1023 : 1023 - (b & 1023));
+}
+__device__ __forceinline__ uint32_t low_word(double v) { return (uint32_t)__builtin_bit_cast(uint64_t, v); }
 template <int CTRL>
-__device__ __forceinline__ uint64_t dpp_u64(uint64_t v) {
-    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, 0xF, 0xF, false);
-    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, 0xF, 0xF, false);
-    return (uint64_t)hi << 32 | lo;
+__device__ __forceinline__ double dpp_double(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xF, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xF, 0xF, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 // over the L lanes of a token, in all of them
 template <int L>
-__device__ __forceinline__ uint64_t max_token(uint64_t v) {
-    v = max64(v, dpp_u64<kDppXor1>(v));
-    v = max64(v, dpp_u64<kDppXor2>(v));
-    v = max64(v, dpp_u64<kDppRowHalfMirror>(v));
-    v = max64(v, dpp_u64<kDppRowMirror>(v));
+__device__ __forceinline__ double max_token(double v) {
+    v = fmax(v, dpp_double<kDppXor1>(v));
+    v = fmax(v, dpp_double<kDppXor2>(v));
+    v = fmax(v, dpp_double<kDppRowHalfMirror>(v));
+    v = fmax(v, dpp_double<kDppRowMirror>(v));
     if (L == 64) {
-        v = max64(v, __shfl_xor((unsigned long long)v, 16));
-        v = max64(v, __shfl_xor((unsigned long long)v, 32));
+        v = fmax(v, __shfl_xor(v, 16));
+        v = fmax(v, __shfl_xor(v, 32));
     }
     return v;
 }
@@ -54,14 +61,42 @@ __device__ __forceinline__ float max_token(float v) {
 }
 template <int L>
 __device__ __forceinline__ double sum_token(double v) {
-#pragma unroll
-    for (int o = 1; o < L; o <<= 1) v += __shfl_xor(v, o);
+    v += dpp_double<kDppXor1>(v);
+    v += dpp_double<kDppXor2>(v);
+    v += dpp_double<kDppRowHalfMirror>(v);
+    v += dpp_double<kDppRowMirror>(v);
+    if (L == 64) {
+        v += __shfl_xor(v, 16);
+        v += __shfl_xor(v, 32);
+    }
     return v;
 }
 
+// exp(v), v <= 0, within 2^-50: 2^n times the series of exp on [-ln 2 / 2, ln 2 / 2], whose 12th power is below 2^-47 / 12!.
+// (-inf: 0; no number: none.)
+__device__ __forceinline__ double exp_below(double v) {
+    const double n = rint(v * 1.4426950408889634);
+    double r = fma(n, -0x1.62e42fefa39efp-1, v);
+    r = fma(n, -0x1.abc9e3b39803fp-56, r);
+    double p = 1.0 / 479001600;
+#pragma unroll
+    for (int i = 11; i >= 0; i--) {
+        constexpr double f[12] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320, 1.0 / 362880, 1.0 / 3628800, 1.0 / 39916800};
+        p = fma(p, r, f[i]);
+    }
+    p = ldexp(p, (int)n);
+    return v < -745.0 ? 0.0 : p;
+}
+// 1 / v, 1 <= v, by two Newton steps from the instruction's estimate
+__device__ __forceinline__ double inverse(double v) {
+    double r = __builtin_amdgcn_rcp(v);
+    r = fma(fma(-v, r, 1.0), r, r);
+    return fma(fma(-v, r, 1.0), r, r);
+}
+
 __device__ __forceinline__ double sigmoid(float z) {
-    const double e = exp(-fabs((double)z));
-    return (z >= 0.0f ? 1.0 : e) / (1.0 + e);  // (no number: no number)
+    const double e = exp_below(-fabs((double)z));
+    return (z >= 0.0f ? 1.0 : e) * inverse(1.0 + e);  // (no number: no number)
 }
 
 // N: experts per lane.  SCORED: c is formed; else the choice is among the logits.
@@ -76,18 +111,21 @@ __global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
     const int mine = g < a.n_groups ? min(max(a.per_group - i0, 0), a.per_lane) : 0;
     const int first = mine > 0 ? g * a.per_group + i0 : 0;
 
-    float x[N];
-    if (a.vec) {  // whole words of four
+    // (loads without branches: what a lane has no experts for is read from where it has some, and dropped)
+    float x[N], bias[SCORED ? N : 1];
+    auto read = [&](const float *from, float *to) {
+        if (a.vec) {  // whole words of four
 #pragma unroll
-        for (int t = 0; t < N; t += 4) {
+            for (int t = 0; t < N; t += 4) __builtin_memcpy(&to[t], from + first + (t < mine ? t : 0), 16);
+        } else {
 #pragma unroll
-            for (int j = 0; j < 4 && t + j < N; j++) x[t + j] = -INFINITY;
-            if (N >= 4 && t < mine) __builtin_memcpy(&x[t], z + first + t, 16);
+            for (int t = 0; t < N; t++) to[t] = from[first + (t < mine ? t : 0)];
         }
-    } else {
+    };
+    read(z, x);
+    if (SCORED && a.bias) read(a.bias, bias);
 #pragma unroll
-        for (int t = 0; t < N; t++) x[t] = t < mine ? z[first + t] : -INFINITY;
-    }
+    for (int t = 0; t < N; t++) x[t] = t < mine ? x[t] : -INFINITY;
 
     // softmax: the maximum, and the sum where it is asked for
     float m = -INFINITY;
@@ -101,32 +139,39 @@ __global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
             double sum = 0.0;
 #pragma unroll
             for (int t = 0; t < N; t++)
-                if (t < a.per_lane) sum += SCORED ? exp((double)x[t] - (double)ref) : (double)expf(x[t] - ref);
+                sum += SCORED ? exp_below((double)x[t] - (double)ref) : (double)expf(x[t] - ref);
             total = sum_token<L>(sum);
         }
         m = ref;
     }
+    const double share = total > 0.0 || total != total ? 1.0 / total : 0.0;
 
-    uint64_t key[N];
+    double key[N];
+    if (SCORED) {
+        if (a.sigmoid) {
+#pragma unroll
+            for (int t = 0; t < N; t++) key[t] = sigmoid(x[t]);
+        } else {
+#pragma unroll
+            for (int t = 0; t < N; t++) key[t] = exp_below((double)x[t] - (double)m) * share;
+        }
+        if (a.bias) {
+#pragma unroll
+            for (int t = 0; t < N; t++) key[t] += (double)bias[t];
+        }
+    } else {
+#pragma unroll
+        for (int t = 0; t < N; t++) key[t] = x[t];
+    }
     double b1 = -INFINITY, b2 = -INFINITY;  // largest c of the lane's experts
     bool bad = false;
 #pragma unroll
     for (int t = 0; t < N; t++) {
-        key[t] = 0;
-        if (t < a.per_lane) {
-            double c = x[t];
-            if (SCORED) {
-                c = a.sigmoid ? sigmoid(x[t]) : exp((double)x[t] - (double)m) / total;
-                if (a.bias) c += t < mine ? (double)a.bias[first + t] : 0.0;
-            }
-            c += 0.0;  // one zero
-            if (x[t] == -INFINITY) c = -INFINITY;
-            if (t < mine) bad |= c != c || (!a.sigmoid && x[t] == INFINITY);
-            if (t < mine && c > -INFINITY) key[t] = (order_bits(c) & ~1023ull) | (uint64_t)(1023 - (first + t));
-            else c = -INFINITY;
-            b2 = fmax(b2, fmin(b1, c));
-            b1 = fmax(b1, c);
-        }
+        const double c = x[t] == -INFINITY ? -INFINITY : key[t] + 0.0;  // (one zero)
+        bad |= c != c || (!a.sigmoid && x[t] == INFINITY);
+        b2 = fmax(b2, fmin(b1, c));
+        b1 = fmax(b1, c);
+        key[t] = c > -INFINITY ? make_key(c, first + t) : kNone;
     }
     bad = (__ballot(bad) >> (lane & ~(L - 1)) & (L == 64 ? ~0ull : 0xffffull)) != 0;
 
@@ -137,30 +182,34 @@ __global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
             b1 = fmax(b1, o1);
         }
         const double score = a.best == 2 && b2 > -INFINITY ? b1 + b2 : b1;
-        const uint64_t gkey = g < a.n_groups && b1 > -INFINITY ? (order_bits(score) & ~63ull) | (uint64_t)(63 - g) : 0;
+        const double gkey = g < a.n_groups && b1 > -INFINITY ? make_key(score, g) : kNone;
         int better = 0;
         for (int o = 0; o < a.n_groups; o++)
-            better += __shfl((unsigned long long)gkey, (lane & ~(L - 1)) + (o << a.lanes_log)) > gkey;
+            better += __shfl(gkey, (lane & ~(L - 1)) + (o << a.lanes_log)) > gkey;
         if (better >= a.top_groups) {
 #pragma unroll
-            for (int t = 0; t < N; t++) key[t] = 0;
+            for (int t = 0; t < N; t++) key[t] = kNone;
         }
     }
 
     int mine_idx = -1;
     for (int j = 0; j < a.k; j++) {
-        uint64_t best = key[0];
+        double best = key[0];
 #pragma unroll
-        for (int t = 1; t < N; t++) best = max64(best, key[t]);
+        for (int t = 1; t < N; t++) best = fmax(best, key[t]);
         best = max_token<L>(best);
-        if (gl == j && best) mine_idx = 1023 - (int)(best & 1023);
+        if (gl == j && best > kNone) mine_idx = key_expert(best);
+        // the lower words differ in the index; what is left of one that goes is the most negative upper word
 #pragma unroll
-        for (int t = 0; t < N; t++) key[t] = key[t] == best ? 0 : key[t];
+        for (int t = 0; t < N; t++) {
+            const uint64_t b = __builtin_bit_cast(uint64_t, key[t]);
+            key[t] = (uint32_t)b == low_word(best) ? __builtin_bit_cast(double, 0xffefffffffffffffull) : key[t];
+        }
     }
     double w = 0.0;
     if (mine_idx >= 0) {
         const float zi = z[mine_idx];
-        w = a.sigmoid ? sigmoid(zi) : exp((double)zi - (double)m);
+        w = a.sigmoid ? sigmoid(zi) : exp_below((double)zi - (double)m);
     }
     if (a.renorm) total = sum_token<L>(w);
     if (a.renorm || !a.sigmoid) w = total > 0.0 ? w / total : 0.0;
@@ -194,7 +243,7 @@ int launch_route(RouteArgs a, hipStream_t s) {
         wide = a.per_lane > 32;
     }
     if (wide) spread(64);
-    a.vec = a.per_group % 4 == 0 && (uintptr_t)a.z % 16 == 0;
+    a.vec = a.per_group % 4 == 0 && ((uintptr_t)a.z | (uintptr_t)a.bias) % 16 == 0;
     const bool scored = a.bias || (a.best == 2 && a.top_groups < a.n_groups);
     if (wide) scored ? launch_lanes<64, true>(a, s) : launch_lanes<64, false>(a, s);
     else scored ? launch_lanes<16, true>(a, s) : launch_lanes<16, false>(a, s);
