@@ -7,7 +7,7 @@
 //   w = s of the chosen, / their sum where asked for, * scale
 // Without a bias, and with groups that score one expert, c grows with z: the choice is made among the logits.
 //
-// L lanes (16 or 64) look after a token and hold its experts in registers, a group's in adjacent lanes.
+// L lanes (16, 32 or 64) look after a token and hold its experts in registers, a group's in adjacent lanes.
 // An expert's place in the order is one number, its key: c with the lowest ten bits giving way to the index.  Scores
 // are formed in 64 bits, so that two that differ are told apart (2^-42 of either is what the ten bits cost); k
 // rounds take the largest key out.
@@ -44,19 +44,15 @@ __device__ __forceinline__ double max_token(double v) {
     v = fmax(v, dpp_double<kDppXor2>(v));
     v = fmax(v, dpp_double<kDppRowHalfMirror>(v));
     v = fmax(v, dpp_double<kDppRowMirror>(v));
-    if (L == 64) {
-        v = fmax(v, __shfl_xor(v, 16));
-        v = fmax(v, __shfl_xor(v, 32));
-    }
+    if (L >= 32) v = fmax(v, __shfl_xor(v, 16));
+    if (L == 64) v = fmax(v, __shfl_xor(v, 32));
     return v;
 }
 template <int L>
 __device__ __forceinline__ float max_token(float v) {
     v = max16(v);
-    if (L == 64) {
-        v = fmaxf(v, __shfl_xor(v, 16));
-        v = fmaxf(v, __shfl_xor(v, 32));
-    }
+    if (L >= 32) v = fmaxf(v, __shfl_xor(v, 16));
+    if (L == 64) v = fmaxf(v, __shfl_xor(v, 32));
     return v;
 }
 template <int L>
@@ -65,10 +61,8 @@ __device__ __forceinline__ double sum_token(double v) {
     v += dpp_double<kDppXor2>(v);
     v += dpp_double<kDppRowHalfMirror>(v);
     v += dpp_double<kDppRowMirror>(v);
-    if (L == 64) {
-        v += __shfl_xor(v, 16);
-        v += __shfl_xor(v, 32);
-    }
+    if (L >= 32) v += __shfl_xor(v, 16);
+    if (L == 64) v += __shfl_xor(v, 32);
     return v;
 }
 
@@ -173,7 +167,7 @@ __global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
         b1 = fmax(b1, c);
         key[t] = c > -INFINITY ? make_key(c, first + t) : kNone;
     }
-    bad = (__ballot(bad) >> (lane & ~(L - 1)) & (L == 64 ? ~0ull : 0xffffull)) != 0;
+    bad = (__ballot(bad) >> (lane & ~(L - 1)) & (L == 64 ? ~0ull : (1ull << (L & 63)) - 1)) != 0;
 
     if (a.top_groups < a.n_groups) {
         for (int o = 1; o < 1 << a.lanes_log; o <<= 1) {
@@ -194,10 +188,14 @@ __global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
 
     int mine_idx = -1;
     for (int j = 0; j < a.k; j++) {
-        double best = key[0];
+        double half[N / 2];
 #pragma unroll
-        for (int t = 1; t < N; t++) best = fmax(best, key[t]);
-        best = max_token<L>(best);
+        for (int t = 0; t < N / 2; t++) half[t] = fmax(key[t], key[t + N / 2]);
+#pragma unroll
+        for (int n = N / 4; n > 0; n /= 2)
+#pragma unroll
+            for (int t = 0; t < n; t++) half[t] = fmax(half[t], half[t + n]);
+        const double best = max_token<L>(half[0]);
         if (gl == j && best > kNone) mine_idx = key_expert(best);
         // the lower words differ in the index; what is left of one that goes is the most negative upper word
 #pragma unroll
@@ -236,16 +234,19 @@ int launch_route(RouteArgs a, hipStream_t s) {
         a.per_lane = (a.per_group + (1 << a.lanes_log) - 1) >> a.lanes_log;
         if (a.per_group % 4 == 0) a.per_lane = (a.per_lane + 3) & ~3;
     };
-    // a lane of 64 holds at most 32 experts: with 2^n < n_groups <= 2^(n+1) it has the 2^(n+5)th part of a group
-    bool wide = a.n_groups > 16 || a.n_tokens < 2048;
-    if (!wide) {
-        spread(16);
-        wide = a.per_lane > 32;
+    // Few lanes a token do least in all, many are done soonest: 256 experts in 8 groups, 1500 tokens, 64 lanes 6.8 us, 16 9.3; 2048
+    // tokens, 32 lanes 7.1, 16 9.4; 8191 13.4 and 13.9; 60,000 65.5 and 62.7 (of 64 experts 28.0 and 15.5).
+    int lanes = a.n_tokens < 2048 ? 64 : a.n_tokens < 16384 && a.n_experts >= 256 ? 32 : 16;
+    // (a lane of 64 holds at most 32 experts: with 2^n < n_groups <= 2^(n+1) it has the 2^(n+5)th part of a group)
+    for (;; lanes *= 2) {
+        if (lanes < a.n_groups && lanes < 64) continue;
+        spread(lanes);
+        if (a.per_lane <= 32) break;
     }
-    if (wide) spread(64);
     a.vec = a.per_group % 4 == 0 && ((uintptr_t)a.z | (uintptr_t)a.bias) % 16 == 0;
     const bool scored = a.bias || (a.best == 2 && a.top_groups < a.n_groups);
-    if (wide) scored ? launch_lanes<64, true>(a, s) : launch_lanes<64, false>(a, s);
+    if (lanes == 64) scored ? launch_lanes<64, true>(a, s) : launch_lanes<64, false>(a, s);
+    else if (lanes == 32) scored ? launch_lanes<32, true>(a, s) : launch_lanes<32, false>(a, s);
     else scored ? launch_lanes<16, true>(a, s) : launch_lanes<16, false>(a, s);
     return check_launch("moe_route");
 }

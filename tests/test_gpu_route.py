@@ -70,7 +70,8 @@ def check(got, want):
     (4, 1020, 9, False, True, 17, 5, 2, False), (6, 64, 2, True, True, 64, 2, 2, True), (11, 51, 5, True, False, 17, 3, 1, True),
     (2048, 128, 8, False, False, 1, 1, 1, True), (2051, 256, 8, True, True, 8, 4, 2, True), (2049, 512, 16, True, True, 16, 1, 1, True),
     (2050, 510, 3, False, True, 1, 1, 1, False), (2053, 174, 15, True, True, 2, 1, 1, True), (2048, 520, 5, True, False, 4, 2, 2, True),
-    (2055, 9, 3, False, False, 3, 2, 2, True)])
+    (2055, 9, 3, False, False, 3, 2, 2, True), (16391, 256, 8, True, True, 8, 4, 2, True), (2060, 1024, 7, True, True, 1, 1, 1, True),
+    (2061, 768, 4, False, True, 24, 3, 2, True), (16385, 340, 5, True, True, 17, 4, 2, False), (16384, 40, 6, False, False, 1, 1, 1, False)])
 def test_against_the_formula(gpu, T, E, k, sigmoid, bias, groups, top_groups, best, renorm):
     rng = np.random.default_rng(T + E)
     z = (2 * rng.standard_normal((T, E))).astype(np.float32)
