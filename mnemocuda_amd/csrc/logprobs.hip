@@ -195,14 +195,17 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(LogprobsArgs a, Lp
             s.S *= f;
             s.m = top;
         }
+        float S = 0.0f, T = 0.0f;  // of the step, so that a long row's sums are not of thousands of additions
 #pragma unroll
         for (int g = 0; g < kLpWords; g++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const float d = y[g][j] - s.m, e = __builtin_amdgcn_exp2f(d * kLpLog2e);
-                s.S += e;
-                s.T = fmaf(e, fmaxf(d, -1e30f), s.T);
+                S += e;
+                T = fmaf(e, fmaxf(d, -1e30f), T);
             }
+        s.S += S;
+        s.T += T;
         const int first = at + 4 * tid;
         if (a.rank) {
             if (at + kLpStep <= t) {

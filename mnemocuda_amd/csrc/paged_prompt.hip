@@ -402,12 +402,14 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
                 }
         }
 
-        float m[RT], l[RT];  // reference (log2) of the lane's row, sum over the lane's positions
+        // reference (log2) of the lane's row, sum over the lane's positions and what its additions have lost: of a long row
+        // they are thousands
+        float m[RT], l[RT], lost[RT];
         f4 o[RT][ND] = {};
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
             m[rt] = -INFINITY;
-            l[rt] = 0.0f;
+            l[rt] = lost[rt] = 0.0f;
         }
         for (; p0 < p_end; p0 += kStep, b ^= KV == kKvF16) {
             // positions that are there; whether there is something that some row does not see
@@ -536,22 +538,26 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
                         const float mn = top > m[rt] + kSlack ? top : m[rt];  // a row's own doing
                         const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - mn);
                         l[rt] *= al;
+                        lost[rt] *= al;
                         m[rt] = mn;
 #pragma unroll
                         for (int i = 0; i < ND; i++) o[rt][i] *= al;
                     }
                     const float ref = m[rt] == -INFINITY ? 0.0f : m[rt] - kLift;
-                    float p[8];
+                    float p[8], sum[4];
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
                         float x = fmaf(s[rt][j / 4][j & 3], KV == kKvF16 ? c[rt] : f[j / 4][j & 3], -ref);
                         if (KV == kKvInt8 && !full) x = seen >> j & 1 ? x : -INFINITY;
                         x = __builtin_amdgcn_exp2f(x);
-                        l[rt] += x;
+                        sum[j & 3] = j < 4 ? x : sum[j & 3] + x;
                         // (the scale of a position that is not seen may be no number)
                         if (KV == kKvInt8) x = full || (seen >> j & 1) ? x * vs[j / 4][j & 3] : 0.0f;
                         p[j] = x;
                     }
+                    const float more = (sum[0] + sum[1]) + (sum[2] + sum[3]), to = l[rt] + more;
+                    lost[rt] += more - (to - l[rt]);  // (exact while l is the larger)
+                    l[rt] = to;
 #pragma unroll
                     for (int j = 0; j < 8; j += 2) {
                         const h2x2 x = two_parts(p[j], p[j + 1]);
@@ -602,7 +608,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
         float *part = a.ws + (size_t)(2 * g + begins) * part_floats(HD);
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
-            const float sum = sum_row(l[rt]);
+            const float sum = sum_row(l[rt] + (l[rt] <= FLT_MAX ? lost[rt] : 0.0f));
             if (lim[rt] == INT_MAX) continue;
             if (begins && finishes) {
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;

@@ -77,11 +77,13 @@ def make(seed, new, before, nkv, G, hd, ps, int8, extra=3):
 
 
 def check(got, want, bar=BAR):
+    """bar: of all tokens, or of each."""
+    bar = np.broadcast_to(bar, len(want))
     for t in range(len(want)):
         if not want[t].any():
             assert not got[t].any(), t
         else:
-            assert rel_l2(got[t], want[t]) <= bar, (t, rel_l2(got[t], want[t]))
+            assert rel_l2(got[t], want[t]) <= bar[t], (t, rel_l2(got[t], want[t]), bar[t])
 
 
 SHAPES = [(128, 64, 4, 16, False), (128, 64, 2, 16, True), (128, 16, 2, 5, False), (128, 16, 2, 5, True), (128, 32, 1, 1, False),
@@ -364,3 +366,14 @@ def test_on_two_streams(gpu):
     torch.cuda.synchronize()
     for i in range(2):
         assert np.array_equal(host(outs[i]), want[i])
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_long_rows_keep_their_bits(gpu, int8):
+    """40,000 positions added up by one lane group after another: the sum of the weights is compensated, and the output is
+    rounded four times a step, 2,500 times with one standard deviation of 2^-24 / sqrt(12) * 2 each at most, 1.7e-6; with
+    the scores' share (see above) below 2.5e-6."""
+    a = make(12, [40], [40000], 1, 3, 128, 64, int8)
+    case(f"paged prompt, long rows int8={int8}")
+    got = host(attend(gpu, *a, 128 ** -0.5))
+    assert rel_l2(got, reference(*a, 128 ** -0.5)) <= 2.5e-6
