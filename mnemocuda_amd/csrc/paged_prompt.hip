@@ -49,18 +49,19 @@ struct Shape {
 };
 __host__ __device__ constexpr int groups_of(int hd) { return hd == 256 ? 256 : 512; }  // workgroups that fill the chip
 
-// Workspace: two partials per workgroup (max [rows], sum [rows], O [rows][hd]), and what they are: begun[g] describes the
-// tile that begins in workgroup g's share and goes on behind it (its second partial), taken[g] is the first unit of the
-// tile that it goes on with from the workgroup before (its first), -1 for none.
+// Workspace: two partials per workgroup (max [rows], sum [rows], O [rows][hd]): of the tile that its share goes on with, and
+// of the one that its share begins and does not end; and what these tiles are.
 __host__ __device__ constexpr int part_floats(int hd) { return kRows * (hd + 2); }
-struct Begun {
-    int first;  // first unit, -1 for none
+struct __align__(16) Cut {
+    int n;   // workgroups that share the tile, 0 for none
+    int g0;  // the first of them
     int row0, n_rows, kvh;  // first token (row of q), rows in use, KV head
+    int pad[3];
 };
-__device__ __forceinline__ Begun *begun_of(const PagedPromptArgs &a) {
-    return (Begun *)(a.ws + (size_t)2 * groups_of(a.c.hd) * part_floats(a.c.hd));
+// [workgroup][0: gone on with, 1: begun]
+__device__ __forceinline__ Cut *cuts_of(const PagedPromptArgs &a) {
+    return (Cut *)(a.ws + (size_t)2 * groups_of(a.c.hd) * part_floats(a.c.hd));
 }
-__device__ __forceinline__ int *taken_of(const PagedPromptArgs &a) { return (int *)(begun_of(a) + groups_of(a.c.hd)); }
 
 // ------------------------------------------------------------------ the row of steps
 struct Seq {
@@ -131,6 +132,11 @@ __device__ __forceinline__ Plan make_plan(const PagedPromptArgs &a, int groups) 
 }
 __device__ __forceinline__ int first_of(const Plan &p, int g) {
     return g >= p.groups ? p.total : g * p.base + min(g, p.more);
+}
+// The workgroup that has unit u.
+__device__ __forceinline__ int group_of(const Plan &p, int u) {
+    const int longer = p.more * (p.base + 1);
+    return u < longer ? u / (p.base + 1) : p.more + (u - longer) / p.base;
 }
 
 // of tile j: the positions that its last token sees
@@ -267,10 +273,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
     const int g = (int)(blockIdx.x >> 3) < per_xcd ? (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3) : blockIdx.x;
     int at = first_of(plan, g);
     const int end = first_of(plan, g + 1);
-    if (tid == 0) {
-        begun_of(a)[g].first = -1;
-        taken_of(a)[g] = -1;
-    }
+    if (tid < 2) cuts_of(a)[2 * g + tid].n = 0;
     // of the lane's rows: the token within a tile and its head
     int tok_of[RT], head_of[RT];
 #pragma unroll
@@ -629,9 +632,9 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
                     __builtin_memcpy(part + 2 * kRows + (size_t)row * HD + 16 * i + 4 * kg, &o[rt][i], 16);
             }
         }
-        if (tid == 0) {
-            if (!begins) taken_of(a)[g] = at - w.unit;
-            else if (!finishes) begun_of(a)[g] = {at - w.unit, w.s.start + tok0, toks * a.gqa, w.kvh};
+        if (tid == begins && !(begins && finishes)) {  // (by the thread that cleared it)
+            const int u = at - w.unit + a.cost, g0 = group_of(plan, u);  // of the tile's first step
+            cuts_of(a)[2 * g + begins] = {group_of(plan, u + w.steps - 1) - g0 + 1, g0, w.s.start + tok0, toks * a.gqa, w.kvh, {}};
         }
         at += units;
         if (at < end) advance(a, w);
@@ -647,35 +650,28 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
         }
 }
 
-// Merges the partials of the tile that begins in workgroup blockIdx.x's share and goes on behind it.  256 threads are
-// HD / 4 lanes of four dims, times threads that divide the partials among them where there are many, times rows;
-// blockIdx.y: which 4 rows.
+// Merges the partials of a tile that workgroups g0 to g0 + n - 1 had shares of: all but the last of them, here workgroups of
+// the same number, divide its rows (blockIdx.y: of which 16).  256 threads are HD / 4 lanes of four dims, times threads that
+// divide a row's partials among them where there are many, or rows.
 template <int HD>
 __global__ void __launch_bounds__(256) paged_prompt_merge_kernel(PagedPromptArgs a) {
-    constexpr int kGroups = groups_of(HD), D4 = HD / 4, PARTS = 256 / D4;
+    constexpr int D4 = HD / 4, PARTS = 256 / D4;
     __shared__ __align__(16) float so[PARTS][HD];
     __shared__ float sm[PARTS], sl[PARTS];
-    const Begun b = begun_of(a)[blockIdx.x];
-    if (b.first < 0 || 4 * (int)blockIdx.y >= b.n_rows) return;
-    const int *taken = taken_of(a);
-    int n = 1;
-    for (int g0 = blockIdx.x + 1; g0 < kGroups; g0 += 64) {  // workgroups that go on with it, one after another
-        const int g = g0 + lane_id();
-        const uint64_t on = __ballot(g < kGroups && taken[min(g, kGroups - 1)] == b.first);
-        const int more = on == ~0ull ? 64 : __ffsll((unsigned long long)~on) - 1;
-        n += more;
-        if (more < 64) break;
-    }
-    // partial i: the second of workgroup blockIdx.x, then the first of each that follows
-    auto part = [&](int i) { return a.ws + (size_t)(2 * (blockIdx.x + i) + (i == 0)) * part_floats(HD); };
-    // few partials: 16 rows by every fourth workgroup; many: 4 rows, by threads that divide the partials
-    const bool few = n <= 4;
-    if (few && blockIdx.y & 3) return;
-    const int chain = few ? 1 : PARTS < 4 ? 1 : PARTS / 4, per_pass = PARTS / chain;  // threads per word, rows at once
+    const Cut *cut = cuts_of(a) + 2 * blockIdx.x;
+    const Cut t = cut[1].n ? cut[1] : cut[0];
+    const int n = t.n, g0 = t.g0, rows16 = min(16, t.n_rows - 16 * (int)blockIdx.y);
+    if (n == 0 || rows16 <= 0) return;
+    const int me = (int)blockIdx.x - g0, per = (rows16 + n - 2) / (n - 1), from = me * per, rows = min(per, rows16 - from);
+    if (me >= n - 1 || rows <= 0) return;
+    // partial i: the second of workgroup g0, then the first of each that follows
+    auto part = [&](int i) { return a.ws + (size_t)(2 * (g0 + i) + (i == 0)) * part_floats(HD); };
+    int per_pass = 1;  // rows at once: a power of two, in one pass where there are so many threads
+    while (per_pass < rows && per_pass < PARTS) per_pass *= 2;
+    const int chain = PARTS / per_pass;  // threads per word of a row
     const int d = 4 * (threadIdx.x % D4), slot = threadIdx.x / D4, c = slot % chain, rr = slot / chain;
-    const int rows = min(few ? 16 : 4, b.n_rows - 4 * (int)blockIdx.y);
     for (int r0 = 0; r0 < rows; r0 += per_pass) {
-        const int row = 4 * blockIdx.y + min(r0 + rr, rows - 1);
+        const int row = 16 * blockIdx.y + from + min(r0 + rr, rows - 1);
         float m = -INFINITY, l = 0.0f;
         f4 x = {};
         for (int i0 = c; i0 < n; i0 += 4 * chain) {  // four loads in flight
@@ -730,7 +726,7 @@ __global__ void __launch_bounds__(256) paged_prompt_merge_kernel(PagedPromptArgs
         if (r0 + rr < rows) {
             x *= l == 0.0f ? 0.0f : 1.0f / l;
             const int tok = row / a.gqa, head = row - tok * a.gqa;
-            __builtin_memcpy(a.out + ((size_t)(b.row0 + tok) * a.nh + b.kvh * a.gqa + head) * HD + d, &x, 16);
+            __builtin_memcpy(a.out + ((size_t)(t.row0 + tok) * a.nh + t.kvh * a.gqa + head) * HD + d, &x, 16);
         }
     }
 }
@@ -739,14 +735,14 @@ template <int KV, int HD>
 int launch_shape(const PagedPromptArgs &a, hipStream_t s) {
     hipLaunchKernelGGL((paged_prompt_kernel<KV, HD>), dim3(groups_of(HD)), dim3(Shape<HD>::kThreads), 0, s, a);
     if (int rc = check_launch("paged_attention_prompt")) return rc;
-    hipLaunchKernelGGL(paged_prompt_merge_kernel<HD>, dim3(groups_of(HD), kRows / 4), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(paged_prompt_merge_kernel<HD>, dim3(groups_of(HD), kRows / 16), dim3(256), 0, s, a);
     return check_launch("paged_attention_prompt");
 }
 
 }  // namespace
 
 size_t paged_prompt_workspace_bytes(int hd) {
-    return (size_t)groups_of(hd) * (2 * part_floats(hd) * sizeof(float) + sizeof(Begun) + sizeof(int));
+    return (size_t)groups_of(hd) * 2 * (part_floats(hd) * sizeof(float) + sizeof(Cut));
 }
 
 int launch_paged_prompt(PagedPromptArgs a, hipStream_t s) {
