@@ -830,7 +830,7 @@ int mnemo_paged_attention_prompt(const float *q, const void *k_pages, const void
                          what, kMaxSeqs);
     if (n_tokens < 0 || n_tokens > 1 << 22) return set_error(kErrBadArg, "%s: n_tokens must be in 0..%d", what, 1 << 22);
     const int gqa = n_heads / n_kv_heads;
-    // the steps, and two for each tile, are counted in an int; a tile has more than 32 / gqa tokens, but for each sequence's last
+    // the steps, and two or three for each tile, are counted in an int; a tile has more than 64 / gqa tokens, but for each sequence's last
     if ((__int128)((long long)n_tokens * gqa / 32 + n_seqs) * n_kv_heads * max_pages * page_size >= (__int128)1 << 35)
         return set_error(kErrBadArg, "%s: (n_tokens * gqa / 32 + n_seqs) * n_kv_heads * max_pages * page_size must be below 2^35",
                          what);

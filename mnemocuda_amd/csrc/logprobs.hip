@@ -334,9 +334,10 @@ static LpPlan lp_plan(int n_rows, int vocab) {
     return p;
 }
 
+// Enough for every call of no more rows: there are at most 1024 parts.
 size_t logprobs_workspace_bytes(int n_rows, int vocab, int k) {
-    const LpPlan p = lp_plan(n_rows, vocab);
-    return p.whole == n_rows ? 16 : (size_t)(n_rows - p.whole) * p.parts * (sizeof(LpSums) + (size_t)k * 8);
+    const long long steps = ((long long)vocab + kLpStep - 1) / kLpStep, most = (steps < 64 ? steps : 64) * n_rows;
+    return (size_t)(most < 1024 ? most : 1024) * (sizeof(LpSums) + (size_t)k * 8);
 }
 
 int launch_logprobs(const LogprobsArgs &a, hipStream_t s) {

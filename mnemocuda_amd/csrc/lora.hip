@@ -307,9 +307,12 @@ static int lo_parts(int n_tokens, int K, int *per_part) {
     return (steps + per - 1) / per;
 }
 
+// Enough for every call of no more tokens: parts times tokens are at most kLoMaxParts times, and at most 1024 tiles more than,
+// the tokens.
 size_t lora_workspace_bytes(int n_tokens, int K, int max_rank) {
-    int per;
-    return (size_t)lo_parts(n_tokens > 0 ? n_tokens : 1, K, &per) * n_tokens * max_rank * sizeof(float);
+    const size_t steps = ((size_t)K + kLoStep - 1) / kLoStep, n = n_tokens;
+    const size_t most = (steps < kLoMaxParts ? steps : kLoMaxParts) * n, rows = n + (1024 + 1) * kLoTile;
+    return (most < rows ? most : rows) * max_rank * sizeof(float);
 }
 
 template <bool BF>

@@ -34,6 +34,10 @@ namespace mnemo {
 namespace {
 
 constexpr float kSlack = 5.0f, kLift = 9.0f;  // powers of two
+// int8: value scales below 2^-98 count as it for the reference, so that a weight is below 2^112.  The weights' sum is kept in
+// units of 2^16: those of 2^30 positions stay in range, and beside
+// scales of 2^90 weights down to 2^-29 of the largest.
+constexpr float kLeastScale = -98.0f, kUnit = 0x1p-16f;
 constexpr int kStep = 64;                     // positions
 // The shares are counted in units: a step is one, and what a tile takes beside its steps (its queries, its output) are
 // a few, `cost`.  A share has kLeast or more, as far as there are any.
@@ -115,12 +119,18 @@ __device__ __forceinline__ Plan make_plan(const PagedPromptArgs &a, int groups) 
     p.short_ = false;
     const int s0 = lane_id() * p.per;
     int sum = 0;
+    float size = 0.0f;
     for (int i = 0; i < p.per; i++)
         if (s0 + i < a.n_seqs) {
             const Seq s = seq_of(a, s0 + i);
             p.short_ |= s.n > s.len;
-            sum += units_of(s, a.tl, a.cost);
+            const int u = units_of(s, a.tl, a.cost);
+            sum += u;
+            size += (float)u;
         }
+    // (starts that do not rise may give the same rows to many sequences, and more units than an int holds: no work at all)
+    const bool fits = wave_sum_all(size) * (float)a.c.nkv < 0x1.fp30f;
+    sum = fits ? sum : 0;
     sum *= a.c.nkv;
     const int incl = wave_scan(sum);
     p.total = __builtin_amdgcn_readlane(incl, 63);
@@ -350,7 +360,8 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
             if (wave < 2) {
                 const float x = sc_raw[wave][lane];
                 (wave ? vsc : ksc)[lane] = x;
-                if (wave) vlg[lane] = __builtin_amdgcn_logf(fabsf(x));
+                // (a scale of 0 or next to it: its weight still counts in the sum, whose range this bounds)
+                if (wave) vlg[lane] = fmaxf(__builtin_amdgcn_logf(fabsf(x)), kLeastScale);
             }
         };
 
@@ -558,7 +569,9 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
                         if (KV == kKvInt8) x = full || (seen >> j & 1) ? x * vs[j / 4][j & 3] : 0.0f;
                         p[j] = x;
                     }
-                    const float more = (sum[0] + sum[1]) + (sum[2] + sum[3]), to = l[rt] + more;
+                    float more = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    if (KV == kKvInt8) more *= kUnit;
+                    const float to = l[rt] + more;
                     lost[rt] += more - (to - l[rt]);  // (exact while l is the larger)
                     l[rt] = to;
 #pragma unroll
@@ -613,6 +626,9 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
         for (int rt = 0; rt < RT; rt++) {
             const float sum = sum_row(l[rt] + (l[rt] <= FLT_MAX ? lost[rt] : 0.0f));
             if (lim[rt] == INT_MAX) continue;
+            if (KV == kKvInt8)
+#pragma unroll
+                for (int i = 0; i < ND; i++) o[rt][i] *= kUnit;
             if (begins && finishes) {
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                 float *out = a.out + io(rt) + 4 * kg;

@@ -377,3 +377,59 @@ def test_long_rows_keep_their_bits(gpu, int8):
     case(f"paged prompt, long rows int8={int8}")
     got = host(attend(gpu, *a, 128 ** -0.5))
     assert rel_l2(got, reference(*a, 128 ** -0.5)) <= 2.5e-6
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("scale", [0.0, -0.1])
+def test_scales_of_the_scores(gpu, scale, int8):
+    """A scale of 0 (all weights equal) and one below 0."""
+    a = make(14, [70, 3], [20, 300], 2, 3, 128, 32, int8)
+    case(f"paged prompt, scale {scale} int8={int8}")
+    check(host(attend(gpu, *a, scale)), reference(*a, scale))
+
+
+def test_value_scales_of_zero(gpu):
+    """Rows of zeros (scale 0) whose scores are the largest by far: their weights count in the sum.  Behind them, before
+    them and alone; and scales of 2^-75 beside them."""
+    q, k, v, ks, vs, table, starts, lens = make(15, [30, 30, 30, 30], [170] * 4, 1, 2, 64, 16, True)
+    q[:] = np.abs(q) + 0.5
+    for s, zero in enumerate([range(0, 100), range(150, 200), range(0, 200), range(0, 200, 2)]):
+        pos = np.array(list(zero))
+        page, off = table[s, pos // 16], pos % 16
+        vs[page, :, off] = 0.0
+        k[page, :, off] = 100  # scores of 20 and more above the others'
+        rest = np.setdiff1d(np.arange(200), pos)
+        if s == 3:
+            vs[table[s, rest // 16], :, rest % 16] *= np.float32(2.0 ** -75)
+    case("paged prompt, value scales of zero")
+    got = host(attend(gpu, q, k, v, ks, vs, table, starts, lens, 0.05))
+    want = reference(q, k, v, ks, vs, table, starts, lens, 0.05)
+    assert np.isfinite(got).all() and not got[60:90].any()
+    check(got, want)
+
+
+def test_starts_that_fall(gpu):
+    """Starts that give all rows to many sequences: whatever comes out, nothing outside the rows is read or written."""
+    rng = np.random.default_rng(16)
+    k, v, _, _ = pool(rng, 4, 1, 16, 64, False)
+    n = 400
+    q = dev(rng.standard_normal((64, 2, 64)).astype(np.float32))
+    table = np.zeros((n, 1), np.int32)
+    buf = torch.full((66, 2, 64), 3.0, device="cuda")
+    case("paged prompt, falling starts")
+    for far in (64, 2 ** 31 - 1):
+        starts = np.array([0, far] * (n // 2) + [0], np.int64).astype(np.int32)
+        attend(gpu, q, k, v, None, None, table, starts, np.full(n, 16, np.int32), 0.2, out=buf[1:65])
+        got = host(buf)
+        assert (got[0] == 3).all() and (got[65] == 3).all()
+
+
+def test_value_scales_of_the_ends(gpu):
+    """Values of up to 2^97, and below 2^-99."""
+    for e in (90, -106):
+        q, k, v, ks, vs, table, starts, lens = make(17, [40, 1], [300, 900], 1, 2, 64, 16, True)
+        vs[:] = np.float32(2.0 ** e)
+        case(f"paged prompt, value scales 2^{e}")
+        a = (q, k, v, ks, vs, table, starts, lens, 0.1)
+        want = reference(*a)
+        check(host(attend(gpu, *a)) * 2.0 ** -e, want * 2.0 ** -e)

@@ -78,12 +78,21 @@ def test_nothing_of_no_rows(L):
 
 
 def test_workspaces(L):
-    assert L.mnemo_lora_workspace_bytes(100, 4096, 16) == 4 * 100 * 16 * 4
-    assert L.mnemo_lora_workspace_bytes(1000, 1 << 20, 256) == 8 * 1000 * 256 * 4
-    assert L.mnemo_lora_workspace_bytes(524288, 8192, 256) == 524288 * 256 * 4  # past 32 bits: nothing is cut off
-    assert L.mnemo_lora_workspace_bytes(10, 60, 16) == L.mnemo_lora_workspace_bytes(10, 64, 260) == 0
-    assert L.mnemo_logprobs_workspace_bytes(1, 151936, 20) > 0
-    assert L.mnemo_logprobs_workspace_bytes(0, 100, 4) == L.mnemo_logprobs_workspace_bytes(1, 100, 65) == 0
+    """What suffices for a call suffices for every smaller one."""
+    lora, lp, at = L.mnemo_lora_workspace_bytes, L.mnemo_logprobs_workspace_bytes, L.mnemo_paged_attention_prompt_workspace_bytes
+    assert lora(100, 4096, 16) == 4 * 100 * 16 * 4  # four parts
+    assert lora(524288, 1 << 20, 256) > 524288 * 256 * 4  # past 32 bits
+    sizes = [1, 2, 15, 16, 17, 100, 1000, 1023, 1024, 1025, 3000, 5000, 8192, 16384, 16385, 60000]
+    for k in (8, 1000, 4096, 9000, 1 << 20):
+        need = [lora(n, k, 64) for n in sizes]
+        assert need == sorted(need) and need[0] > 0
+    for v in (1, 5000, 151936, 1 << 30):
+        need = [lp(n, v, 20) for n in sizes]
+        assert need == sorted(need) and need[0] > 0
+        assert lp(7, v, 0) <= lp(7, v, 1) <= lp(7, v, 64)
+    assert lora(10, 60, 16) == lora(10, 64, 260) == lora(-1, 64, 16) == 0
+    assert lp(0, 100, 4) == lp(1, 100, 65) == 0
+    assert at(8, 2, 128) == at(64, 4, 128) > 0 and at(8, 2, 96) == at(0, 2, 128) == 0
 
 
 def test_wrappers_refuse_host_tensors_and_shapes(L):
