@@ -186,3 +186,36 @@ def test_unaligned_rows(gpu):
     case("lora unaligned")
     gpu.ops.lora_add(x, d["a"], d["b"], d["ids"], d["ranks"], d["scales"], base, out, ws)
     check(host(out), want, bound)
+
+
+@pytest.mark.parametrize("typ", ["f16", "bf16"])
+@pytest.mark.parametrize("T,K,M,N,R,ids", [(1030, 264, 520, 5, 128, "mixed"), (1041, 136, 300, 3, 256, "runs"), (1030, 1500 * 8, 24, 2, 8, "runs"),
+                                           (16401, 2056, 24, 4, 8, "runs")])
+def test_many_tokens(gpu, typ, T, K, M, N, R, ids):
+    """High ranks; and parts of K that are more than one pass of a workgroup."""
+    a = inputs(T + K, T, K, M, N, R, typ, ids)
+    want, bound = reference(a)
+    case(f"lora {typ} T={T} K={K} M={M} N={N} R={R} ids={ids}")
+    got = run(gpu, a)
+    check(got, want, bound)
+    assert rel_l2(got, want) <= 2.0 ** -19
+
+
+def test_two_streams_with_their_own_workspaces(gpu):
+    """Calls of two streams at once, each as if alone."""
+    a, b = inputs(30, 900, 1032, 260, 6, 16, "f16"), inputs(31, 40, 4096, 1000, 40, 64, "bf16")
+    want = [run(gpu, a), run(gpu, b)]
+    todo = []
+    for c in (a, b):
+        d = {k: t.cuda() for k, t in c.items()}
+        ws = torch.empty(gpu.ops.lora_workspace_bytes(*d["x"].shape, d["a"].shape[1]), dtype=torch.uint8, device="cuda")
+        todo.append((torch.cuda.Stream(), d, torch.empty_like(d["base"]), ws))
+    torch.cuda.synchronize()
+    case("lora, two streams")
+    for _ in range(5):
+        for stream, d, out, ws in todo:
+            with torch.cuda.stream(stream):
+                gpu.ops.lora_add(d["x"], d["a"], d["b"], d["ids"], d["ranks"], d["scales"], d["base"], out, ws)
+    torch.cuda.synchronize()
+    for (_, _, out, _), w in zip(todo, want):
+        assert np.array_equal(host(out), w)
