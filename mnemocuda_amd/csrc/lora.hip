@@ -325,8 +325,8 @@ template <bool BF>
 static int launch_typed(const LoraArgs &a, hipStream_t s) {
     int per_part;
     const int parts = lo_parts(a.n_tokens, a.K, &per_part), tiles = (a.n_tokens + kLoTile - 1) / kLoTile;
-    // Outputs of a wave: one token takes 8.9 us by 64, 9.9 by 128, 11.4 by 256; 3001 tokens of ranks to 32 73, 69 and 75; of ranks to
-    // 256 a wave forms its operands of v for more outputs.
+    // Outputs of a wave: one token takes 8.9 us by 64, 9.9 by 128, 11.4 by 256; 3001 tokens of ranks to 32 73, 69 and 75, of
+    // 200 of 256 192 by 256 and 221 by 64: a wave forms its operands of v once.
     const int per_wave = tiles < 64 ? 64 : a.max_rank <= 64 ? 128 : 256, m_blocks = (a.M + kLoExpandWaves * per_wave - 1) / (kLoExpandWaves * per_wave);
     // a tile's adapters by workgroups of their own, as far as the chip has room for them: 1024 workgroups of either launch are at
     // work at once (61 tokens of 61 adapters take 24 us with room for 1024 of the second, 26 for 2048, 26 for 768)

@@ -41,17 +41,13 @@ constexpr float kLeastScale = -98.0f, kUnit = 0x1p-16f;
 constexpr int kStep = 64;                     // positions
 // The shares are counted in units: a step is one, and what a tile takes beside its steps (its queries, its output) are
 // a few, `cost`.  A share has kLeast or more, as far as there are any.
-constexpr int kLeast = 3;
+constexpr int kLeast = 2;
 
-// 128 rows, by 4 waves of 32 or, at head_dim 256, 8 of 16: two waves per SIMD either way.
+// 128 rows, by 4 waves of 32 or 8 of 16 (RT tiles of 16 rows each).
 constexpr int kRows = 128;
-template <int HD>
-struct Shape {
-    static constexpr int RT = HD == 256 ? 1 : 2;  // tiles of 16 rows per wave
-    static constexpr int kThreads = 64 * kRows / (16 * RT);
-    static constexpr int kKs = HD / 32, kNd = HD / 16;  // dim steps of S, dim tiles of O
-};
-__host__ __device__ constexpr int groups_of(int hd) { return hd == 256 ? 256 : 512; }  // workgroups that fill the chip
+__host__ __device__ constexpr int threads_of(int rt) { return 64 * kRows / (16 * rt); }
+__host__ __device__ constexpr int waves_of(int hd, int rt) { return hd == 64 && rt == 1 ? 4 : 2; }  // per SIMD
+__host__ __device__ constexpr int groups_of(int hd, int rt) { return 256 * 4 * 64 * waves_of(hd, rt) / threads_of(rt); }  // as many fill the chip
 
 // Workspace: two partials per workgroup (max [rows], sum [rows], O [rows][hd]): of the tile that its share goes on with, and
 // of the one that its share begins and does not end; and what these tiles are.
@@ -63,8 +59,9 @@ struct __align__(16) Cut {
     int pad[3];
 };
 // [workgroup][0: gone on with, 1: begun]
+template <int HD, int RT>
 __device__ __forceinline__ Cut *cuts_of(const PagedPromptArgs &a) {
-    return (Cut *)(a.ws + (size_t)2 * groups_of(a.c.hd) * part_floats(a.c.hd));
+    return (Cut *)(a.ws + (size_t)2 * groups_of(HD, RT) * part_floats(HD));
 }
 
 // ------------------------------------------------------------------ the row of steps
@@ -238,10 +235,9 @@ __device__ __forceinline__ h2x2 two_parts(float a, float b) {
     return x;
 }
 
-template <int KV, int HD>
-__global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(PagedPromptArgs a) {
-    using S = Shape<HD>;
-    constexpr int RT = S::RT, KS = S::kKs, ND = S::kNd, kThreads = S::kThreads, kGroups = groups_of(HD);
+template <int KV, int HD, int RT>
+__global__ void __launch_bounds__(threads_of(RT), waves_of(HD, RT)) paged_prompt_kernel(PagedPromptArgs a) {
+    constexpr int KS = HD / 32, ND = HD / 16, kThreads = threads_of(RT), kGroups = groups_of(HD, RT);  // dim steps of S, dim tiles of O
     constexpr int EB = KV == kKvF16 ? 2 : 1;
     constexpr int kWords = kStep * HD / 8;  // 16-byte words of K, and of V, of a step in LDS
     // f16: a step's words are copied straight into one buffer while the other is worked on.  int8: they are copied as
@@ -283,7 +279,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
     const int g = (int)(blockIdx.x >> 3) < per_xcd ? (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3) : blockIdx.x;
     int at = first_of(plan, g);
     const int end = first_of(plan, g + 1);
-    if (tid < 2) cuts_of(a)[2 * g + tid].n = 0;
+    if (tid < 2) cuts_of<HD, RT>(a)[2 * g + tid].n = 0;
     // of the lane's rows: the token within a tile and its head
     int tok_of[RT], head_of[RT];
 #pragma unroll
@@ -650,7 +646,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
         }
         if (tid == begins && !(begins && finishes)) {  // (by the thread that cleared it)
             const int u = at - w.unit + a.cost, g0 = group_of(plan, u);  // of the tile's first step
-            cuts_of(a)[2 * g + begins] = {group_of(plan, u + w.steps - 1) - g0 + 1, g0, w.s.start + tok0, toks * a.gqa, w.kvh, {}};
+            cuts_of<HD, RT>(a)[2 * g + begins] = {group_of(plan, u + w.steps - 1) - g0 + 1, g0, w.s.start + tok0, toks * a.gqa, w.kvh, {}};
         }
         at += units;
         if (at < end) advance(a, w);
@@ -669,12 +665,12 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 2) paged_prompt_kernel(Pa
 // Merges the partials of a tile that workgroups g0 to g0 + n - 1 had shares of: all but the last of them, here workgroups of
 // the same number, divide its rows (blockIdx.y: of which 16).  256 threads are HD / 4 lanes of four dims, times threads that
 // divide a row's partials among them where there are many, or rows.
-template <int HD>
+template <int HD, int RT>
 __global__ void __launch_bounds__(256) paged_prompt_merge_kernel(PagedPromptArgs a) {
     constexpr int D4 = HD / 4, PARTS = 256 / D4;
     __shared__ __align__(16) float so[PARTS][HD];
     __shared__ float sm[PARTS], sl[PARTS];
-    const Cut *cut = cuts_of(a) + 2 * blockIdx.x;
+    const Cut *cut = cuts_of<HD, RT>(a) + 2 * blockIdx.x;
     const Cut t = cut[1].n ? cut[1] : cut[0];
     const int n = t.n, g0 = t.g0, rows16 = min(16, t.n_rows - 16 * (int)blockIdx.y);
     if (n == 0 || rows16 <= 0) return;
@@ -747,18 +743,29 @@ __global__ void __launch_bounds__(256) paged_prompt_merge_kernel(PagedPromptArgs
     }
 }
 
+template <int KV, int HD, int RT>
+int launch_rows(const PagedPromptArgs &a, hipStream_t s) {
+    hipLaunchKernelGGL((paged_prompt_kernel<KV, HD, RT>), dim3(groups_of(HD, RT)), dim3(threads_of(RT)), 0, s, a);
+    if (int rc = check_launch("paged_attention_prompt")) return rc;
+    hipLaunchKernelGGL((paged_prompt_merge_kernel<HD, RT>), dim3(groups_of(HD, RT), kRows / 16), dim3(256), 0, s, a);
+    return check_launch("paged_attention_prompt");
+}
+// Waves of 16 rows are done with a step sooner, of 32 read each operand from LDS half as often: 3 to 6 tokens of 5 sequences
+// take 23 us by 16 and 29 by 32, 8 behind 100,000 positions 66 and 71, a prompt of 4096 592 and 500, 300 tokens 33 and 36,
+// but chunks of 400 behind long ones 2.31 and 1.89 ms.  So rows of one tile a sequence, as the average is, are taken by 16.  At
+// head_dim 256 the registers hold no more than 16; at 64 they hold four waves a SIMD of them, which is best for all (60 times 3
+// tokens 104 us and 141 by 32, 4096 299 either way), but int8 rows of 64 are too few words for 8 waves to copy.
 template <int KV, int HD>
 int launch_shape(const PagedPromptArgs &a, hipStream_t s) {
-    hipLaunchKernelGGL((paged_prompt_kernel<KV, HD>), dim3(groups_of(HD)), dim3(Shape<HD>::kThreads), 0, s, a);
-    if (int rc = check_launch("paged_attention_prompt")) return rc;
-    hipLaunchKernelGGL(paged_prompt_merge_kernel<HD>, dim3(groups_of(HD), kRows / 16), dim3(256), 0, s, a);
-    return check_launch("paged_attention_prompt");
+    if constexpr (HD == 256 || (HD == 64 && KV == kKvF16)) return launch_rows<KV, HD, 1>(a, s);
+    else if constexpr (HD == 64) return launch_rows<KV, HD, 2>(a, s);
+    else return (long long)a.n_tokens * a.gqa <= (long long)kRows * a.n_seqs ? launch_rows<KV, HD, 1>(a, s) : launch_rows<KV, HD, 2>(a, s);
 }
 
 }  // namespace
 
 size_t paged_prompt_workspace_bytes(int hd) {
-    return (size_t)groups_of(hd) * 2 * (part_floats(hd) * sizeof(float) + sizeof(Cut));
+    return (size_t)groups_of(hd, hd == 256 ? 1 : 2) * 2 * (part_floats(hd) * sizeof(float) + sizeof(Cut));
 }
 
 int launch_paged_prompt(PagedPromptArgs a, hipStream_t s) {
