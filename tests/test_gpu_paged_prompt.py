@@ -52,7 +52,13 @@ def reference(q, k, v, ks, vs, table, starts, lens, scale):
     return out
 
 
-def attend(gpu, q, k, v, ks, vs, table, starts, lens, scale, out=None, ws=None):
+def attend(gpu, q, k, v, ks, vs, table, starts, lens, scale, out=None, ws=None, wide=False):
+    """wide: with rows of no sequence behind the last, so many that the rows are not few."""
+    if wide:
+        more = 128 * len(lens) + 1
+        got = attend(gpu, np.concatenate([q, np.ones((more, *q.shape[1:]), np.float32)]), k, v, ks, vs, table, starts, lens, scale)
+        assert torch.isnan(got[len(q):]).all()
+        return got[:len(q)]
     T, nh, hd = q.shape
     if ws is None:
         ws = torch.full((gpu.ops.paged_attention_prompt_workspace_bytes(nh, k.shape[1], hd),), 255, dtype=torch.uint8, device="cuda")
@@ -93,12 +99,13 @@ EDGE_NEW = [1, 0, 2, 7, 8, 9, 1, 63, 64, 65, 1, 130, 3, 17, 40]
 EDGE_BEFORE = [0, 30, 0, 0, 1, 63, 64, 0, 0, 64, 127, 65, 600, 15, 0]
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("hd,ps,nkv,G,int8", SHAPES)
-def test_at_the_edges(gpu, hd, ps, nkv, G, int8):
+def test_at_the_edges(gpu, hd, ps, nkv, G, int8, wide):
     a = make(hd + ps + G, EDGE_NEW, EDGE_BEFORE, nkv, G, hd, ps, int8)
     case(f"paged prompt hd={hd} ps={ps} nkv={nkv} gqa={G} int8={int8} edges")
-    got = attend(gpu, *a, hd ** -0.5)
-    assert torch.equal(got, attend(gpu, *a, hd ** -0.5))
+    got = attend(gpu, *a, hd ** -0.5, wide=wide)
+    assert torch.equal(got, attend(gpu, *a, hd ** -0.5, wide=wide))
     check(host(got), reference(*a, hd ** -0.5))
 
 
@@ -131,9 +138,10 @@ def test_single_tokens_as_in_decoding(gpu, hd, ps, int8):
         assert rel_l2(got[t], one[t]) <= 2 * BAR
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("int8", [False, True])
 @pytest.mark.parametrize("hd,ps", [(64, 64), (128, 16), (256, 32)])
-def test_nothing_of_what_a_token_does_not_see(gpu, hd, ps, int8):
+def test_nothing_of_what_a_token_does_not_see(gpu, hd, ps, int8, wide):
     """NaN and infinities in later tokens' keys and values, past the end, in pages that nothing names and in the
     table's rest; tokens that see them get no numbers in the heads concerned."""
     q, k, v, ks, vs, table, starts, lens = make(7, [90, 5, 20], [10, 200, 0], 2, 3, hd, ps, int8, extra=6)
@@ -165,7 +173,7 @@ def test_nothing_of_what_a_token_does_not_see(gpu, hd, ps, int8):
         else:
             v[page, h, 5, off] = x
     case(f"paged prompt, NaN ahead, hd={hd} ps={ps} int8={int8}")
-    got = host(attend(gpu, q, k, v, ks, vs, table, starts, lens, 0.1))
+    got = host(attend(gpu, q, k, v, ks, vs, table, starts, lens, 0.1, wide=wide))
     for t in range(len(q)):
         s = int(np.searchsorted(starts, t, "right")) - 1
         p = int(lens[s] - starts[s + 1] + t)
@@ -180,8 +188,9 @@ def test_nothing_of_what_a_token_does_not_see(gpu, hd, ps, int8):
                 assert not np.isfinite(mine[:, 5]).any() and rel_l2(np.delete(mine, 5, 1), np.delete(want, 5, 1)) <= BAR, (t, h)
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("int8", [False, True])
-def test_pages_that_are_not_there(gpu, int8):
+def test_pages_that_are_not_there(gpu, int8, wide):
     """Entries outside the pool are absent positions, a row of them gives zeros, a length past the table is cut."""
     rng = np.random.default_rng(3)
     lens = np.array([300, 64, 200, 100000], np.int32)
@@ -192,7 +201,7 @@ def test_pages_that_are_not_there(gpu, int8):
     table[1, :4] = [-1, -5, 40, -2 ** 31]
     q = rng.standard_normal((90, 6, 128)).astype(np.float32)
     case(f"paged prompt, invalid pages, int8={int8}")
-    got = host(attend(gpu, q, k, v, ks, vs, table, starts, lens, 0.09))
+    got = host(attend(gpu, q, k, v, ks, vs, table, starts, lens, 0.09, wide=wide))
     check(got, reference(q, k, v, ks, vs, table, starts, lens, 0.09))
     assert not got[40:50].any()
 
@@ -245,20 +254,22 @@ def test_size_of_the_query(gpu, int8):
         assert torch.equal(attend(gpu, a[0] * np.float32(f), *a[1:], float(np.float32(0.08)) / f), base), f
 
 
-def test_value_scales_of_any_size(gpu):
+@pytest.mark.parametrize("wide", [False, True])
+def test_value_scales_of_any_size(gpu, wide):
     """int8 value scales from 1e-20 to 1e20, within a sequence too: what has weight keeps its bits."""
     q, k, v, ks, vs, table, starts, lens = make(9, [40] * 5, [110] * 5, 2, 2, 128, 16, True)
     for i, f in enumerate([1e-20, 1e-3, 1.0, 1e8, 1e20]):
         vs[table[i, :10]] *= np.float32(f)
     vs[table[2, 3], :, 7] *= np.float32(1e6)
     case("paged prompt, value scales")
-    got = host(attend(gpu, q, k, v, ks, vs, table, starts, lens, 0.09))
+    got = host(attend(gpu, q, k, v, ks, vs, table, starts, lens, 0.09, wide=wide))
     check(got, reference(q, k, v, ks, vs, table, starts, lens, 0.09))
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("int8", [False, True])
 @pytest.mark.parametrize("rise", [1, -1])
-def test_scores_that_rise_and_fall(gpu, rise, int8):
+def test_scores_that_rise_and_fall(gpu, rise, int8, wide):
     """Scores that climb (or fall) by 400 along the sequence: the reference of the softmax moves many times."""
     q, k, v, ks, vs, table, starts, lens = make(10, [100], [900], 1, 4, 64, 32, int8)
     q[:] = 1.0
@@ -271,22 +282,23 @@ def test_scores_that_rise_and_fall(gpu, rise, int8):
     else:
         k[page, 0, off] = (level[:, None] + 0 * k[page, 0, off]).astype(np.float16)
     case(f"paged prompt, scores rise={rise} int8={int8}")
-    got = host(attend(gpu, q, k, v, ks, vs, table, starts, lens, 1.0))
+    got = host(attend(gpu, q, k, v, ks, vs, table, starts, lens, 1.0, wide=wide))
     # scores of 400 round at 400 * 2^-24 some ten times: ~1e-4 of a weight
     check(got, reference(q, k, v, ks, vs, table, starts, lens, 1.0), 1e-4)
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("int8", [False, True])
-def test_queries_that_are_no_number(gpu, int8):
+def test_queries_that_are_no_number(gpu, int8, wide):
     """NaN or an infinity in a head of a token gives no numbers there and leaves all others as they are, in tiles
     that are cut, too."""
     a = make(11, [60, 2], [100, 9000], 2, 3, 128, 64, int8)
     case(f"paged prompt, NaN queries int8={int8}")
-    base = host(attend(gpu, *a, 0.1)).copy()
+    base = host(attend(gpu, *a, 0.1, wide=wide)).copy()
     q = a[0].copy()
     for t, h, x in ((0, 1, np.nan), (30, 5, np.inf), (59, 0, np.nan), (61, 4, -np.inf), (60, 2, np.nan)):
         q[t, h, 17] = x
-    got = host(attend(gpu, q, *a[1:], 0.1))
+    got = host(attend(gpu, q, *a[1:], 0.1, wide=wide))
     for t in range(62):
         for h in range(6):
             if (t, h) in ((0, 1), (30, 5), (59, 0), (61, 4), (60, 2)):
@@ -388,7 +400,8 @@ def test_scales_of_the_scores(gpu, scale, int8):
     check(host(attend(gpu, *a, scale)), reference(*a, scale))
 
 
-def test_value_scales_of_zero(gpu):
+@pytest.mark.parametrize("wide", [False, True])
+def test_value_scales_of_zero(gpu, wide):
     """Rows of zeros (scale 0) whose scores are the largest by far: their weights count in the sum.  Behind them, before
     them and alone; and scales of 2^-75 beside them."""
     q, k, v, ks, vs, table, starts, lens = make(15, [30, 30, 30, 30], [170] * 4, 1, 2, 64, 16, True)
@@ -402,7 +415,7 @@ def test_value_scales_of_zero(gpu):
         if s == 3:
             vs[table[s, rest // 16], :, rest % 16] *= np.float32(2.0 ** -75)
     case("paged prompt, value scales of zero")
-    got = host(attend(gpu, q, k, v, ks, vs, table, starts, lens, 0.05))
+    got = host(attend(gpu, q, k, v, ks, vs, table, starts, lens, 0.05, wide=wide))
     want = reference(q, k, v, ks, vs, table, starts, lens, 0.05)
     assert np.isfinite(got).all() and not got[60:90].any()
     check(got, want)
@@ -424,7 +437,8 @@ def test_starts_that_fall(gpu):
         assert (got[0] == 3).all() and (got[65] == 3).all()
 
 
-def test_value_scales_of_the_ends(gpu):
+@pytest.mark.parametrize("wide", [False, True])
+def test_value_scales_of_the_ends(gpu, wide):
     """Values of up to 2^97, and below 2^-99."""
     for e in (90, -106):
         q, k, v, ks, vs, table, starts, lens = make(17, [40, 1], [300, 900], 1, 2, 64, 16, True)
@@ -432,4 +446,4 @@ def test_value_scales_of_the_ends(gpu):
         case(f"paged prompt, value scales 2^{e}")
         a = (q, k, v, ks, vs, table, starts, lens, 0.1)
         want = reference(*a)
-        check(host(attend(gpu, *a)) * 2.0 ** -e, want * 2.0 ** -e)
+        check(host(attend(gpu, *a, wide=wide)) * 2.0 ** -e, want * 2.0 ** -e)
