@@ -10,6 +10,9 @@
 // looked at: a thread compares the largest of its 16 logits with the workgroup's n-th best so far.  Lists are
 // merged as two halves of a bitonic sequence.
 // Rows are cut into parts where they do not fill the chip; a second launch joins the parts.
+//
+// Bound by reading the logits once, which are loaded past the caches: 1201 rows of 151,936 take 132 us, 5.5 TB/s.  Few rows
+// are bound by the two launches and what each waits for: one row takes 14 us, 31 of 32,003 12.
 #include <float.h>
 #include <math.h>
 

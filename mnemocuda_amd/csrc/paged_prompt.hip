@@ -4,21 +4,29 @@
 // Sequence s has n tokens, rows starts[s] .. starts[s+1]-1 of q, the last of them at position L - 1 (L = lens[s]).
 // Token i, at p = L - n + i:  out = sum_{j<=p} P_j v_j / sum_{j<=p} P_j,  P_j = exp(scale q.k_j - m).
 //
-// A tile is the query heads of one KV head for a power of two of tokens, 128 rows (64 at head_dim 256): 4 waves of
-// 32 (16) rows share the K and V of 64 positions, a step, in LDS.  The steps of all tiles stand in one row,
-// [sequence][KV head][tile][step], which the workgroups divide into equal shares, whatever the lengths are: the sum
-// of a sequence's steps has a closed form, so every workgroup finds its share by itself.  A tile that several
-// shares cut leaves partials (max, sum, O) in memory, which a second launch merges.
+// A tile is the query heads of one KV head for a power of two of tokens, 128 rows, whose waves share the K and V of 64
+// positions, a step, in LDS.  The steps of all tiles stand in one row, [sequence][KV head][tile][step], which the
+// workgroups divide into equal shares, whatever the lengths are: the sum of a sequence's steps has a closed form, so
+// every workgroup finds its share by itself.  A tile that several shares cut leaves partials (max, sum, O) in memory,
+// which a second launch merges.
 //
 // S^T = K Q^T (positions x rows) leaves a lane with positions of one row, which is how O^T = V^T P^T (dims x rows)
 // wants P^T, when the K rows of a tile are picked so: lane row m of tile t is position 16 (m/4) + 4t + m%4, so that
 // a lane's positions over the tiles are 16 consecutive ones.  Words of 16 bytes in LDS are permuted within their
 // row, so that the 16 lanes of an operand's column lie in different banks.
 //
-// Precision: as in paged_attn.hip, Q is scaled by a power of two per row and split into two f16 parts; f16 pages: P likewise,
-// relative to a reference that follows the maximum only when a score exceeds it by 2^kSlack, and 2^kLift at the
-// reference.  int8 pages: K enters as f16 (exact), P times the value's scale as three bf16 parts (24 bits,
-// the range of fp32), V as bf16 (exact).
+// Precision: Q is scaled by a power of two per row and split into two f16 parts, P likewise, relative to a reference
+// that moves only when a weight (int8: times its value's scale, by which P is multiplied) exceeds it by 2^kSlack, and
+// is 2^kLift at the reference: 22 bits or more of each.  K and V enter as f16, which is exact.  Sums are fp32, the
+// weights' with what their additions lose.  So an output is off by 4e-7 of its size (int8 1e-6), fp32 products of
+// the same values by 7e-7 to 3e-6.
+//
+// Long calls are bound by the matrix cores: two products for each.  4096 tokens of 64 heads of 128 on 4 KV heads, 275 GFLOP
+// and 550 executed, take 500 us, 1100 TFLOP/s; a large f16 product of the library's runs at 1150 to 1180, what the card's
+// power allows with such values (both are a third faster with zeros).  Of 2000 tokens' 160 us some 25 are partials
+// written and merged.  Short calls are bound by the chain of a share: plan, table, K and V, two dependent products and a
+// softmax per step, partials, second launch: one token behind 500 positions takes 12 us, 21 tokens of 5 sequences
+// behind 13,000 positions 23.
 #include <limits.h>
 #include <math.h>
 
@@ -40,7 +48,8 @@ constexpr float kSlack = 5.0f, kLift = 9.0f;  // powers of two
 constexpr float kLeastScale = -98.0f, kUnit = 0x1p-16f;
 constexpr int kStep = 64;                     // positions
 // The shares are counted in units: a step is one, and what a tile takes beside its steps (its queries, its output) are
-// a few, `cost`.  A share has kLeast or more, as far as there are any.
+// a few, `cost`.  A share has kLeast or more, as far as there are any: one token behind 500 positions takes 10.8, 11.6 and
+// 12.5 us with 1, 2 and 3, five behind 3000 17.5, 16.0 and 16.9.
 constexpr int kLeast = 2;
 
 // 128 rows, by 4 waves of 32 or 8 of 16 (RT tiles of 16 rows each).
