@@ -42,10 +42,11 @@ namespace mnemo {
 namespace {
 
 constexpr float kSlack = 5.0f, kLift = 9.0f;  // powers of two
-// int8: value scales below 2^-98 count as it for the reference, so that a weight is below 2^112.  The weights' sum is kept in
-// units of 2^16: those of 2^30 positions stay in range, and beside
-// scales of 2^90 weights down to 2^-29 of the largest.
-constexpr float kLeastScale = -98.0f, kUnit = 0x1p-16f;
+// int8: a reference moves when a weight times its value's scale is more than kMost, which is seen from the products themselves
+// (1.87 ms for three long chunks; 1.90 with the products' logarithms looked at first).  Value scales below 2^-98 count as it for the
+// reference, and the sum of eight weights is below 2^112 (in its unit: kMost / kMostSum).  The weights' sum is kept in
+// units of 2^16: those of 2^30 positions stay in range, and beside scales of 2^90 weights down to 2^-29 of the largest.
+constexpr float kLeastScale = -98.0f, kUnit = 0x1p-16f, kMost = 0x1p14f, kMostSum = 0x1p-82f;
 constexpr int kStep = 64;                     // positions
 // The shares are counted in units: a step is one, and what a tile takes beside its steps (its queries, its output) are
 // a few, `cost`.  A share has kLeast or more, as far as there are any: one token behind 500 positions takes 10.8, 11.6 and
@@ -529,53 +530,77 @@ __global__ void __launch_bounds__(threads_of(RT), waves_of(HD, RT)) paged_prompt
                         const int live = min(max(lim[rt] - (p0 + first), -1), 7) + 1;
                         seen = (uint32_t)(there >> first) & ((1u << live) - 1);
                     }
-                    float top = -INFINITY;  // of the lane's scores
                     f4 f[2], vs[2];
-                    if (KV == kKvF16) {
-                        if (!full) {
-#pragma unroll
-                            for (int j = 0; j < 8; j++) s[rt][j / 4][j & 3] = seen >> j & 1 ? s[rt][j / 4][j & 3] : -INFINITY;
-                        }
-#pragma unroll
-                        for (int j = 0; j < 8; j++) top = fmaxf(top, s[rt][j / 4][j & 3]);
-                        top *= c[rt];
-                    } else {
+                    if (KV == kKvInt8) {
 #pragma unroll
                         for (int t = 0; t < 2; t++) {
                             f[t] = *(const f4 *)&ksc[first + 4 * t] * c[rt];
                             vs[t] = *(const f4 *)&vsc[first + 4 * t];
-                            const f4 lg = *(const f4 *)&vlg[first + 4 * t];
+                        }
+                    }
+                    if (!full) {
 #pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                const float y = fmaf(s[rt][t][i], f[t][i], lg[i]);
-                                top = fmaxf(top, full || (seen >> (4 * t + i) & 1) ? y : -INFINITY);
+                        for (int j = 0; j < 8; j++) {
+                            const bool in = seen >> j & 1;
+                            s[rt][j / 4][j & 3] = in ? s[rt][j / 4][j & 3] : -INFINITY;
+                            if (KV == kKvInt8) {  // (the scales of a position that is not seen may be no numbers)
+                                f[j / 4][j & 3] = in ? f[j / 4][j & 3] : 1.0f;
+                                vs[j / 4][j & 3] = in ? vs[j / 4][j & 3] : 0.0f;
                             }
                         }
                     }
-                    if (__any(top > m[rt] + kSlack)) {  // uniform
+                    // moves the reference of rows that have need of it, which is a row's own doing, to their largest score
+                    auto move = [&](float top, bool need) {
                         top = max_row(top);
-                        const float mn = top > m[rt] + kSlack ? top : m[rt];  // a row's own doing
+                        const float mn = need ? top : m[rt];
                         const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - mn);
                         l[rt] *= al;
                         lost[rt] *= al;
                         m[rt] = mn;
 #pragma unroll
                         for (int i = 0; i < ND; i++) o[rt][i] *= al;
-                    }
-                    const float ref = m[rt] == -INFINITY ? 0.0f : m[rt] - kLift;
-                    float p[8], sum[4];
+                    };
+                    float p[8], more;
+                    auto weigh = [&] {
+                        const float ref = m[rt] == -INFINITY ? 0.0f : m[rt] - kLift;
+                        float sum[4];
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        float x = fmaf(s[rt][j / 4][j & 3], KV == kKvF16 ? c[rt] : f[j / 4][j & 3], -ref);
-                        if (KV == kKvInt8 && !full) x = seen >> j & 1 ? x : -INFINITY;
-                        x = __builtin_amdgcn_exp2f(x);
-                        sum[j & 3] = j < 4 ? x : sum[j & 3] + x;
-                        // (the scale of a position that is not seen may be no number)
-                        if (KV == kKvInt8) x = full || (seen >> j & 1) ? x * vs[j / 4][j & 3] : 0.0f;
-                        p[j] = x;
+                        for (int j = 0; j < 8; j++) {
+                            const float x = __builtin_amdgcn_exp2f(fmaf(s[rt][j / 4][j & 3], KV == kKvF16 ? c[rt] : f[j / 4][j & 3], -ref));
+                            sum[j & 3] = j < 4 ? x : sum[j & 3] + x;
+                            p[j] = KV == kKvInt8 ? x * vs[j / 4][j & 3] : x;
+                        }
+                        more = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                        if (KV == kKvInt8) more *= kUnit;
+                    };
+                    if (KV == kKvF16) {
+                        float top = -INFINITY;  // of the lane's scores
+#pragma unroll
+                        for (int j = 0; j < 8; j++) top = fmaxf(top, s[rt][j / 4][j & 3]);
+                        top *= c[rt];
+                        if (__any(top > m[rt] + kSlack)) {  // uniform
+                            top = max_row(top);
+                            move(top, top > m[rt] + kSlack);
+                        }
+                        weigh();
+                    } else {
+                        weigh();
+                        float most = more * kMostSum;
+#pragma unroll
+                        for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(p[j]));
+                        const bool need = most > kMost || m[rt] == -INFINITY;
+                        if (__any(need)) {  // uniform
+                            float top = -INFINITY;
+#pragma unroll
+                            for (int t = 0; t < 2; t++) {
+                                const f4 lg = *(const f4 *)&vlg[first + 4 * t];
+#pragma unroll
+                                for (int i = 0; i < 4; i++) top = fmaxf(top, fmaf(s[rt][t][i], f[t][i], lg[i]));
+                            }
+                            move(top, max_row(need ? 1.0f : 0.0f) != 0.0f);
+                            weigh();
+                        }
                     }
-                    float more = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    if (KV == kKvInt8) more *= kUnit;
                     const float to = l[rt] + more;
                     lost[rt] += more - (to - l[rt]);  // (exact while l is the larger)
                     l[rt] = to;
