@@ -11,7 +11,7 @@
 // merged as two halves of a bitonic sequence.
 // Rows are cut into parts where they do not fill the chip; a second launch joins the parts.
 //
-// Bound by reading the logits once, which are loaded past the caches: 1201 rows of 151,936 take 129 us, 5.7 TB/s.  Few rows
+// Bound by reading the logits once, which are loaded past the caches: 1201 rows of 151,936 take 122 to 129 us, 5.7 to 6.0 TB/s.  Few rows
 // are bound by the two launches and what each waits for: one row takes 14 us, 31 of 32,003 12; short rows by the lists'
 // beginnings: 1000 of 32,003 take 24 us without, 28 with 5 tokens each and 38 with 20.
 #include <float.h>
