@@ -52,6 +52,10 @@ constexpr int kStep = 64;                     // positions
 // a few, `cost`.  A share has kLeast or more, as far as there are any: one token behind 500 positions takes 10.8, 11.6 and
 // 12.5 us with 1, 2 and 3, five behind 3000 17.5, 16.0 and 16.9.
 constexpr int kLeast = 2;
+// Where one sequence alone has tokens, and no workgroup gets more than kUneven units, or half, above the average, whole tiles are
+// dealt out instead, in kRounds at most: nothing is cut, nothing merged.  1300 tokens of 64 heads of 128 take 81 us and 87 in
+// shares, 2000 133 and 155, 4096 473 and 498; where it is less even 600 47 and 45, 1000 67 and 65.
+constexpr int kUneven = 8, kRounds = 8;
 
 // 128 rows, by 4 waves of 32 or 8 of 16 (RT tiles of 16 rows each).
 constexpr int kRows = 128;
@@ -119,7 +123,15 @@ struct Plan {
     bool short_;     // lane: a sequence of its has tokens before position 0
     int per;         // sequences per lane of the sums
     int before;      // lane: units before its sequences
+    int alone;       // the sequence whose tiles are taken whole, or -1
 };
+// of tile j: the positions that its last token sees
+__device__ __forceinline__ int tile_steps(const Seq &s, int tl, int j) {
+    return (s.len - s.n + min((j + 1) << tl, s.n) + kStep - 1) / kStep;
+}
+// Round r of workgroup g of as many: the tiles of all KV heads are dealt out from the longest, in turn forwards and backwards.
+__device__ __forceinline__ int dealt(int r, int g, int groups) { return r * groups + (r & 1 ? groups - 1 - g : g); }
+
 __device__ __forceinline__ Plan make_plan(const PagedPromptArgs &a, int groups) {
     Plan p;
     p.per = (a.n_seqs + 63) / 64;
@@ -145,6 +157,22 @@ __device__ __forceinline__ Plan make_plan(const PagedPromptArgs &a, int groups) 
     p.groups = max(min(groups, p.total / kLeast), 1);
     p.base = p.total / p.groups;
     p.more = p.total - p.base * p.groups;
+    p.alone = -1;
+    const uint64_t some = __ballot(sum > 0);
+    const int mean = p.total / groups;
+    if (p.per == 1 && __popcll(some) == 1 && mean >= kUneven) {  // (a sample of the workgroups, with the first and the last)
+        const int seq = __ffsll((unsigned long long)some) - 1;
+        const Seq s = seq_of(a, seq);
+        const int each = tiles_of(s, a.tl), g = lane_id() * (groups - 1) / 63;
+        if (s.n <= s.len && each * a.c.nkv <= kRounds * groups) {
+            int load = 0;
+            for (int r = 0; r < kRounds; r++) {
+                const int i = dealt(r, g, groups);
+                if (i < each * a.c.nkv) load += tile_steps(s, a.tl, each - 1 - i / a.c.nkv) + a.cost;
+            }
+            if (!__any(load > mean + min(kUneven, mean / 2))) p.alone = seq;
+        }
+    }
     return p;
 }
 __device__ __forceinline__ int first_of(const Plan &p, int g) {
@@ -154,11 +182,6 @@ __device__ __forceinline__ int first_of(const Plan &p, int g) {
 __device__ __forceinline__ int group_of(const Plan &p, int u) {
     const int longer = p.more * (p.base + 1);
     return u < longer ? u / (p.base + 1) : p.more + (u - longer) / p.base;
-}
-
-// of tile j: the positions that its last token sees
-__device__ __forceinline__ int tile_steps(const Seq &s, int tl, int j) {
-    return (s.len - s.n + min((j + 1) << tl, s.n) + kStep - 1) / kStep;
 }
 
 struct Where {
@@ -196,6 +219,16 @@ __device__ __forceinline__ Where find(const PagedPromptArgs &a, const Plan &p, i
     w.unit = at - units_before(w.s, a.tl, a.cost, lo);
     w.steps = tile_steps(w.s, a.tl, lo);
     return w;
+}
+// The tile of round r, where whole tiles are dealt out.
+__device__ __forceinline__ bool deal(const PagedPromptArgs &a, Where &w, int r, int g, int groups) {
+    const int each = tiles_of(w.s, a.tl), i = dealt(r, g, groups), j = i / a.c.nkv;
+    if (j >= each) return false;
+    w.tile = each - 1 - j;
+    w.kvh = i - j * a.c.nkv;
+    w.unit = 0;
+    w.steps = tile_steps(w.s, a.tl, w.tile);
+    return true;
 }
 // The tile after w, from its first unit on (there is one).
 __device__ __forceinline__ void advance(const PagedPromptArgs &a, Where &w) {
@@ -288,7 +321,7 @@ __global__ void __launch_bounds__(threads_of(RT), waves_of(HD, RT)) paged_prompt
     const int per_xcd = (plan.groups + 7) / 8;
     const int g = (int)(blockIdx.x >> 3) < per_xcd ? (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3) : blockIdx.x;
     int at = first_of(plan, g);
-    const int end = first_of(plan, g + 1);
+    int end = first_of(plan, g + 1);
     if (tid < 2) cuts_of<HD, RT>(a)[2 * g + tid].n = 0;
     // of the lane's rows: the token within a tile and its head
     int tok_of[RT], head_of[RT];
@@ -302,7 +335,13 @@ __global__ void __launch_bounds__(threads_of(RT), waves_of(HD, RT)) paged_prompt
     const int tok_first = __builtin_amdgcn_readfirstlane(tok_of[0]), tok_last = __builtin_amdgcn_readlane(tok_of[RT - 1], 15);
 
     Where w;
-    if (at < end) w = find(a, plan, at);
+    int round = 0;
+    if (plan.alone >= 0) {
+        w.seq = plan.alone;
+        w.s = seq_of(a, w.seq);
+        at = 0;
+        end = deal(a, w, 0, g, kGroups) ? INT_MAX : 0;
+    } else if (at < end) w = find(a, plan, at);
     while (at < end) {
         const int units = min(end - at, w.steps + a.cost - w.unit);
         const int step = max(w.unit - a.cost, 0), n = max(w.unit + units - a.cost, 0) - step;
@@ -683,7 +722,9 @@ __global__ void __launch_bounds__(threads_of(RT), waves_of(HD, RT)) paged_prompt
             cuts_of<HD, RT>(a)[2 * g + begins] = {group_of(plan, u + w.steps - 1) - g0 + 1, g0, w.s.start + tok0, toks * a.gqa, w.kvh, {}};
         }
         at += units;
-        if (at < end) advance(a, w);
+        if (plan.alone >= 0) {
+            if (!deal(a, w, ++round, g, kGroups)) break;
+        } else if (at < end) advance(a, w);
     }
 
     if (__any(plan.short_))  // tokens before position 0: zeros

@@ -447,3 +447,45 @@ def test_value_scales_of_the_ends(gpu, wide):
         a = (q, k, v, ks, vs, table, starts, lens, 0.1)
         want = reference(*a)
         check(host(attend(gpu, *a, wide=wide)) * 2.0 ** -e, want * 2.0 ** -e)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("n,before,nkv,G,hd,ps", [(1700, 0, 4, 16, 128, 64), (1305, 0, 4, 16, 64, 16), (2003, 0, 2, 16, 256, 128), (2048, 777, 4, 16, 128, 16),
+                                                  (2300, 0, 9, 5, 64, 64), (4099, 0, 4, 8, 128, 32), (3500, 10, 16, 3, 128, 64)])
+def test_one_long_prompt(gpu, n, before, nkv, G, hd, ps, int8):
+    """Prompts whose tiles are dealt out whole, and next to them others; with rows that take nothing beside them.  Some heads
+    of the first and the last KV head are looked at."""
+    a = make(n + hd, [0, n, 0], [50, before, 0], nkv, G, hd, ps, int8)
+    q, k, v, ks, vs, table, starts, lens = a
+    case(f"paged prompt, one of {n} behind {before}, nkv={nkv} gqa={G} hd={hd} ps={ps} int8={int8}")
+    got = attend(gpu, *a, hd ** -0.5)
+    assert torch.equal(got, attend(gpu, *a, hd ** -0.5))
+    got = host(got)
+    assert np.isfinite(got).all()
+    for h in (0, nkv - 1):
+        some = [h * G, h * G + G - 1]
+        of = lambda x: None if x is None else x[:, h:h + 1]  # noqa: E731
+        check(got[:, some], reference(q[:, some], of(k), of(v), of(ks), of(vs), table, starts, lens, hd ** -0.5))
+
+
+def test_one_long_prompt_that_ends_early(gpu):
+    """More tokens than positions; values that are no numbers ahead of most tokens; a page that is not there."""
+    q, k, v, _, _, table, starts, lens = make(77, [1800], [0], 4, 16, 128, 64, False)
+    v[table[0, 1700 // 64], 1, 7, 1700 % 64] = np.nan
+    table[0, 5] = -1
+    case("paged prompt, one long, NaN ahead")
+    got = host(attend(gpu, q, k, v, None, None, table, starts, lens, 0.09))
+    assert np.isnan(got[1700:, 16:32, 7]).all()
+    got[1700:, 16:32, 7] = 0
+    assert np.isfinite(got).all()
+    for h in (0, 1):
+        some = [16 * h, 16 * h + 15]
+        want = reference(q[:, some], k[:, h:h + 1], np.nan_to_num(v[:, h:h + 1]), None, None, table, starts, lens, 0.09)
+        if h == 1:
+            want[1700:, :, 7] = 0
+        check(got[:, some], want)
+    lens[0] = 1500
+    case("paged prompt, one long, 300 tokens before the first position")
+    got = host(attend(gpu, q, k, v, None, None, table, starts, lens, 0.09))
+    assert not got[:300].any()
+    check(got[300:, [0, 15]], reference(q[300:, [0, 15]], k[:, :1], v[:, :1], None, None, table, starts - np.array([0, 300], np.int32), lens, 0.09))
