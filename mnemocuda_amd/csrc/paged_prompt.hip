@@ -8,7 +8,7 @@
 // positions, a step, in LDS.  The steps of all tiles stand in one row, [sequence][KV head][tile][step], which the
 // workgroups divide into equal shares, whatever the lengths are: the sum of a sequence's steps has a closed form, so
 // every workgroup finds its share by itself.  A tile that several shares cut leaves partials (max, sum, O) in memory,
-// which a second launch merges.
+// which a second launch merges.  A long prompt alone is dealt out in whole tiles where they balance.
 //
 // S^T = K Q^T (positions x rows) leaves a lane with positions of one row, which is how O^T = V^T P^T (dims x rows)
 // wants P^T, when the K rows of a tile are picked so: lane row m of tile t is position 16 (m/4) + 4t + m%4, so that
@@ -22,9 +22,8 @@
 // the same values by 7e-7 to 3e-6.
 //
 // Long calls are bound by the matrix cores: two products for each.  4096 tokens of 64 heads of 128 on 4 KV heads, 275 GFLOP
-// and 550 executed, take 500 us, 1100 TFLOP/s; a large f16 product of the library's runs at 1150 to 1180, what the card's
-// power allows with such values (both are a third faster with zeros).  Of 2000 tokens' 160 us some 25 are partials
-// written and merged.  Short calls are bound by the chain of a share: plan, table, K and V, two dependent products and a
+// and 550 executed, take 475 us, 1160 TFLOP/s; a large f16 product of the library's runs at 1150 to 1180, what the card's
+// power allows with such values (both are a third faster with zeros).  Short calls are bound by the chain of a share: plan, table, K and V, two dependent products and a
 // softmax per step, partials, second launch: one token behind 500 positions takes 12 us, 21 tokens of 5 sequences
 // behind 13,000 positions 23.
 #include <limits.h>
