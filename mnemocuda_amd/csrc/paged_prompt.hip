@@ -23,9 +23,9 @@
 //
 // Long calls are bound by the matrix cores: two products for each.  4096 tokens of 64 heads of 128 on 4 KV heads, 275 GFLOP
 // and 550 executed, take 475 us, 1160 TFLOP/s; a large f16 product of the library's runs at 1150 to 1180, what the card's
-// power allows with such values (both are a third faster with zeros).  Short calls are bound by the chain of a share: plan, table, K and V, two dependent products and a
-// softmax per step, partials, second launch: one token behind 500 positions takes 12 us, 21 tokens of 5 sequences
-// behind 13,000 positions 23.
+// power allows with such values (both are a third faster with zeros).  Short calls are bound by the chain of a share: plan,
+// table, K and V, two dependent products and a softmax per step, partials, second launch: one token behind 500 positions
+// takes 12 us, 21 tokens of 5 sequences behind 13,000 positions 23.
 #include <limits.h>
 #include <math.h>
 
