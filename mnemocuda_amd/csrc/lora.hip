@@ -11,7 +11,9 @@
 // take 70 us with nothing in the caches, 8000 tokens 145 (4.5 TB/s; a copy reaches 5.2), of which the first launch, x, is a
 // third.  Few tokens are bound by what a launch waits for in turn, ids, ranks, words and the other launch: one token 9 us,
 // 61 of as many adapters 24, where lines of B of which a low rank has a part are read whole as well.  Asking for B before v
-// is known costs more in registers than it hides (24 and 23, but one token 9 and 9.5, 3001 70 and 74).
+// is known costs more in registers than it hides (24 and 23, but one token 9 and 9.5, 3001 70 and 74).  High ranks of many
+// tokens are bound by A and B, which every tile reads again from the L2 caches: 3001 tokens of rank 200 take 192 us, 4.9 TB/s of
+// them (the next words of B asked for ahead of the products: 193 f16, 225 bf16, for spilled registers).
 //
 // Precision: x and v, fp32, meet f16 adapters as two f16 parts, scaled by a power of two per token so that the largest
 // is in [2^13, 2^14) (parts are off by 2^-38 of the largest, or 2^-23 of the value), bf16 adapters as three bf16 parts (exact).
