@@ -23,7 +23,8 @@
 namespace mnemo {
 
 // An expert's key: c with its lowest ten bits replaced by what orders its index, smaller before larger.  Keys are
-// compared as numbers.  kNone is below all of them.
+// compared as numbers, no two of which are equal (only 0 and -0 would be, and a c below 0, made of a fp32 number, is
+// never so small that its key is -0).  kNone is below all of them.
 constexpr double kNone = -0x1.fffffffffffffp1023;
 __device__ __forceinline__ double make_key(double c, int e) {
     const uint64_t b = __builtin_bit_cast(uint64_t, fmin(c, -kNone));  // (an infinity has no bits to spare)
@@ -33,7 +34,6 @@ __device__ __forceinline__ int key_expert(double key) {
     const uint64_t b = __builtin_bit_cast(uint64_t, key);
     return (int)(b >> 63 ? b & 1023 : 1023 - (b & 1023));
 }
-__device__ __forceinline__ uint32_t low_word(double v) { return (uint32_t)__builtin_bit_cast(uint64_t, v); }
 template <int CTRL>
 __device__ __forceinline__ double dpp_double(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
@@ -201,12 +201,9 @@ __global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
             for (int t = 0; t < n; t++) half[t] = fmax(half[t], half[t + n]);
         const double best = max_token<L>(half[0]);
         if (gl == j && best > kNone) mine_idx = key_expert(best);
-        // the lower words differ in the index; what is left of one that goes is the most negative upper word
+        // (whole keys: the index's bits alone are the same for a key of e above 0 and one of 1023 - e below it)
 #pragma unroll
-        for (int t = 0; t < N; t++) {
-            const uint64_t b = __builtin_bit_cast(uint64_t, key[t]);
-            key[t] = (uint32_t)b == low_word(best) ? __builtin_bit_cast(double, 0xffefffffffffffffull) : key[t];
-        }
+        for (int t = 0; t < N; t++) key[t] = key[t] == best ? kNone : key[t];
     }
     double w = 0.0;
     if (mine_idx >= 0) {

@@ -1,0 +1,111 @@
+"""Routing of many tokens where scores of both signs are chosen, against the formula in 64 bits.
+
+Logits are whole numbers and biases eighths, so that two scores are equal or far apart: the order has no rounding in it.
+A weight is a quotient in 64 bits rounded to fp32 once: off by 2^-24 of it, and by 2^-150 where it has no normal number;
+the bound is twice that."""
+import numpy as np
+import pytest
+import torch
+
+from tests.gpu_util import case, dev, host
+
+pytestmark = pytest.mark.gpu
+
+
+def reference(z, k, sigmoid=False, bias=None, groups=1, top_groups=1, best=1):
+    """(ids, renormalised weights).  Without a bias the order is that of the logits, with groups that score two experts
+    that of the scores."""
+    T, E = z.shape
+    z64 = z.astype(np.float64)
+    with np.errstate(over="ignore"):
+        p = 1 / (1 + np.exp(-z64)) if sigmoid else np.exp(z64 - z64.max(1, keepdims=True))
+    if not sigmoid:
+        p /= p.sum(1, keepdims=True)
+    if bias is not None:
+        c = p + bias.astype(np.float64)
+    else:
+        c = p.copy() if best == 2 and top_groups < groups else z64.copy()
+    c[z64 == -np.inf] = -np.inf
+    if bias is not None:
+        c[:, bias == -np.inf] = -np.inf
+    if top_groups < groups:
+        by = -np.sort(-c.reshape(T, groups, -1), axis=2)
+        score = by[:, :, :best].sum(2)
+        place = np.empty((T, groups), int)
+        np.put_along_axis(place, np.argsort(-score, axis=1, kind="stable"), np.arange(groups)[None], 1)
+        c = np.where(np.repeat(place < top_groups, E // groups, axis=1), c, -np.inf)
+    idx = np.argsort(-c, axis=1, kind="stable")[:, :k].astype(np.int32)
+    there = np.take_along_axis(c, idx, 1) > -np.inf
+    w = np.where(there, np.take_along_axis(p, idx, 1), 0.0)
+    total = w.sum(1, keepdims=True)
+    return np.where(there, idx, -1), np.divide(w, total, out=np.zeros_like(w), where=total > 0)
+
+
+def check(gpu, z, k, **how):
+    T = z.shape[0]
+    idx, w = torch.empty((T, k), dtype=torch.int32, device="cuda"), torch.empty((T, k), device="cuda")
+    bias = how.get("bias")
+    gpu.ops.moe_route(dev(z), idx, w, how.get("sigmoid", False), None if bias is None else dev(bias), how.get("groups", 1),
+                      how.get("top_groups", 1), how.get("best", 1))
+    want, weights = reference(z, k, **how)
+    got = host(idx)
+    wrong = np.flatnonzero((got != want).any(1))
+    assert wrong.size == 0, f"{wrong.size} of {T} tokens, the first: {got[wrong[0]]} for {want[wrong[0]]}"
+    assert (np.abs(host(w) - weights) <= 2.0 ** -23 * weights + 2.0 ** -149).all()
+
+
+def live(rng, T, E):
+    """Some 20 experts a row: ten with, where there are such, the one whose index has the complement of their bits, and others."""
+    on = rng.random((T, E)) < 6 / E
+    e = rng.integers(max(0, min(1023 - (E - 1), E - 1)), E, (T, 10))
+    np.put_along_axis(on, e, True, 1)
+    np.put_along_axis(on, np.clip(1023 - e, 0, E - 1), True, 1)
+    return on
+
+
+SIZES = [(T, E) for T in (7, 2050, 16387) for E in (512, 513, 520, 768, 1023, 1024)]
+
+
+@pytest.mark.parametrize("T,E", SIZES)
+def test_a_choice_leaves_the_others(gpu, T, E):
+    """The best expert of a row, e, is above 0, the second, 1023 - e, below 0: their indices' bits are each other's complement."""
+    rng = np.random.default_rng(T + E)
+    z = np.full((T, E), -10.0, np.float32)
+    lo = max(0, 1023 - (E - 1))
+    for t in range(T):
+        e = int(rng.integers(min(lo, E - 1), E))
+        z[t, (e * 3 + 1) % E] = -2.0
+        z[t, min(max(1023 - e, 0), E - 1)] = -1.0
+        z[t, e] = 1.0
+    z[0, [0, E - 1]] = [1.0, -1.0]
+    case(f"route pair T={T} E={E}")
+    check(gpu, z, 3)
+    check(gpu, z, 3, sigmoid=True)
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("T,E", SIZES)
+def test_choices_of_both_signs(gpu, T, E, sigmoid):
+    """A few logits above 0 and the rest below, of whole numbers, many of them equal; rows of which a mask leaves some 20."""
+    rng = np.random.default_rng(T + E + sigmoid)
+    z = np.rint(rng.normal(-3.5, 1.5, (T, E))).astype(np.float32)
+    z[::3][~live(rng, len(z[::3]), E)] = -np.inf
+    case(f"route signs T={T} E={E} sigmoid={sigmoid}")
+    check(gpu, z, 16, sigmoid=sigmoid)
+    check(gpu, z, 8, sigmoid=sigmoid)
+
+
+@pytest.mark.parametrize("groups,top_groups", [(1, 1), (4, 2)])
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("T,E", [(T, E) for T in (7, 2050, 16387) for E in (512, 520, 768, 1024)])
+def test_biases_beside_which_scores_vanish(gpu, T, E, sigmoid, groups, top_groups):
+    """Scores of 1e-87 or less beside biases of eighths of both signs, few of them above 0: the bias alone orders the experts."""
+    rng = np.random.default_rng(T + E + groups)
+    z = np.full((T, E), -200.0, np.float32)
+    z[::2][~live(rng, len(z[::2]), E)] = -np.inf
+    if not sigmoid:
+        z[np.arange(T), rng.integers(0, E, T)] = 100.0
+    bias = (np.rint(8 * rng.normal(-2.5, 1.2, E)) / 8).astype(np.float32)
+    bias[bias == 0] = 0.125  # (a score beside no bias is one)
+    case(f"route biases T={T} E={E} sigmoid={sigmoid} groups={groups}/{top_groups}")
+    check(gpu, z, 9, sigmoid=sigmoid, bias=bias, groups=groups, top_groups=top_groups)
