@@ -489,7 +489,8 @@ int mnemo_paged_attention_prompt(const float *q, const void *k_pages, const void
 /* Routing of n_tokens tokens from their router logits [n_tokens][n_experts], for mnemo_moe_prefill:
  *   s_e = 1 / (1 + exp(-z_e)) (score 1) or exp(z_e) / sum_f exp(z_f) (score 0);  c_e = s_e + bias[e]
  *   The experts are n_groups runs of n_experts / n_groups.  A group scores the sum of its group_best
- *   (1 or 2) largest c; the top_groups best groups are kept (ties to the lower index).
+ *   (1 or 2; 1 for groups of one expert) largest c, -inf where fewer of its experts can be chosen; the
+ *   top_groups best groups are kept (ties to the lower index).
  *   topk_idx[t] = the k experts of largest c in the kept groups, best first, ties to the lower index
  *   topk_w[t] = scale * s of those, divided by their sum where renormalise is not 0
  * (bias NULL: none.)  The choice is made in 64 bits, c within 2^-42 of each other being a tie.  An expert whose logit or bias is

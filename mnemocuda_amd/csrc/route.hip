@@ -2,7 +2,7 @@
 //
 // For every token, from its logits z[e]:
 //   s_e = 1 / (1 + exp(-z_e))  or  exp(z_e) / sum_f exp(z_f),   c_e = s_e + bias_e
-//   a group of experts scores the sum of its one or two largest c; the best groups are kept
+//   a group of experts scores the sum of its one or two largest c (-inf where it has too few); the best groups are kept
 //   the k largest c among them are chosen, ties to the lower index
 //   w = s of the chosen, / their sum where asked for, * scale
 // Without a bias, and with groups that score one expert, c grows with z: the choice is made among the logits.
@@ -179,8 +179,9 @@ __global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
             b2 = fmax(fmin(b1, o1), fmax(b2, o2));
             b1 = fmax(b1, o1);
         }
-        const double score = a.best == 2 && b2 > -INFINITY ? b1 + b2 : b1;
-        const double gkey = g < a.n_groups && b1 > -INFINITY ? make_key(score, g) : kNone;
+        // (of two experts of which one is masked: -inf, whatever the other scores)
+        const double score = a.best == 1 || a.per_group == 1 ? b1 : b2 > -INFINITY ? b1 + b2 : -INFINITY;
+        const double gkey = g < a.n_groups ? make_key(fmax(score, kNone), g) : kNone;
         int better = 0;
         for (int o = 0; o < a.n_groups; o++)
             better += __shfl(gkey, (lane & ~(L - 1)) + (o << a.lanes_log)) > gkey;

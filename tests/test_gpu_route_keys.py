@@ -1,6 +1,7 @@
 """Routing of many tokens where scores of both signs are chosen, against the formula in 64 bits.
 
-Logits are whole numbers and biases eighths, so that two scores are equal or far apart: the order has no rounding in it.
+Logits are whole numbers or eighths, and biases eighths where they alone decide, so that two scores are equal or far apart:
+the order has no rounding in it.
 A weight is a quotient in 64 bits rounded to fp32 once: off by 2^-24 of it, and by 2^-150 where it has no normal number;
 the bound is twice that."""
 import numpy as np
@@ -17,10 +18,10 @@ def reference(z, k, sigmoid=False, bias=None, groups=1, top_groups=1, best=1):
     that of the scores."""
     T, E = z.shape
     z64 = z.astype(np.float64)
-    with np.errstate(over="ignore"):
+    with np.errstate(over="ignore", invalid="ignore"):  # (a row without experts has no scores)
         p = 1 / (1 + np.exp(-z64)) if sigmoid else np.exp(z64 - z64.max(1, keepdims=True))
-    if not sigmoid:
-        p /= p.sum(1, keepdims=True)
+        if not sigmoid:
+            p /= p.sum(1, keepdims=True)
     if bias is not None:
         c = p + bias.astype(np.float64)
     else:
@@ -29,8 +30,8 @@ def reference(z, k, sigmoid=False, bias=None, groups=1, top_groups=1, best=1):
     if bias is not None:
         c[:, bias == -np.inf] = -np.inf
     if top_groups < groups:
-        by = -np.sort(-c.reshape(T, groups, -1), axis=2)
-        score = by[:, :, :best].sum(2)
+        by = -np.sort(-c.reshape(T, groups, -1), axis=2)[:, :, :best]
+        score = np.where((by == -np.inf).any(2), -np.inf, by.sum(2, where=by > -np.inf))  # (an infinite bias and a masked one)
         place = np.empty((T, groups), int)
         np.put_along_axis(place, np.argsort(-score, axis=1, kind="stable"), np.arange(groups)[None], 1)
         c = np.where(np.repeat(place < top_groups, E // groups, axis=1), c, -np.inf)
@@ -109,3 +110,29 @@ def test_biases_beside_which_scores_vanish(gpu, T, E, sigmoid, groups, top_group
     bias[bias == 0] = 0.125  # (a score beside no bias is one)
     case(f"route biases T={T} E={E} sigmoid={sigmoid} groups={groups}/{top_groups}")
     check(gpu, z, 9, sigmoid=sigmoid, bias=bias, groups=groups, top_groups=top_groups)
+
+
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("E,groups,top_groups", [(40, 8, 3), (256, 8, 4), (24, 24, 5), (1024, 64, 9), (520, 4, 1)])
+@pytest.mark.parametrize("T", [7, 2050, 16387])
+def test_groups_of_which_a_mask_leaves_less_than_two(gpu, T, E, groups, top_groups, sigmoid, bias):
+    """The sum of a group's two largest scores is -inf where it has one: any other group comes first, and of such groups
+    the first ones."""
+    rng = np.random.default_rng(T + E + 2 * sigmoid + bias)
+    # (all below 0, where no two pairs of sigmoids have one sum)
+    z = (rng.permuted(np.tile(np.arange(E), (T, 1)), axis=1) % 61 / 8.0 - 7.75).astype(np.float32)
+    left = rng.integers(0, 4, (T, groups, 1))  # of each group
+    order = rng.permuted(np.tile(np.arange(E // groups), (T, groups, 1)), axis=2)
+    z[(order >= left).reshape(T, E)] = -np.inf
+    z[0] = -np.inf
+    z[0, E // groups * (groups - 1)] = 3.0  # one expert in all, of the last group
+    z[1] = -np.inf
+    z[1, :E // groups] = 1.0
+    b = None
+    if bias:
+        b = (2 * rng.standard_normal(E)).astype(np.float32)
+        b[E // 2] = np.inf
+        b[E - 1] = -np.inf
+    case(f"route groups T={T} E={E} groups={groups}/{top_groups} sigmoid={sigmoid} bias={bias}")
+    check(gpu, z, 6, sigmoid=sigmoid, bias=b, groups=groups, top_groups=top_groups, best=2)
