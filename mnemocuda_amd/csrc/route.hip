@@ -5,7 +5,7 @@
 //   a group of experts scores the sum of its one or two largest c (-inf where it has too few); the best groups are kept
 //   the k largest c among them are chosen, ties to the lower index
 //   w = s of the chosen, / their sum where asked for, * scale
-// Without a bias, and with groups that score one expert, c grows with z: the choice is made among the logits.
+// Without a bias, and with groups that score one expert or are all kept, c grows with z: the choice is made among the logits.
 //
 // L lanes (16, 32 or 64) look after a token and hold its experts in registers, a group's in adjacent lanes.
 // An expert's place in the order is one number, its key: c with the lowest ten bits giving way to the index.  Scores
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
             b1 = fmax(b1, o1);
         }
         // (of two experts of which one is masked: -inf, whatever the other scores)
-        const double score = a.best == 1 || a.per_group == 1 ? b1 : b2 > -INFINITY ? b1 + b2 : -INFINITY;
+        const double score = a.best == 1 ? b1 : b2 > -INFINITY ? b1 + b2 : -INFINITY;
         const double gkey = g < a.n_groups ? make_key(fmax(score, kNone), g) : kNone;
         int better = 0;
         for (int o = 0; o < a.n_groups; o++)
@@ -230,6 +230,7 @@ static void launch_lanes(const RouteArgs &a, hipStream_t s) {
 
 int launch_route(RouteArgs a, hipStream_t s) {
     a.per_group = a.n_experts / a.n_groups;
+    if (a.per_group == 1) a.best = 1;
     auto spread = [&](int lanes) {  // a power of two of lanes per group
         a.lanes_log = 0;
         while ((2 << a.lanes_log) * a.n_groups <= lanes) a.lanes_log++;

@@ -14,8 +14,8 @@ pytestmark = pytest.mark.gpu
 
 
 def reference(z, k, sigmoid=False, bias=None, groups=1, top_groups=1, best=1):
-    """(ids, renormalised weights).  Without a bias the order is that of the logits, with groups that score two experts
-    that of the scores."""
+    """(ids, renormalised weights).  Without a bias the order is that of the logits, but with groups that are left out by
+    the sum of two experts that of the scores."""
     T, E = z.shape
     z64 = z.astype(np.float64)
     with np.errstate(over="ignore", invalid="ignore"):  # (a row without experts has no scores)
@@ -25,7 +25,7 @@ def reference(z, k, sigmoid=False, bias=None, groups=1, top_groups=1, best=1):
     if bias is not None:
         c = p + bias.astype(np.float64)
     else:
-        c = p.copy() if best == 2 and top_groups < groups else z64.copy()
+        c = p.copy() if best == 2 and top_groups < groups < E else z64.copy()
     c[z64 == -np.inf] = -np.inf
     if bias is not None:
         c[:, bias == -np.inf] = -np.inf
@@ -136,3 +136,20 @@ def test_groups_of_which_a_mask_leaves_less_than_two(gpu, T, E, groups, top_grou
         b[E - 1] = -np.inf
     case(f"route groups T={T} E={E} groups={groups}/{top_groups} sigmoid={sigmoid} bias={bias}")
     check(gpu, z, 6, sigmoid=sigmoid, bias=b, groups=groups, top_groups=top_groups, best=2)
+
+
+@pytest.mark.parametrize("T", [5, 2050, 16387])
+@pytest.mark.parametrize("bias,groups,top_groups,best,want", [
+    (False, 1, 1, 1, [5, 2, 6]), (False, 4, 3, 1, [5, 2, 6]), (False, 4, 4, 2, [5, 2, 6]), (False, 8, 5, 2, [5, 2, 6]),
+    (True, 1, 1, 1, [0, 2, 5]), (True, 4, 3, 1, [0, 2, 5]), (False, 4, 3, 2, [0, 5, 6])])
+def test_sigmoids_that_are_one(gpu, T, bias, groups, top_groups, best, want):
+    """exp(-38) is below 2^-54, so sigmoids of 38 and more are 1 in 64 bits: the logits tell them apart where they are the
+    order, and the index where c is."""
+    z = np.full((T, 8), -3.0, np.float32)
+    z[:, 0], z[:, 2], z[:, 5], z[:, 6] = 38.0, 40.0, 41.0, 39.0
+    z[:, 4] = 2.0
+    z[:, 7] = 1.0
+    case(f"route ones T={T} bias={bias} groups={groups}/{top_groups} best={best}")
+    b = np.zeros(8, np.float32) if bias else None
+    assert reference(z, 3, True, b, groups, top_groups, best)[0][0].tolist() == want
+    check(gpu, z, 3, sigmoid=True, bias=b, groups=groups, top_groups=top_groups, best=best)
