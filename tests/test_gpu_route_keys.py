@@ -153,3 +153,31 @@ def test_sigmoids_that_are_one(gpu, T, bias, groups, top_groups, best, want):
     b = np.zeros(8, np.float32) if bias else None
     assert reference(z, 3, True, b, groups, top_groups, best)[0][0].tolist() == want
     check(gpu, z, 3, sigmoid=True, bias=b, groups=groups, top_groups=top_groups, best=best)
+
+
+@pytest.mark.parametrize("sigmoid", [True, False])
+@pytest.mark.parametrize("seed", range(3))
+def test_scores_hold_49_bits(gpu, seed, sigmoid):
+    """A score s (a sigmoid, or the softmax of it and 0) less its fp32 value, which is exact, lies between fp32 biases just
+    below and above: exp is off by 2^-50 of it and what follows it by five roundings of 2^-53 or less, together less
+    than 2^-49 of s, and the biases are further away."""
+    rng = np.random.default_rng(seed)
+    T, E = 340, 1023
+    zt = rng.uniform(-30.0, 0.0 if not sigmoid else 12.0, T).astype(np.float32)
+    e = np.exp(-np.abs(zt.astype(np.longdouble)))
+    s = np.where(zt >= 0, np.longdouble(1), e) / (1 + e)
+    rest = s - s.astype(np.float32).astype(np.longdouble)
+    up, down = np.float32(np.inf), np.float32(-np.inf)
+    hi = np.nextafter((rest + s * 2.0 ** -49).astype(np.float32), up)
+    lo = np.nextafter((rest - s * 2.0 ** -49).astype(np.float32), down)
+    z, bias = np.full((T, E), -np.inf, np.float32), np.zeros(E, np.float32)
+    at = rng.permutation(E - 3)[:3 * T].reshape(T, 3)  # of each token: below, s, above
+    np.put_along_axis(z, at, np.stack([np.full(T, -200.0), zt, np.full(T, -200.0)], 1).astype(np.float32), 1)
+    bias[at] = np.stack([lo, -s.astype(np.float32), hi], 1)
+    if not sigmoid:
+        z[:, E - 1] = 0.0  # in the sum, and never chosen
+        bias[E - 1] = -np.inf
+    case(f"route 49 bits seed={seed} sigmoid={sigmoid}")
+    idx, w = torch.empty((T, 4), dtype=torch.int32, device="cuda"), torch.empty((T, 4), device="cuda")
+    gpu.ops.moe_route(dev(z), idx, w, sigmoid, dev(bias))
+    assert np.array_equal(host(idx), np.concatenate([at[:, ::-1], np.full((T, 1), -1)], 1))
