@@ -1,13 +1,10 @@
 // gemm_ops.hpp -- operand conversions, matrix instruction and LDS copies shared by the plain
 // GEMM (gemm.hip) and the grouped expert GEMM (gemm_grouped.hip).
 #pragma once
+#include "mfma_types.hpp"
 #include "mnemo_common.hpp"
 
 namespace mnemo {
-
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef float f4 __attribute__((ext_vector_type(4)));
 
 // ------------------------------------------------------------------ operand conversions
 // Byte selectors placing bytes (0, 1) / (2, 3) of a dword under the f16 exponent byte 0x64:

@@ -48,11 +48,12 @@ constexpr float kSlack = 5.0f, kLift = 9.0f;  // powers of two
 constexpr float kLeastScale = -98.0f, kUnit = 0x1p-16f, kMost = 0x1p14f, kMostSum = 0x1p-82f;
 constexpr int kStep = 64;                     // positions
 // The shares are counted in units: a step is one, and what a tile takes beside its steps (its queries, its output) are
-// a few, `cost`.  A share has kLeast or more, as far as there are any: one token behind 500 positions takes 10.8, 11.6 and
-// 12.5 us with 1, 2 and 3, five behind 3000 17.5, 16.0 and 16.9.
+// a few, `cost`.  A share has kLeast or more, as far as there are any: one token behind 500 positions takes 11.3, 12.1 and
+// 12.8 us with 1, 2 and 3, five behind 3000 18.0, 16.6 and 17.5.
 constexpr int kLeast = 2;
-// Where one sequence alone has tokens, and no workgroup gets more than kUneven units, or half, above the average, whole tiles are
-// dealt out instead, in kRounds at most: nothing is cut, nothing merged.  1300 tokens of 64 heads of 128 take 81 us and 87 in
+// Where one sequence alone has tokens, of a table of 64 rows at most, and none of the 64 workgroups that are looked at gets more
+// than kUneven units, or half, above the average, whole tiles are dealt out instead, in kRounds at most: nothing is cut,
+// nothing merged.  1300 tokens of 64 heads of 128 take 81 us and 87 in
 // shares, 2000 133 and 155, 4096 473 and 498; where it is less even 600 47 and 45, 1000 67 and 65.
 constexpr int kUneven = 8, kRounds = 8;
 
@@ -159,7 +160,7 @@ __device__ __forceinline__ Plan make_plan(const PagedPromptArgs &a, int groups) 
     p.alone = -1;
     const uint64_t some = __ballot(sum > 0);
     const int mean = p.total / groups;
-    if (p.per == 1 && __popcll(some) == 1 && mean >= kUneven) {  // (a sample of the workgroups, with the first and the last)
+    if (p.per == 1 && __popcll(some) == 1 && mean >= kUneven) {  // (64 of the workgroups, the first and the last among them)
         const int seq = __ffsll((unsigned long long)some) - 1;
         const Seq s = seq_of(a, seq);
         const int each = tiles_of(s, a.tl), g = lane_id() * (groups - 1) / 63;
@@ -825,10 +826,13 @@ int launch_rows(const PagedPromptArgs &a, hipStream_t s) {
     return check_launch("paged_attention_prompt");
 }
 // Waves of 16 rows are done with a step sooner, of 32 read each operand from LDS half as often: 3 to 6 tokens of 5 sequences
-// take 23 us by 16 and 29 by 32, 8 behind 100,000 positions 66 and 71, a prompt of 4096 592 and 500, 300 tokens 33 and 36,
-// but chunks of 400 behind long ones 2.31 and 1.89 ms.  So rows of one tile a sequence, as the average is, are taken by 16.  At
-// head_dim 256 the registers hold no more than 16; at 64 they hold four waves a SIMD of them, which is best for all (60 times 3
-// tokens 104 us and 141 by 32, 4096 299 either way), but int8 rows of 64 are too few words for 8 waves to copy.
+// take 23 us by 16 and 30 by 32, 8 behind 100,000 positions 67 and 72, 300 to 512 behind 6000 to 30,000 1.93 and 1.72 ms (int8 1.99
+// and 1.88), and of prompts alone, in whole tiles, 300 tokens 26 and 31 us, 1000 51 and 67, 2000 146 and 132, 4096 531 and 465.  So
+// rows of one tile a sequence, as the average is, are taken by 16; the host knows the table's rows, not how many of them have
+// tokens, and many idle ones lead to 16 as well (512 tokens behind 30,000: 830 us, in a table of 64 rows 913; int8 994 and
+// 1033).  At head_dim 256 the registers hold no more than 16; at 64 they hold four waves a SIMD of them, which is best for all (60
+// times 3 tokens behind 2000 34 us and 43 by 32, a prompt of 4096 291 and 286), but int8 rows of 64 are too few words for 8 waves
+// to copy.
 template <int KV, int HD>
 int launch_shape(const PagedPromptArgs &a, hipStream_t s) {
     if constexpr (HD == 256 || (HD == 64 && KV == kKvF16)) return launch_rows<KV, HD, 1>(a, s);
@@ -843,11 +847,13 @@ size_t paged_prompt_workspace_bytes(int hd) {
 }
 
 int launch_paged_prompt(PagedPromptArgs a, hipStream_t s) {
-    // tokens of a tile: a power of two, whose rows fill the tile as far as they can
+    // Tokens of a tile: a power of two, whose rows fill the tile as far as they can.  Where gqa is no power of two rows stay
+    // idle, and are multiplied all the same: 4096 tokens of 8 KV heads reach 1136 TFLOP/s (two products for each) with 8 query
+    // heads for each, 993 with 6 (96 rows of 128), 834 with 5 (80), 749 with 9 (72).
     a.tl = 0;
     while ((2 << a.tl) * a.gqa <= kRows) a.tl++;
-    // 4096 tokens of 32 heads of 256 take 527 us at 2, 492 at 3; of 64 heads of 128, int8, 631 and 639, of 12 of 64, mixed, 33.4
-    // and 34.1 (2000 of 64 heads of 128: 239 with none)
+    // three prompts of 700 tokens of 32 heads of 256 take 106, 90 and 84 us with 1, 2 and 3, of 64 heads of 128 97, 87 and 85, a mixed
+    // step of 12 heads of 64 29.8, 29.4 and 30.8 (one prompt in whole tiles is the same with all)
     a.cost = a.c.hd == 256 ? 3 : 2;
     if (a.c.kv_type == kKvF16)
         return a.c.hd == 64 ? launch_shape<kKvF16, 64>(a, s) : a.c.hd == 128 ? launch_shape<kKvF16, 128>(a, s)
