@@ -10,7 +10,7 @@
 // Bound by memory: x, base and out once, each adapter once per tile.  3001 tokens of ranks to 32 (bf16, 4096 to 8192 features, 248 MB)
 // take 70 us with nothing in the caches, 8000 tokens 145 (4.5 TB/s; a copy reaches 5.2), of which the first launch, x, is a
 // third.  Few tokens are bound by what a launch waits for in turn, ids, ranks, words and the other launch: one token 9 us,
-// 61 of as many adapters 24, where lines of B of which a low rank has a part are read whole as well.  Asking for B before v
+// 61 of 40 adapters 24, where lines of B of which a low rank has a part are read whole as well.  Asking for B before v
 // is known costs more in registers than it hides (24 and 23, but one token 9 and 9.5, 3001 70 and 74).  High ranks of many
 // tokens are bound by A and B, which every tile reads again from the L2 caches: 3001 tokens of rank 200 take 192 us, 4.9 TB/s of
 // them (the next words of B asked for ahead of the products: 193 f16, 225 bf16, for spilled registers).
@@ -331,7 +331,7 @@ static int launch_typed(const LoraArgs &a, hipStream_t s) {
     // 200 of 256 192 by 256 and 221 by 64: a wave forms its operands of v once.
     const int per_wave = tiles < 64 ? 64 : a.max_rank <= 64 ? 128 : 256, m_blocks = (a.M + kLoExpandWaves * per_wave - 1) / (kLoExpandWaves * per_wave);
     // a tile's adapters by workgroups of their own, as far as the chip has room for them: 1024 workgroups of either launch are at
-    // work at once (61 tokens of 61 adapters take 24 us with room for 1024 of the second, 26 for 2048, 26 for 768)
+    // work at once (61 tokens of 40 adapters take 24 us with room for 1024 of the second, 26 for 2048, 26 for 768)
     auto apart = [&](long long groups, long long room) {
         long long z = room / groups;
         z = z < kLoTile ? z : kLoTile;
