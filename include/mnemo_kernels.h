@@ -497,8 +497,9 @@ int mnemo_paged_attention_prompt(const float *q, const void *k_pages, const void
  * of the logits, which c grows with: sigmoids of 38 and 40, both 1 in 64 bits, are told apart.  Else c is
  * formed in 64 bits, and those that agree in the first 42 of their fraction are a tie; so a bias of zeros
  * may choose otherwise than none does.  An expert whose logit or bias is -inf is never chosen; a slot
- * that no expert is left for gets id -1 and weight 0 (mnemo_moe_prefill skips it).  A token whose scores hold a NaN (of a logit, or the bias of an expert whose logit is not
- * -inf, that is none, or of a logit of +inf with score 0) gets ids -1 and weights NaN.
+ * that no expert is left for gets id -1 and weight 0 (mnemo_moe_prefill skips it).  A token whose scores
+ * hold a NaN (of a logit, or of the bias of an expert whose logit is not -inf, or of a logit of +inf with
+ * score 0) gets ids -1 and weights NaN.
  * k <= 16, k <= n_experts <= 1024 (mnemo_moe_prefill takes 512), n_experts % n_groups == 0, n_groups <= 64,
  * n_tokens * k <= 4,194,304. */
 int mnemo_moe_route(const float *logits, int n_tokens, int n_experts, int score, const float *bias,
